@@ -57,6 +57,23 @@ extern "C" {
 #define VX_MAX_CANDIDATES     1048575 /* per image; sort key holds the index in 20 bits  */
 #define VX_MAX_COORDINATE     2048  /* postprocess/utils/nms.py:94 */
 
+/* bits of the token-model operators' status words */
+#define VX_STATUS_BAD_TOKEN   32    /* a token id at or beyond the number of table rows / logits (drafted tokens: or below 0) */
+#define VX_STATUS_EMPTY_ROW   64    /* every logit of a row that is used is masked (-inf): there is nothing to draw */
+
+/* element types of the token-model operators */
+#define VX_DTYPE_F32          0
+#define VX_DTYPE_F16          1
+#define VX_DTYPE_BF16         2
+
+#define VX_MAX_TOKENS         1073741823 /* tokens of one embedding call, rows of one quantisation */
+#define VX_MAX_VOCAB          1073741823 /* rows of an embedding table, logits of a row   */
+#define VX_MAX_TOKEN_WIDTH    1048576    /* columns of an embedding table                 */
+#define VX_MAX_I8_DEPTH       131072     /* K of the 8-bit product: 127 * 127 * K fits 32 bits */
+#define VX_MAX_LINEAR_ROWS    4194240    /* M and N of the 8-bit product                  */
+#define VX_MAX_DRAFTS         64         /* drafted tokens of a sequence                  */
+#define VX_MAX_VERIFY_BATCH   65535      /* sequences of one verification                 */
+
 #define VX_MAX_FORMAT_COLS    64    /* columns of one formatted result row                */
 
 /* use_threshold argument of the decoders: bit 0 = apply the score threshold.  vx_yolo_fused_decode also takes
@@ -315,6 +332,74 @@ int vx_yolo_pipeline_step(const uint8_t *d_img, float *d_norm, int Hs, int Ws, c
 int vx_format_results(const float *d_src, const int32_t *d_counts, int B, int capacity, int D,
                       const int32_t *h_cols, const uint8_t *h_kinds, int n_cols,
                       const float *d_image_wh, float *d_dst, int32_t *d_total, void *stream);
+
+/* ================================================================ token models
+ * The two ends of a language model around its network: token ids -> scaled vectors (the counterpart of the image
+ * pre-process), the 8-bit product of a vocabulary head or a 1x1 convolution, and the verification of drafted tokens
+ * (the counterpart of the softmax post-process).  No reference counterpart.  Tensors are row-major; `dtype` is a
+ * VX_DTYPE_*; strides are in elements.  No atomics on floating values: the same inputs give the same bits.
+ *
+ * ---------------------------------------------------------------- embedding lookup with scaling
+ *   d_out[t,0..D) = scale * d_table[ids[t],0..D)      (fp32 product, rounded once to dtype)
+ * d_ids: id_bytes 4 (i32) or 8 (i64).  An id below 0 is padding: a row of zeros.  An id >= n_rows: a row of zeros and
+ * VX_STATUS_BAD_TOKEN ORed into *d_status (may be NULL; the caller zeroes it).  d_out is [n_tokens, D] contiguous, of the
+ * table's type.  Pointers are aligned to their element. */
+int vx_embed_tokens(const void *d_ids, int id_bytes, int64_t n_tokens, const void *d_table, int64_t n_rows, int D,
+                    int64_t table_stride, int dtype, float scale, void *d_out, int32_t *d_status, void *stream);
+
+/* Its gradient: d_grad_table[v,0..D) = scale * sum over the t with ids[t] == v of d_grad_out[t,0..D).
+ * fp32 sums in a fixed order.  accumulate == 0: every one of the n_rows rows is written (zeros where no id points).
+ * accumulate != 0: only rows that some id points to are read and written, d_grad_table[v] + the sum above, rounded once.
+ * Padding ids and ids >= n_rows contribute nothing (the latter set VX_STATUS_BAD_TOKEN, as above).
+ * table_dtype: grad_dtype or VX_DTYPE_F32.  The workspace is 256-byte aligned. */
+size_t vx_embed_tokens_grad_workspace_bytes(int64_t n_tokens, int64_t n_rows, int D);
+int vx_embed_tokens_grad(const void *d_ids, int id_bytes, int64_t n_tokens, const void *d_grad_out, int grad_dtype,
+                         int64_t n_rows, int D, float scale, void *d_grad_table, int table_dtype, int accumulate,
+                         int32_t *d_status, void *d_workspace, size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------- 8-bit products
+ * Rows of d_x [M,K] to 8 bits: amax = max_k |x[m,k]|, d_scale[m] = amax / 127, d_q[m,k] = rint(127 x[m,k] / amax) exactly
+ * (ties to even); columns K .. q_stride-1 of d_q are zeroed.  amax 0: q = 0, scale 0.  A row that holds a NaN or an
+ * infinity: q = 0, scale NaN, so every product of the row is NaN. */
+int vx_quantize_rows_i8(const void *d_x, int dtype, int64_t M, int K, int64_t x_stride, int8_t *d_q, int64_t q_stride,
+                        float *d_scale, void *stream);
+
+/* d_out[m,n] = d_scale[m] * d_w_scale[n] * (sum_k d_q[m,k] d_w[n,k]) (+ d_bias[n]): the sum exact in 32-bit integers, the
+ * rest fp32 (the two scales first), rounded once to out_dtype.  d_q [M,K] and d_w [N,K] hold any 8-bit integers.
+ * d_bias f32[N] or NULL.  The workspace is 256-byte aligned; K <= VX_MAX_I8_DEPTH. */
+size_t vx_linear_i8_workspace_bytes(int64_t M, int64_t N, int K);
+int vx_linear_i8(const int8_t *d_q, int64_t q_stride, const float *d_scale, int64_t M, const int8_t *d_w, int64_t w_stride,
+                 const float *d_w_scale, int64_t N, int K, const float *d_bias, void *d_out, int out_dtype,
+                 int64_t out_stride, void *d_workspace, size_t workspace_bytes, void *stream);
+
+/* vx_quantize_rows_i8 of d_x followed by vx_linear_i8: the same bits as the two calls. */
+size_t vx_linear_w8a8_workspace_bytes(int64_t M, int64_t N, int K);
+int vx_linear_w8a8(const void *d_x, int x_dtype, int64_t x_stride, int64_t M, const int8_t *d_w, int64_t w_stride,
+                   const float *d_w_scale, int64_t N, int K, const float *d_bias, void *d_out, int out_dtype,
+                   int64_t out_stride, void *d_workspace, size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------- verification of drafted tokens
+ * Sequence b has n_b = clamp(d_draft_lens[b], 0, K) drafted tokens x_j = d_draft_tokens[b,j] (d_draft_lens NULL: K), target
+ * logits in rows 0 .. n_b of d_target [B, K+1, V] and draft logits in rows 0 .. n_b-1 of d_draft [B, K, V].  With
+ * p_j = softmax(target[b,j] / T_b) and q_j = softmax(draft[b,j] / T_b) (d_draft NULL: 1 at x_j, 0 elsewhere):
+ *   d_accept[b,j] = min(1, p_j(x_j) / q_j(x_j)) for j < n_b (0 where p_j(x_j) is 0), 0 for j >= n_b
+ *   x_j is accepted iff u_{b,j} q_j(x_j) < p_j(x_j) and all before it are; n = the number accepted
+ *   the token behind them is the first i with sum_{i' <= i} r_i' > u_{b,K} sum r, r = max(0, p_n - q_n) when x_n was
+ *   rejected, r = p_n when n = n_b
+ *   d_tokens[b,0..n) = x_0 .. x_{n-1}, d_tokens[b,n] = that token, -1 behind it; d_counts[b] = n + 1
+ * d_temperature[b] not above 0: greedy -- x_j is accepted iff it is the first arg-max of target row j (d_accept 1 or 0), the
+ * token behind is the arg-max of row n; the draft logits and d_uniforms are not used.  d_uniforms [B, K+1] in [0, 1).
+ * -inf masks a token (in either distribution).  K = 0 draws one token from each row 0.
+ * Everything is fp64 from the logits on.  d_status[b] (written, not ORed): VX_STATUS_NAN a NaN or +inf in a row that is used,
+ * VX_STATUS_EMPTY_ROW all of such a row is -inf, VX_STATUS_BAD_TOKEN a drafted token outside [0, V) (it is rejected).  A
+ * draft is rejected at an invalid row; where the row that is drawn from is invalid, the token behind is -1.
+ * Rows behind n_b, and their drafted tokens, are not read.  The workspace is 256-byte aligned. */
+size_t vx_verify_drafts_workspace_bytes(int B, int K, int V);
+int vx_verify_drafts(const void *d_target, int64_t target_seq_stride, int64_t target_row_stride, const void *d_draft,
+                     int64_t draft_seq_stride, int64_t draft_row_stride, int dtype, const int64_t *d_draft_tokens,
+                     const int32_t *d_draft_lens, const float *d_uniforms, const float *d_temperature, int B, int K, int V,
+                     int64_t *d_tokens, int32_t *d_counts, float *d_accept, int32_t *d_status, void *d_workspace,
+                     size_t workspace_bytes, void *stream);
 
 /* ---------------------------------------------------------------- measurement hooks (no reference
  * counterpart; bench.py's roofline leg).  When enabled, every kernel family launched by this library is

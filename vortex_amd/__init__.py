@@ -10,6 +10,8 @@ reference's own nn.Module API for that path:
     prior.PriorBoxDecoder / PriorBoxPostProcess
     predictor.BasePredictor / create_predictor / get_prediction_results
     detr.DETRPostProcess
+    preprocess.TokenEmbedding / heads.Int8Head / postprocess.DraftVerifyPostProcess   (the two ends of a token model:
+                embedding with its gradient, 8-bit head, verification of drafted tokens)
     runtime.resize_batch / format_detections / adjust_coordinates / InferenceHelper
     parallel.shard_batch / allgather_detections
     YoloV3PipelineStep                   (pre-process + fused post-process in ONE library call: vx_yolo_pipeline_step)
@@ -17,11 +19,11 @@ reference's own nn.Module API for that path:
     export                               (torch.library custom ops + ONNX symbolic; import on demand)
 """
 from . import _lib, ops, runtime  # noqa: F401
-from .preprocess import Normalize, FlipNormalize, get_preprocess  # noqa: F401
-from .heads import YoloV3Layer, YoloV3HeadDecode, yolo_feature_maps  # noqa: F401
+from .preprocess import Normalize, FlipNormalize, TokenEmbedding, get_preprocess  # noqa: F401
+from .heads import YoloV3Layer, YoloV3HeadDecode, Int8Head, yolo_feature_maps  # noqa: F401
 from .postprocess import (YoloV3Decoder, BatchedNMS, NMS, NoNMS, BasicNMSPostProcess,  # noqa: F401
                           BatchedNMSPostProcess, YoloV3PostProcess, YoloV3FusedPostProcess,
-                          NoOpPostProcess, SoftmaxPostProcess, batched_nms, get_postprocess)
+                          NoOpPostProcess, SoftmaxPostProcess, DraftVerifyPostProcess, batched_nms, get_postprocess)
 from .prior import PriorBoxDecoder, PriorBoxPostProcess  # noqa: F401
 from .detr import DETRPostProcess  # noqa: F401
 from .predictor import BasePredictor, create_predictor, get_prediction_results  # noqa: F401

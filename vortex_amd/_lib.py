@@ -17,6 +17,13 @@ VX_STATUS_BAD_CLASS = 2
 VX_STATUS_RANGE = 4
 VX_STATUS_DEFERRED = 8
 VX_STATUS_RANGE2 = 16
+VX_STATUS_BAD_TOKEN = 32
+VX_STATUS_EMPTY_ROW = 64
+VX_DTYPE_F32 = 0
+VX_DTYPE_F16 = 1
+VX_DTYPE_BF16 = 2
+VX_MAX_I8_DEPTH = 131072
+VX_MAX_DRAFTS = 64
 VX_MAX_CLASSES = 4096
 VX_MAX_CANDIDATES = 1048575
 VX_RESIZE_STRETCH = 0
@@ -73,6 +80,22 @@ _SIGNATURES = {
                              c_int, c_void_p]),
     "vx_format_results": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, ctypes.POINTER(ctypes.c_int32),
                                   ctypes.POINTER(ctypes.c_uint8), c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "vx_embed_tokens": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int64, c_int, c_int64, c_int, c_float, c_void_p,
+                                c_void_p, c_void_p]),
+    "vx_embed_tokens_grad_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int]),
+    "vx_embed_tokens_grad": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_int, c_int64, c_int, c_float, c_void_p, c_int,
+                                     c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "vx_quantize_rows_i8": (c_int, [c_void_p, c_int, c_int64, c_int, c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
+    "vx_linear_i8_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int]),
+    "vx_linear_i8": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p,
+                             c_void_p, c_int, c_int64, c_void_p, c_size_t, c_void_p]),
+    "vx_linear_w8a8_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int]),
+    "vx_linear_w8a8": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p,
+                               c_void_p, c_int, c_int64, c_void_p, c_size_t, c_void_p]),
+    "vx_verify_drafts_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "vx_verify_drafts": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p,
+                                 c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
+                                 c_void_p]),
     "vx_profile_enable": (c_int, [c_int]),
     "vx_profile_select": (c_int, [ctypes.c_uint]),
     "vx_profile_disable": (c_int, []),

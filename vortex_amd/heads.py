@@ -77,3 +77,47 @@ class YoloV3HeadDecode(nn.Module):
             raise RuntimeError("vx_yolo_head_decode3 expects 3 anchors x (5 + %d) channels, got %s"
                                % (self.n_classes, tuple(h1.shape),))
         return ops.yolo_head_decode3((h1, h2, h3), self.img_size, self.anchors, out=out)
+
+
+class Int8Head(nn.Module):
+    """The last linear layer of a network (a vocabulary head, a classifier in front of SoftmaxPostProcess) or the 1x1
+    convolution in front of a YoloV3Layer as an 8-bit product: weights quantised once, a scale for each output channel;
+    inputs quantised on the way in, a scale for each token (cell).  Inference only: the result carries no gradient.
+
+        head = Int8Head.from_module(linear)            # nn.Linear: [..., K] -> [..., N]
+        head = Int8Head.from_module(conv)              # nn.Conv2d, 1x1: [B, K, H, W] -> [B, N, H, W]"""
+
+    def __init__(self, qweight: torch.Tensor, weight_scale: torch.Tensor, bias: torch.Tensor = None,
+                 out_dtype: torch.dtype = None, channels_first: bool = False):
+        super().__init__()
+        self.register_buffer("qweight", qweight)
+        self.register_buffer("weight_scale", weight_scale)
+        self.register_buffer("bias", bias)
+        self.out_dtype, self.channels_first = out_dtype, channels_first
+
+    def _apply(self, fn, *a, **k):
+        # .half() / .bfloat16() are about the network's activations: the scales and the bias stay fp32
+        keep = {n: getattr(self, n) for n in ("weight_scale", "bias")}
+        super()._apply(fn, *a, **k)
+        for n, t in keep.items():
+            if t is not None and getattr(self, n).dtype != t.dtype:
+                setattr(self, n, t.to(getattr(self, n).device))
+        return self
+
+    @classmethod
+    @torch.no_grad()
+    def from_module(cls, module: nn.Module, out_dtype: torch.dtype = None) -> "Int8Head":
+        conv = isinstance(module, nn.Conv2d)
+        if conv:
+            one = all(tuple(getattr(module, n)) == (1, 1) for n in ("kernel_size", "stride", "dilation"))
+            if not one or module.groups != 1 or tuple(module.padding) != (0, 0):
+                raise RuntimeError("Int8Head takes a 1x1 convolution without stride, padding or groups, got %s" % module)
+        elif not isinstance(module, nn.Linear):
+            raise RuntimeError("Int8Head takes nn.Linear or a 1x1 nn.Conv2d, got %s" % type(module).__name__)
+        q, s = ops.quantize_rows_i8(module.weight.detach().flatten(1))
+        return cls(q, s, module.bias.detach().float() if module.bias is not None else None, out_dtype, conv)
+
+    def forward(self, input: torch.Tensor) -> torch.Tensor:
+        x = input.permute(0, 2, 3, 1) if self.channels_first else input
+        y = ops.linear_w8a8(x, self.qweight, self.weight_scale, self.bias, self.out_dtype)
+        return y.permute(0, 3, 1, 2) if self.channels_first else y

@@ -386,6 +386,37 @@ class SoftmaxPostProcess(nn.Module):
         return out.unsqueeze(2) if self.keepdim else out
 
 
+class DraftVerifyPostProcess(nn.Module):
+    """Post-process of a token model that was given drafted tokens: how many of them the target's distribution accepts,
+    and the token behind them (speculative sampling; temperature 0 is greedy, no drafts at all is plain sampling).
+
+        forward(logits[B,K+1,V], draft_tokens i64[B,K], uniforms f32[B,K+1], ...) -> tuple of i64[n_i], the new tokens of
+        each sequence (the accepted drafts and one more): one D2H read of the counts, like the detection post-processes
+        forward_device(...) -> (tokens i64[B,K+1], counts i32[B], accept f32[B,K], status i32[B]) without one
+
+    A NaN in the logits raises ValueError (as the detection post-processes do), and so does a row whose every token is
+    masked; a drafted token outside the vocabulary raises VortexHipError.  See ops.verify_drafts."""
+
+    def __init__(self, temperature: float = 1.0):
+        super().__init__()
+        self.temperature = temperature
+
+    def forward_device(self, input: torch.Tensor, draft_tokens: torch.Tensor, uniforms: torch.Tensor,
+                       draft_logits: Optional[torch.Tensor] = None, draft_lens: Optional[torch.Tensor] = None, temperature=None):
+        return ops.verify_drafts(input, draft_tokens, uniforms, draft_logits, draft_lens,
+                                 self.temperature if temperature is None else temperature)
+
+    @torch.no_grad()
+    def forward(self, input: torch.Tensor, draft_tokens: torch.Tensor, uniforms: torch.Tensor,
+                draft_logits: Optional[torch.Tensor] = None, draft_lens: Optional[torch.Tensor] = None,
+                temperature=None) -> Tuple[torch.Tensor, ...]:
+        tokens, counts, _, status = self.forward_device(input, draft_tokens, uniforms, draft_logits, draft_lens, temperature)
+        counts, status = torch.stack((counts, status)).tolist()
+        for s in status:
+            ops.raise_on_status(s)
+        return tuple(tokens[b, :n] for b, n in enumerate(counts))
+
+
 class NoOpPostProcess(nn.Module):
     def __init__(self):
         super(NoOpPostProcess, self).__init__()

@@ -61,6 +61,37 @@ class FlipNormalize(Normalize):
         return super().forward(input)
 
 
+class _EmbedTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, weight, scale):
+        ctx.save_for_backward(ids)
+        ctx.n_rows, ctx.scale = weight.size(0), scale
+        return ops.embed_tokens(ids, weight, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        ids, = ctx.saved_tensors
+        return None, ops.embed_tokens_grad(ids, grad, ctx.n_rows, ctx.scale), None
+
+
+class TokenEmbedding(nn.Module):
+    """The pre-process of a token model: integer ids -> the network's input vectors, scale * weight[ids] (what Normalize
+    is for images).  An id below 0 is padding: a row of zeros that gets no gradient.  The gradient of `weight` is summed in
+    fp32 over the tokens in a fixed order (vx_embed_tokens_grad), dense, in the type of `weight`."""
+
+    def __init__(self, n_rows: int, dim: int, scale: float = 1.0, dtype=None, device=None):
+        super(TokenEmbedding, self).__init__()
+        self.scale = float(scale)
+        self.weight = nn.Parameter(torch.empty(n_rows, dim, dtype=dtype, device=device))
+        nn.init.normal_(self.weight, std=dim ** -0.5)
+
+    def forward(self, input: torch.Tensor) -> torch.Tensor:
+        if torch.is_grad_enabled() and self.weight.requires_grad:
+            return _EmbedTokens.apply(input, self.weight, self.scale)
+        return ops.embed_tokens(input, self.weight, self.scale)
+
+
 preproc_map = dict(
     normalizer=Normalize, normalize=Normalize,
     flip_normalizer=FlipNormalize, flip_normalize=FlipNormalize,
