@@ -27,3 +27,54 @@ __device__ __forceinline__ typename vx_elem<DT>::type vx_store_cast(float y) {
     if (DT == VX_DTYPE_F16) asm("" : "+v"(y));
     return (typename vx_elem<DT>::type)y;
 }
+
+// 16 bytes of a row: VEC = 16 / sizeof(element) values.  Rows start at any multiple of the element (odd widths, slices), so
+// the access is declared with the element's alignment only: gfx950 loads and stores 16 bytes at any address.
+template <int DT>
+union vx_vec {
+    vx_v4 raw;
+    typename vx_elem<DT>::type e[16 / sizeof(typename vx_elem<DT>::type)];
+};
+typedef float vx_v4_at2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef float vx_v4_at4 __attribute__((ext_vector_type(4), aligned(4)));
+template <int DT>
+__device__ __forceinline__ vx_v4 vx_load16(const typename vx_elem<DT>::type *p) {
+    return DT == VX_DTYPE_F32 ? (vx_v4)*(const vx_v4_at4 *)p : (vx_v4)*(const vx_v4_at2 *)p;
+}
+
+// A lane's VEC columns [c, c + VEC) of a row of D: where they stick out of the row, the lane works on the row's last VEC
+// columns instead (`at`), so that every load is one unconditional 16-byte load, and stores only columns from c on.
+// TINY: the row itself is shorter than VEC.
+template <int DT>
+struct vx_cols {
+    static constexpr int VEC = 16 / sizeof(typename vx_elem<DT>::type);
+    int c, at;
+    __device__ __forceinline__ vx_cols(int c_, int D) : c(c_), at(c_ <= D - VEC ? c_ : (D > VEC ? D - VEC : 0)) {}
+    // values of the row at its columns `at`
+    template <bool TINY>
+    __device__ __forceinline__ vx_vec<DT> load(const typename vx_elem<DT>::type *row, int D) const {
+        vx_vec<DT> v;
+        if (!TINY) {
+            v.raw = vx_load16<DT>(row + at);
+        } else {
+            v.raw = vx_v4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < VEC - 1; ++k)
+                if (k < D) v.e[k] = row[k];
+        }
+        return v;
+    }
+    __device__ __forceinline__ void store(typename vx_elem<DT>::type *row, const float *f, int D) const {
+        vx_vec<DT> v;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v.e[k] = vx_store_cast<DT>(f[k]);
+        if (c == at && c + VEC <= D) {
+            if (DT == VX_DTYPE_F32) *(vx_v4_at4 *)(row + c) = v.raw;
+            else *(vx_v4_at2 *)(row + c) = v.raw;
+        } else if (c < D) {
+#pragma unroll
+            for (int k = 0; k < VEC; ++k)
+                if (at + k >= c && at + k < D) row[at + k] = v.e[k];
+        }
+    }
+};

@@ -8,19 +8,35 @@ __device__ __forceinline__ long long vx_id_at(const void *ids, int id_bytes, lon
     return id_bytes == 8 ? ((const long long *)ids)[t] : (long long)((const int *)ids)[t];
 }
 
-// One workgroup per token.
-template <int DT>
-__global__ __launch_bounds__(256) void vx_k_embed(const void *__restrict__ ids, int id_bytes, const void *__restrict__ table,
-                                                  long long n_rows, int D, long long stride, float scale,
-                                                  void *__restrict__ out, int *__restrict__ status) {
+// ------------------------------------------------------------------------------------------------ lookup
+// One wave per slice of one token's row, U 16-byte pieces for each lane, all loads issued before the first store.
+template <int DT, int U, bool TINY>
+__global__ __launch_bounds__(256) void vx_k_embed(const void *__restrict__ ids, int id_bytes, long long T,
+                                                  const void *__restrict__ table, long long n_rows, int D, int slices,
+                                                  long long stride, float scale, void *__restrict__ out,
+                                                  int *__restrict__ status) {
     typedef typename vx_elem<DT>::type E;
-    const long long t = blockIdx.x;
+    constexpr int VEC = 16 / sizeof(E);
+    const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (item >= T * slices) return;
+    const long long t = item / slices;
+    const int slice = (int)(item - t * slices), lane = vx_lane();
     const long long id = vx_id_at(ids, id_bytes, t);
     const bool ok = id >= 0 && id < n_rows;
-    if (id >= n_rows && status && threadIdx.x == 0) atomicOr(status, VX_STATUS_BAD_TOKEN);
+    if (id >= n_rows && status && lane == 0 && slice == 0) atomicOr(status, VX_STATUS_BAD_TOKEN);
     const E *src = (const E *)table + (ok ? id * stride : 0);
     E *dst = (E *)out + t * D;
-    for (int c = threadIdx.x; c < D; c += 256) dst[c] = ok ? vx_store_cast<DT>((float)src[c] * scale) : (E)0.0f;
+    const int c0 = slice * 64 * VEC * U + lane * VEC;
+    vx_vec<DT> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = vx_cols<DT>(c0 + u * 64 * VEC, D).template load<TINY>(src, D);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        float f[VEC];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) f[k] = ok ? (float)v[u].e[k] * scale : 0.f;
+        vx_cols<DT>(c0 + u * 64 * VEC, D).store(dst, f, D);
+    }
 }
 
 extern "C" int vx_embed_tokens(const void *d_ids, int id_bytes, int64_t n_tokens, const void *d_table, int64_t n_rows,
@@ -33,45 +49,469 @@ extern "C" int vx_embed_tokens(const void *d_ids, int id_bytes, int64_t n_tokens
     if ((((uintptr_t)d_table | (uintptr_t)d_out) & (es - 1)) || ((uintptr_t)d_ids & (id_bytes - 1)) || ((uintptr_t)d_status & 3))
         return VX_ERR_ALIGNMENT;
     hipStream_t st = (hipStream_t)stream;
+    // few tokens: short slices, so that the row of one token is spread over several waves
+    const int vec = 16 / es;
+    const bool wide = n_tokens * (int64_t)D > 1 << 20;
+    const int slices = (D + 64 * vec * (wide ? 4 : 1) - 1) / (64 * vec * (wide ? 4 : 1));
+    const int64_t blocks = (n_tokens * slices + 3) / 4;
+    if (blocks > 2147483647LL) return VX_ERR_UNSUPPORTED;
     vx_prof_begin(VX_PROF_EMBED, st);
-    VX_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL((vx_k_embed<DT>), dim3((unsigned)n_tokens), dim3(256), 0, st, d_ids, id_bytes,
-                                                d_table, (long long)n_rows, D, (long long)table_stride, scale, d_out, d_status));
+    VX_DISPATCH_DTYPE(dtype, {
+        if (D < vec)
+            hipLaunchKernelGGL((vx_k_embed<DT, 1, true>), dim3((unsigned)blocks), dim3(256), 0, st, d_ids, id_bytes, (long long)n_tokens,
+                               d_table, (long long)n_rows, D, slices, (long long)table_stride, scale, d_out, d_status);
+        else if (wide)
+            hipLaunchKernelGGL((vx_k_embed<DT, 4, false>), dim3((unsigned)blocks), dim3(256), 0, st, d_ids, id_bytes, (long long)n_tokens,
+                               d_table, (long long)n_rows, D, slices, (long long)table_stride, scale, d_out, d_status);
+        else
+            hipLaunchKernelGGL((vx_k_embed<DT, 1, false>), dim3((unsigned)blocks), dim3(256), 0, st, d_ids, id_bytes, (long long)n_tokens,
+                               d_table, (long long)n_rows, D, slices, (long long)table_stride, scale, d_out, d_status);
+    });
     vx_prof_end(VX_PROF_EMBED, st);
     return hipGetLastError() == hipSuccess ? VX_OK : VX_ERR_LAUNCH;
 }
 
-// One wave per (table row, 64 columns): the ids are scanned in order, so the sum has one order.
-template <int GT, int TT>
-__global__ __launch_bounds__(64) void vx_k_embed_grad(const void *__restrict__ ids, int id_bytes, long long T,
-                                                      const void *__restrict__ grad, long long n_rows, int D, float scale,
-                                                      void *__restrict__ out, int accumulate, int *__restrict__ status) {
-    typedef typename vx_elem<GT>::type G;
-    typedef typename vx_elem<TT>::type E;
-    const long long v = blockIdx.x;
-    const int lane = vx_lane(), c = blockIdx.y * 64 + lane;
-    float sum = 0.f;
-    bool any = false;
-    for (long long t0 = 0; t0 < T; t0 += 64) {
-        const long long id = t0 + lane < T ? vx_id_at(ids, id_bytes, t0 + lane) : -1;
-        const bool hit = id == v;
-        if (v == 0 && status && id >= n_rows) atomicOr(status, VX_STATUS_BAD_TOKEN);
-        u64 m = __ballot(hit);
-        while (m) {
-            const long long t = t0 + __builtin_ctzll(m);
-            m &= m - 1;
-            any = true;
-            if (c < D) sum += (float)((const G *)grad)[t * D + c];
+// ------------------------------------------------------------------------------------------------ gradient
+// 1. The tokens are sorted by id, stably, so the tokens of a table row lie next to each other in their own order: the sums
+//    have one order whatever the launch does.  Up to 16384 tokens by counting, for each token, the tokens in front of it
+//    (T^2 / 64 compares of a wave: 14 us of the chip's issue at 16384, 3.5 at 8192), beyond by a radix sort.
+// 2. Beyond 2048 tokens every full chunk of 32 sorted tokens of one id is summed once, and (from 8192 tokens) every full
+//    chunk of 32 such chunks: a frequent token's row costs at most 62 rows of grad_out, 62 chunks and one row for each
+//    further 1024 tokens, instead of all its tokens on one wave.
+// 3. Each table row is written once, from its chunks and the tokens at their ends.
+#define VX_EG_COUNT_MAX 16384     // tokens sorted by counting
+#define VX_EG_SUB 2048            // tokens one workgroup of the radix sort ranks at a time: 256 threads x 8
+#define VX_EG_TILES 256           // workgroups of a sorting pass at most
+#define VX_EG_BINS 512            // 9 bits of the id for each pass at most
+#define VX_EG_CHUNK 32
+#define VX_EG_CHUNK_MIN 2048      // up to here no chunks: a long row is split over the waves of its workgroup
+#define VX_EG_CHUNK2_MIN 8192
+#define VX_EG_ROWS 8              // table rows of one workgroup
+
+// Columns of one wave's slice: U pieces of 64 lanes x 16 bytes of grad_out, 512 columns in every type (fp32 with one piece:
+// 27 instead of 24 us at 2048 x 1024; 16-bit types with two: 33 instead of 24 us at 5001 x 1000 fp16, no gain at 4096 columns).
+#define VX_EG_SLICE 512
+template <int GT> __host__ __device__ constexpr int vx_eg_u() { return GT == VX_DTYPE_F32 ? 2 : 1; }
+
+struct vx_eg_plan {
+    int bits, passes, tiles;
+    long long tile;               // tokens of one tile, a multiple of VX_EG_SUB
+    int chunks, chunks2;
+    long long pitch;              // columns of a row of partial sums
+    size_t key[2], pos[2], hist, part1, part2, total;
+};
+
+static vx_eg_plan vx_eg_make_plan(int64_t T, int64_t n_rows, int D) {
+    vx_eg_plan p;
+    int kb = 1;
+    while (kb < 31 && (n_rows >> kb)) ++kb;                       // keys 0 .. n_rows (n_rows: no row)
+    p.passes = (kb + 8) / 9;
+    p.bits = (kb + p.passes - 1) / p.passes;
+    const int64_t subs = (T + VX_EG_SUB - 1) / VX_EG_SUB, per = (subs + VX_EG_TILES - 1) / VX_EG_TILES;
+    p.tile = per * VX_EG_SUB;
+    p.tiles = (int)((T + p.tile - 1) / p.tile);
+    p.chunks = T > VX_EG_CHUNK_MIN ? (int)(T / VX_EG_CHUNK) : 0;
+    p.chunks2 = T >= VX_EG_CHUNK2_MIN ? p.chunks / VX_EG_CHUNK : 0;
+    const bool radix = T > VX_EG_COUNT_MAX;
+    size_t at = 0;
+    auto take = [&](size_t n) { const size_t o = at; at += (n + 255) & ~(size_t)255; return o; };
+    for (int i = 0; i < 2; ++i) {
+        p.key[i] = take(i == 0 || radix ? (size_t)T * 4 : 0);
+        p.pos[i] = take(i == 0 || radix ? (size_t)T * 4 : 0);
+    }
+    p.hist = take(radix ? (size_t)p.tiles * VX_EG_BINS * 4 : 0);
+    p.pitch = (D + VX_EG_SLICE - 1) / VX_EG_SLICE * VX_EG_SLICE;
+    p.part1 = take((size_t)p.chunks * p.pitch * 4);
+    p.part2 = take((size_t)p.chunks2 * p.pitch * 4);
+    p.total = at;
+    return p;
+}
+
+__device__ __forceinline__ unsigned vx_eg_key(const void *ids, int id_bytes, long long t, long long n_rows, int *status) {
+    const long long id = vx_id_at(ids, id_bytes, t);
+    if (id >= n_rows && status) atomicOr(status, VX_STATUS_BAD_TOKEN);
+    return (unsigned)(id >= 0 && id < n_rows ? id : n_rows);
+}
+
+// Stable sort by counting: a workgroup places 64 tokens, one for each lane; its 16 waves share the scan of all keys, four
+// to an LDS read, a compare and an add-with-carry each.  Keys behind a token count when they are smaller, keys in front of
+// it also when they are equal.
+__global__ __launch_bounds__(1024) void vx_k_eg_count_sort(const void *__restrict__ ids, int id_bytes, int T, long long n_rows,
+                                                           unsigned *__restrict__ key_out, int *__restrict__ pos_out,
+                                                           int *__restrict__ status) {
+    __shared__ __attribute__((aligned(16))) unsigned s_key[VX_EG_COUNT_MAX];
+    __shared__ int s_count[64];
+    const int lane = vx_lane(), w = threadIdx.x >> 6;
+    const int groups = (T + 3) >> 2;                              // of four keys
+    for (int i = threadIdx.x; i < groups * 4; i += 1024)
+        s_key[i] = i < T ? vx_eg_key(ids, id_bytes, i, n_rows, blockIdx.x == 0 ? status : nullptr) : ~0u;
+    if (threadIdx.x < 64) s_count[threadIdx.x] = 0;
+    __syncthreads();
+    const int t0 = blockIdx.x * 64, t = min(t0 + lane, T - 1);
+    const unsigned k = s_key[t];
+    const int per = (groups + 15) / 16, g0 = min(groups, w * per), g1 = min(groups, g0 + per);
+    int n = 0;
+    for (int g = g0; g < g1; ++g) {
+        const uint4 q = *(const uint4 *)&s_key[4 * g];
+        if (4 * g + 3 < t0) {
+            n += (q.x <= k) + (q.y <= k) + (q.z <= k) + (q.w <= k);
+        } else if (4 * g >= t0 + 64) {
+            n += (q.x < k) + (q.y < k) + (q.z < k) + (q.w < k);
+        } else {
+            n += (q.x < k || (q.x == k && 4 * g < t)) + (q.y < k || (q.y == k && 4 * g + 1 < t)) +
+                 (q.z < k || (q.z == k && 4 * g + 2 < t)) + (q.w < k || (q.w == k && 4 * g + 3 < t));
         }
     }
-    if (c >= D) return;
-    E *dst = (E *)out + v * D + c;
-    if (!accumulate) *dst = vx_store_cast<TT>(sum * scale);
-    else if (any) *dst = vx_store_cast<TT>((float)*dst + sum * scale);
+    atomicAdd(&s_count[lane], n);
+    __syncthreads();
+    if (w == 0 && t0 + lane < T) {
+        const int at = s_count[lane];
+        key_out[at] = k;
+        pos_out[at] = t;
+    }
+}
+
+// Histogram of one digit of each tile.  Pass 0 reads the ids, the others the keys of the pass before.
+__global__ __launch_bounds__(256) void vx_k_eg_hist(const void *__restrict__ ids, int id_bytes, const unsigned *__restrict__ key_in,
+                                                    long long T, long long n_rows, int bits, int pass, long long tile,
+                                                    int *__restrict__ hist, int *__restrict__ status) {
+    __shared__ int s_h[VX_EG_BINS];
+    const int bins = 1 << bits;
+    for (int i = threadIdx.x; i < bins; i += 256) s_h[i] = 0;
+    __syncthreads();
+    const long long lo = blockIdx.x * tile, hi = min(T, lo + tile);
+    for (long long t = lo + threadIdx.x; t < hi; t += 256) {
+        const unsigned k = pass ? key_in[t] : vx_eg_key(ids, id_bytes, t, n_rows, status);
+        atomicAdd(&s_h[(k >> (pass * bits)) & (bins - 1)], 1);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < bins; i += 256) hist[(size_t)blockIdx.x * VX_EG_BINS + i] = s_h[i];
+}
+
+// One radix sorting pass: each workgroup places the tokens of its tile, 2048 at a time, in order.
+__global__ __launch_bounds__(256) void vx_k_eg_pass(const void *__restrict__ ids, int id_bytes, long long T, long long n_rows,
+                                                    int bits, int pass, long long tile, const int *__restrict__ hist,
+                                                    const unsigned *__restrict__ key_in, const int *__restrict__ pos_in,
+                                                    unsigned *__restrict__ key_out, int *__restrict__ pos_out) {
+    __shared__ int s_wave[4][VX_EG_BINS];     // digits seen by each wave: counts, then the wave's first place of each digit
+    __shared__ int s_base[VX_EG_BINS];        // next place of each digit
+    __shared__ int s_scan[4];
+    const int bins = 1 << bits, tiles = gridDim.x, shift = pass * bits, lane = vx_lane(), w = threadIdx.x >> 6;
+    // digits 2 tid and 2 tid + 1: how often in all tiles, how often in the tiles before this one
+    int total[2] = {}, before[2] = {};
+#pragma unroll 8
+    for (int t = 0; t < tiles; ++t) {
+        const int2 c = 2 * (int)threadIdx.x < bins ? *(const int2 *)&hist[(size_t)t * VX_EG_BINS + 2 * threadIdx.x] : int2{0, 0};
+        total[0] += c.x; total[1] += c.y;
+        if (t < (int)blockIdx.x) { before[0] += c.x; before[1] += c.y; }
+    }
+    int run = total[0] + total[1];
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(run, d, VX_WAVE);
+        if (lane >= d) run += o;
+    }
+    if (lane == 63) s_scan[w] = run;
+    __syncthreads();
+    run -= total[0] + total[1];
+    for (int i = 0; i < w; ++i) run += s_scan[i];
+    if (2 * (int)threadIdx.x < bins) {
+        s_base[2 * threadIdx.x] = run + before[0];
+        s_base[2 * threadIdx.x + 1] = run + total[0] + before[1];
+    }
+    const long long lo = blockIdx.x * tile, hi = min(T, lo + tile);
+    for (long long t0 = lo; t0 < hi; t0 += VX_EG_SUB) {
+        const int n = (int)min((long long)VX_EG_SUB, hi - t0);
+        unsigned key[8];
+        int pos[8], place[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {                             // wave w holds tokens w*512 + r*64 + lane: its own in order
+            const int i = w * 512 + r * 64 + lane;
+            key[r] = 0;
+            pos[r] = (int)(t0 + i);
+            if (i < n) {
+                if (pass) { key[r] = key_in[t0 + i]; pos[r] = pos_in[t0 + i]; }
+                else key[r] = vx_eg_key(ids, id_bytes, t0 + i, n_rows, nullptr);
+            }
+        }
+        for (int i = lane; i < bins; i += 64) s_wave[w][i] = 0;   // the wave's own counters: LDS keeps a wave's order
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const bool in = w * 512 + r * 64 + lane < n;
+            const int d = (key[r] >> shift) & (bins - 1);
+            u64 same = __ballot(in);
+            for (int b = 0; b < bits; ++b) {
+                const u64 one = __ballot((d >> b) & 1);
+                same &= ((d >> b) & 1) ? one : ~one;
+            }
+            place[r] = 0;
+            if (in) {
+                place[r] = s_wave[w][d] + vx_mbcnt(same);
+                if (vx_mbcnt(same) == 0) s_wave[w][d] += __popcll(same);
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < bins; i += 256) {
+            int at = s_base[i];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int c = s_wave[q][i];
+                s_wave[q][i] = at;
+                at += c;
+            }
+            s_base[i] = at;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+            if (w * 512 + r * 64 + lane < n) {
+                const int at = place[r] + s_wave[w][(key[r] >> shift) & (bins - 1)];
+                key_out[at] = key[r];
+                pos_out[at] = pos[r];
+            }
+        __syncthreads();
+    }
+}
+
+// sum[] += N rows of grad_out at pos(0..N-1), all of them in flight together, added in that order
+template <int GT, int U, bool TINY, int N, class P>
+__device__ __forceinline__ void vx_eg_add_n(const typename vx_elem<GT>::type *__restrict__ grad, P pos, int D, int c, float *sum) {
+    constexpr int VEC = 16 / sizeof(typename vx_elem<GT>::type);
+    vx_vec<GT> v[N][U];
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+#pragma unroll
+        for (int q = 0; q < U; ++q) v[u][q] = vx_cols<GT>(c + q * 64 * VEC, D).template load<TINY>(grad + (long long)pos(u) * D, D);
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+#pragma unroll
+        for (int q = 0; q < U; ++q)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) sum[q * VEC + k] += (float)v[u][q].e[k];
+}
+
+// sum[] += rows of grad_out at pos[a..b), in that order.
+// LONG (chunks, and the rows of a call without chunks): the lanes fetch 64 positions together, eight rows are in flight.
+// Else (the ends of a row whose middle has chunks; most rows have a token or two): scalar positions and few registers --
+// with LONG's registers the rows of 65536 tokens x 4096 columns bf16 took 317 to 355 us instead of 270, and without LONG
+// the rows of 2048 x 1024 fp32 57 instead of 25 us.
+template <int GT, int U, bool TINY, bool LONG>
+__device__ __forceinline__ void vx_eg_add_tokens(const typename vx_elem<GT>::type *__restrict__ grad, const int *__restrict__ pos,
+                                                 int a, int b, int D, int c, float *sum) {
+    if (!LONG || b - a < 8) {
+        auto at = [&](int u) { return pos[a + u]; };
+        for (; b - a >= 4; a += 4) vx_eg_add_n<GT, U, TINY, 4>(grad, at, D, c, sum);
+        if ((b - a) & 2) { vx_eg_add_n<GT, U, TINY, 2>(grad, at, D, c, sum); a += 2; }
+        if ((b - a) & 1) vx_eg_add_n<GT, U, TINY, 1>(grad, at, D, c, sum);
+        return;
+    }
+    for (; a < b; a += 64) {
+        const int n = min(64, b - a), lane = vx_lane();
+        const int mine = lane < n ? pos[a + lane] : 0;
+        int i = 0;
+        auto at = [&](int u) { return __builtin_amdgcn_readlane(mine, i + u); };
+        for (; i + 8 <= n; i += 8) vx_eg_add_n<GT, U, TINY, 8>(grad, at, D, c, sum);
+        if (n & 4) { vx_eg_add_n<GT, U, TINY, 4>(grad, at, D, c, sum); i += 4; }
+        if (n & 2) { vx_eg_add_n<GT, U, TINY, 2>(grad, at, D, c, sum); i += 2; }
+        if (n & 1) vx_eg_add_n<GT, U, TINY, 1>(grad, at, D, c, sum);
+    }
+}
+
+// sum[] += rows a..b of fp32 partial sums.  Their rows are padded to VX_EG_SLICE columns (pitch), so no column sticks out: a
+// lane keeps the columns of its sums, those of vx_cols.
+template <int GT, int U>
+__device__ __forceinline__ void vx_eg_add_partials(const float *__restrict__ part, long long a, long long b, long long pitch, int c, float *sum) {
+    constexpr int VEC = 16 / sizeof(typename vx_elem<GT>::type);
+#pragma unroll 4
+    for (long long i = a; i < b; ++i)
+#pragma unroll
+        for (int q = 0; q < U; ++q)
+#pragma unroll
+            for (int k = 0; k < VEC; k += 4) {
+                const vx_f4 v = *(const vx_f4 *)(part + i * pitch + c + q * 64 * VEC + k);
+                sum[q * VEC + k] += v.x; sum[q * VEC + k + 1] += v.y; sum[q * VEC + k + 2] += v.z; sum[q * VEC + k + 3] += v.w;
+            }
+}
+
+// One wave per (chunk of 32 sorted tokens, slice of columns); chunks of several ids have no sum of their own.
+template <int GT, int U, bool TINY>
+__global__ __launch_bounds__(256) void vx_k_eg_chunks(const unsigned *__restrict__ key, const int *__restrict__ pos, int chunks,
+                                                      unsigned n_rows, const void *__restrict__ grad, int D, int slices,
+                                                      long long pitch, float *__restrict__ part1) {
+    typedef typename vx_elem<GT>::type G;
+    constexpr int VEC = 16 / sizeof(G);
+    const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const long long c1 = item / slices;
+    if (c1 >= chunks) return;
+    const int a = (int)c1 * VX_EG_CHUNK, c = (int)(item - c1 * slices) * VX_EG_SLICE + vx_lane() * VEC;
+    const unsigned k0 = key[a];
+    if (k0 >= n_rows || key[a + VX_EG_CHUNK - 1] != k0) return;
+    float sum[U * VEC] = {};
+    vx_eg_add_tokens<GT, U, TINY, true>((const G *)grad, pos, a, a + VX_EG_CHUNK, D, c, sum);
+#pragma unroll
+    for (int q = 0; q < U; ++q)
+#pragma unroll
+        for (int k = 0; k < VEC; k += 4)
+            *(vx_f4 *)(part1 + c1 * pitch + c + q * 64 * VEC + k) = vx_f4{sum[q * VEC + k], sum[q * VEC + k + 1], sum[q * VEC + k + 2], sum[q * VEC + k + 3]};
+}
+
+// The same over 32 chunks; 256 columns for each wave.
+__global__ __launch_bounds__(256) void vx_k_eg_chunks2(const unsigned *__restrict__ key, int chunks, unsigned n_rows, int slices,
+                                                       long long pitch, const float *__restrict__ part1, float *__restrict__ part2) {
+    const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const long long c2 = item / slices;
+    if (c2 >= chunks) return;
+    const int a = (int)c2 * VX_EG_CHUNK * VX_EG_CHUNK, c = (int)(item - c2 * slices) * 256 + vx_lane() * 4;
+    const unsigned k0 = key[a];
+    if (k0 >= n_rows || key[a + VX_EG_CHUNK * VX_EG_CHUNK - 1] != k0) return;
+    float sum[4] = {};
+    vx_eg_add_partials<VX_DTYPE_F32, 1>(part1, c2 * VX_EG_CHUNK, (c2 + 1) * VX_EG_CHUNK, pitch, c, sum);
+    *(vx_f4 *)(part2 + c2 * pitch + c) = vx_f4{sum[0], sum[1], sum[2], sum[3]};
+}
+
+// first i in [0, n] with key[i] >= target, by the 16 lanes of a quarter wave: a sixteenth of the range is left each step
+__device__ __forceinline__ int vx_eg_lower_bound(const unsigned *__restrict__ key, int n, unsigned target) {
+    const int lane = vx_lane(), sub = lane & 15, at = lane & 48;
+    int lo = 0, hi = n;
+    while (__any(hi > lo)) {
+        const int step = (hi - lo + 15) >> 4;
+        const long long p = (long long)lo + (long long)(sub + 1) * step - 1;
+        const bool less = p < hi && key[p] < target;
+        const int c = __popc((unsigned)(__ballot(less) >> at) & 0xffffu);
+        const long long top = (long long)lo + (long long)(c + 1) * step - 1;
+        lo = (int)min((long long)hi, (long long)lo + (long long)c * step);
+        hi = (int)min((long long)hi, top);
+        hi = max(hi, lo);
+    }
+    return lo;
+}
+
+// Table rows blockIdx + i * gridDim (i < 8): frequent ids lie next to each other, so neighbours go to different workgroups.
+// A wave sums one slice of one row; without chunks rows of more than 32 tokens follow, their tokens split
+// over the four waves and joined through LDS in wave order.
+template <int GT, int TT, int U, bool TINY, bool CHUNKED>
+__global__ __launch_bounds__(256) void vx_k_eg_rows(const unsigned *__restrict__ key, const int *__restrict__ pos, int T,
+                                                    const void *__restrict__ grad, long long n_rows, int D, int slices, float scale,
+                                                    void *__restrict__ out, int accumulate, int chunked2, long long pitch,
+                                                    const float *__restrict__ part1, const float *__restrict__ part2) {
+    typedef typename vx_elem<GT>::type G;
+    typedef typename vx_elem<TT>::type E;
+    constexpr int VEC = 16 / sizeof(G);
+    __shared__ int s_at[2 * VX_EG_ROWS];
+    __shared__ float s_sum[CHUNKED ? 1 : 3][U * VEC][CHUNKED ? 1 : 64];
+    const int lane = vx_lane(), w = threadIdx.x >> 6;
+    {
+        const int q = threadIdx.x >> 4;                           // 16 searches: the beginning and the end of 8 rows
+        const long long v = blockIdx.x + (long long)(q >> 1) * gridDim.x + (q & 1);
+        const int at = vx_eg_lower_bound(key, T, (unsigned)min(v, n_rows));
+        if ((lane & 15) == 0) s_at[q] = at;
+    }
+    __syncthreads();
+    auto finish = [&](long long v, int c, float *sum) {
+        E *dst = (E *)out + v * D;
+#pragma unroll
+        for (int k = 0; k < U * VEC; ++k) sum[k] *= scale;
+        // columns at .. at + VEC of the sums, from c on to be stored; the table's pieces are VEC wide, or half of it where a
+        // 16-bit gradient is summed into fp32
+        constexpr int W = 16 / sizeof(E);
+#pragma unroll
+        for (int q = 0; q < U; ++q) {
+            const vx_cols<GT> col(c + q * 64 * VEC, D);
+            if (col.c >= D) continue;
+#pragma unroll
+            for (int k = 0; k < VEC; k += W) {
+                vx_cols<TT> part(0, D);
+                part.c = max(col.c, col.at + k);
+                part.at = col.at + k;
+                float *f = sum + q * VEC + k;
+                if (accumulate) {
+                    vx_vec<TT> old;
+                    if (!TINY) {
+                        old.raw = vx_load16<TT>(dst + part.at);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < W; ++j) old.e[j] = part.at + j < D ? dst[part.at + j] : (E)0.0f;
+                    }
+#pragma unroll
+                    for (int j = 0; j < W; ++j) f[j] = (float)old.e[j] + f[j];
+                }
+                part.store(dst, f, D);
+            }
+        }
+    };
+    for (int item = w; item < VX_EG_ROWS * slices; item += 4) {
+        const int i = item / slices, c = (item - i * slices) * VX_EG_SLICE + lane * VEC;
+        const long long v = blockIdx.x + (long long)i * gridDim.x;
+        const int s = __builtin_amdgcn_readfirstlane(s_at[2 * i]), e = __builtin_amdgcn_readfirstlane(s_at[2 * i + 1]);
+        if (v >= n_rows || (accumulate && s == e) || (!CHUNKED && e - s > VX_EG_CHUNK)) continue;
+        float sum[U * VEC] = {};
+        const int a1 = (s + VX_EG_CHUNK - 1) / VX_EG_CHUNK, b1 = e / VX_EG_CHUNK;
+        if (a1 >= b1 || !CHUNKED) {
+            vx_eg_add_tokens<GT, U, TINY, !CHUNKED>((const G *)grad, pos, s, e, D, c, sum);
+        } else {
+            vx_eg_add_tokens<GT, U, TINY, !CHUNKED>((const G *)grad, pos, s, a1 * VX_EG_CHUNK, D, c, sum);
+            const int a2 = (a1 + VX_EG_CHUNK - 1) / VX_EG_CHUNK, b2 = b1 / VX_EG_CHUNK;
+            if (a2 >= b2 || !chunked2) {
+                vx_eg_add_partials<GT, U>(part1, a1, b1, pitch, c, sum);
+            } else {
+                vx_eg_add_partials<GT, U>(part1, a1, (long long)a2 * VX_EG_CHUNK, pitch, c, sum);
+                vx_eg_add_partials<GT, U>(part2, a2, b2, pitch, c, sum);
+                vx_eg_add_partials<GT, U>(part1, (long long)b2 * VX_EG_CHUNK, b1, pitch, c, sum);
+            }
+            vx_eg_add_tokens<GT, U, TINY, !CHUNKED>((const G *)grad, pos, b1 * VX_EG_CHUNK, e, D, c, sum);
+        }
+        if (c < D) finish(v, c, sum);
+    }
+    if (CHUNKED) return;
+    for (int i = 0; i < VX_EG_ROWS; ++i) {
+        const long long v = blockIdx.x + (long long)i * gridDim.x;
+        const int s = __builtin_amdgcn_readfirstlane(s_at[2 * i]), e = __builtin_amdgcn_readfirstlane(s_at[2 * i + 1]);
+        if (v >= n_rows || e - s <= VX_EG_CHUNK) continue;        // the same for the whole workgroup
+        const int per = (e - s + 3) / 4, a = min(e, s + w * per), b = min(e, a + per);
+        for (int sl = 0; sl < slices; ++sl) {
+            const int c = sl * VX_EG_SLICE + lane * VEC;
+            float sum[U * VEC] = {};
+            vx_eg_add_tokens<GT, U, TINY, !CHUNKED>((const G *)grad, pos, a, b, D, c, sum);
+            if (w)
+#pragma unroll
+                for (int k = 0; k < U * VEC; ++k) s_sum[w - 1][k][lane] = sum[k];
+            __syncthreads();
+            if (w == 0 && c < D) {
+#pragma unroll
+                for (int q = 0; q < 3; ++q)
+#pragma unroll
+                    for (int k = 0; k < U * VEC; ++k) sum[k] += s_sum[q][k][lane];
+                finish(v, c, sum);
+            }
+            __syncthreads();
+        }
+    }
 }
 
 extern "C" size_t vx_embed_tokens_grad_workspace_bytes(int64_t n_tokens, int64_t n_rows, int D) {
     if (n_tokens <= 0 || n_rows <= 0 || D <= 0 || n_tokens > VX_MAX_TOKENS || n_rows > VX_MAX_VOCAB || D > VX_MAX_TOKEN_WIDTH) return 0;
-    return 256;
+    return vx_eg_make_plan(n_tokens, n_rows, D).total;
+}
+
+// steps 2 and 3, once the tokens are sorted (key, pos)
+template <int GT, int TT, bool TINY>
+static void vx_eg_sum(const vx_eg_plan &p, const unsigned *key, const int *pos, int T, const void *grad, long long n_rows, int D,
+                      float scale, void *out, int accumulate, float *part1, float *part2, hipStream_t st) {
+    constexpr int U = vx_eg_u<GT>();
+    const int slices = (int)(p.pitch / VX_EG_SLICE), slices2 = (int)(p.pitch / 256);
+    if (p.chunks)
+        hipLaunchKernelGGL((vx_k_eg_chunks<GT, U, TINY>), dim3((unsigned)(((int64_t)p.chunks * slices + 3) / 4)), dim3(256), 0, st, key,
+                           pos, p.chunks, (unsigned)n_rows, grad, D, slices, p.pitch, part1);
+    if (p.chunks2)
+        hipLaunchKernelGGL(vx_k_eg_chunks2, dim3((unsigned)(((int64_t)p.chunks2 * slices2 + 3) / 4)), dim3(256), 0, st, key, p.chunks2,
+                           (unsigned)n_rows, slices2, p.pitch, part1, part2);
+    const dim3 grid((unsigned)((n_rows + VX_EG_ROWS - 1) / VX_EG_ROWS));
+    if (p.chunks)
+        hipLaunchKernelGGL((vx_k_eg_rows<GT, TT, U, TINY, true>), grid, dim3(256), 0, st, key, pos, T, grad, n_rows, D, slices, scale, out,
+                           accumulate, p.chunks2 > 0, p.pitch, part1, part2);
+    else
+        hipLaunchKernelGGL((vx_k_eg_rows<GT, TT, U, TINY, false>), grid, dim3(256), 0, st, key, pos, T, grad, n_rows, D, slices, scale, out,
+                           accumulate, 0, p.pitch, part1, part2);
 }
 
 extern "C" int vx_embed_tokens_grad(const void *d_ids, int id_bytes, int64_t n_tokens, const void *d_grad_out,
@@ -82,21 +522,43 @@ extern "C" int vx_embed_tokens_grad(const void *d_ids, int id_bytes, int64_t n_t
     if ((id_bytes != 4 && id_bytes != 8) || !vx_dtype_ok(grad_dtype) || !vx_dtype_ok(table_dtype)) return VX_ERR_INVALID_ARG;
     if (n_tokens > VX_MAX_TOKENS || n_rows > VX_MAX_VOCAB || D > VX_MAX_TOKEN_WIDTH) return VX_ERR_UNSUPPORTED;
     if (table_dtype != grad_dtype && table_dtype != VX_DTYPE_F32) return VX_ERR_UNSUPPORTED;
-    if (workspace_bytes < vx_embed_tokens_grad_workspace_bytes(n_tokens, n_rows, D)) return VX_ERR_WORKSPACE;
+    const vx_eg_plan p = vx_eg_make_plan(n_tokens, n_rows, D);
+    if (workspace_bytes < p.total) return VX_ERR_WORKSPACE;
     if (((uintptr_t)d_grad_out & (vx_elem_size(grad_dtype) - 1)) || ((uintptr_t)d_grad_table & (vx_elem_size(table_dtype) - 1)) ||
         ((uintptr_t)d_ids & (id_bytes - 1)) || ((uintptr_t)d_status & 3) || ((uintptr_t)d_workspace & 255))
         return VX_ERR_ALIGNMENT;
+    const int T = (int)n_tokens;
+    if ((int64_t)p.chunks * (p.pitch / VX_EG_SLICE) > 4LL * 2147483647 || (int64_t)p.chunks2 * (p.pitch / 256) > 4LL * 2147483647)
+        return VX_ERR_UNSUPPORTED;
+    char *ws = (char *)d_workspace;
+    unsigned *key[2] = {(unsigned *)(ws + p.key[0]), (unsigned *)(ws + p.key[1])};
+    int *pos[2] = {(int *)(ws + p.pos[0]), (int *)(ws + p.pos[1])}, *hist = (int *)(ws + p.hist);
+    float *part1 = (float *)(ws + p.part1), *part2 = (float *)(ws + p.part2);
     hipStream_t st = (hipStream_t)stream;
-    const dim3 grid((unsigned)n_rows, (unsigned)((D + 63) / 64));
     vx_prof_begin(VX_PROF_EMBED_GRAD, st);
+    int at = 0;                                                   // the buffers that hold the sorted tokens
+    if (T <= VX_EG_COUNT_MAX) {
+        hipLaunchKernelGGL(vx_k_eg_count_sort, dim3((T + 63) / 64), dim3(1024), 0, st, d_ids, id_bytes, T, (long long)n_rows, key[0],
+                           pos[0], d_status);
+    } else {
+        for (int i = 0; i < p.passes; ++i) {
+            at = i & 1;
+            hipLaunchKernelGGL(vx_k_eg_hist, dim3(p.tiles), dim3(256), 0, st, d_ids, id_bytes, key[at ^ 1], (long long)T,
+                               (long long)n_rows, p.bits, i, p.tile, hist, d_status);
+            hipLaunchKernelGGL(vx_k_eg_pass, dim3(p.tiles), dim3(256), 0, st, d_ids, id_bytes, (long long)T, (long long)n_rows, p.bits,
+                               i, p.tile, hist, key[at ^ 1], pos[at ^ 1], key[at], pos[at]);
+        }
+    }
     VX_DISPATCH_DTYPE(grad_dtype, {
-        if (table_dtype == DT)
-            hipLaunchKernelGGL((vx_k_embed_grad<DT, DT>), grid, dim3(64), 0, st, d_ids, id_bytes, (long long)n_tokens,
-                               d_grad_out, (long long)n_rows, D, scale, d_grad_table, accumulate, d_status);
-        else
-            hipLaunchKernelGGL((vx_k_embed_grad<DT, VX_DTYPE_F32>), grid, dim3(64), 0, st, d_ids, id_bytes,
-                               (long long)n_tokens, d_grad_out, (long long)n_rows, D, scale, d_grad_table, accumulate,
-                               d_status);
+        if (D < 16 / vx_elem_size(DT)) {
+            if (table_dtype == DT) vx_eg_sum<DT, DT, true>(p, key[at], pos[at], T, d_grad_out, n_rows, D, scale, d_grad_table, accumulate, part1, part2, st);
+            else vx_eg_sum<DT, VX_DTYPE_F32, true>(p, key[at], pos[at], T, d_grad_out, n_rows, D, scale, d_grad_table, accumulate, part1,
+                                                    part2, st);
+        } else {
+            if (table_dtype == DT) vx_eg_sum<DT, DT, false>(p, key[at], pos[at], T, d_grad_out, n_rows, D, scale, d_grad_table, accumulate, part1, part2, st);
+            else vx_eg_sum<DT, VX_DTYPE_F32, false>(p, key[at], pos[at], T, d_grad_out, n_rows, D, scale, d_grad_table, accumulate, part1,
+                                                     part2, st);
+        }
     });
     vx_prof_end(VX_PROF_EMBED_GRAD, st);
     return hipGetLastError() == hipSuccess ? VX_OK : VX_ERR_LAUNCH;
