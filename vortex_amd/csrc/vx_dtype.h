@@ -35,11 +35,29 @@ union vx_vec {
     vx_v4 raw;
     typename vx_elem<DT>::type e[16 / sizeof(typename vx_elem<DT>::type)];
 };
+typedef float vx_v2 __attribute__((ext_vector_type(2)));
+typedef float vx_v2_at2 __attribute__((ext_vector_type(2), aligned(2)));
 typedef float vx_v4_at2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef float vx_v4_at4 __attribute__((ext_vector_type(4), aligned(4)));
 template <int DT>
 __device__ __forceinline__ vx_v4 vx_load16(const typename vx_elem<DT>::type *p) {
     return DT == VX_DTYPE_F32 ? (vx_v4)*(const vx_v4_at4 *)p : (vx_v4)*(const vx_v4_at2 *)p;
+}
+
+// VEC values at p, `left` of them inside the row (none for left <= 0): the others are 0 and not read.
+template <int DT>
+__device__ __forceinline__ vx_vec<DT> vx_load_vec(const typename vx_elem<DT>::type *p, int left) {
+    constexpr int VEC = 16 / sizeof(typename vx_elem<DT>::type);
+    vx_vec<DT> v;
+    v.raw = vx_v4{0.f, 0.f, 0.f, 0.f};
+    if (left >= VEC) {
+        v.raw = vx_load16<DT>(p);
+    } else {
+#pragma unroll
+        for (int k = 0; k < VEC - 1; ++k)
+            if (k < left) v.e[k] = p[k];
+    }
+    return v;
 }
 
 // A lane's VEC columns [c, c + VEC) of a row of D: where they stick out of the row, the lane works on the row's last VEC

@@ -14,37 +14,83 @@ __device__ __forceinline__ int vx_quant1(float x, float amax) {
     return (int)rintf((x * 127.0f) / amax);
 }
 
-// One workgroup per row.  A row with a NaN or an infinity gets the scale NaN (and q = 0): its products are all NaN.
-template <int DT>
-__global__ __launch_bounds__(256) void vx_k_quant_rows(const void *__restrict__ x, int K, long long xs, int8_t *__restrict__ q,
-                                                       long long qs, float *__restrict__ scale) {
+// WAVES waves per row.  The row's values stay in registers between the two passes (maximum, quotients) up to
+// WAVES * 64 * VEC * U of them; longer rows are read again.  A row with a NaN or an infinity gets the scale NaN (and q = 0):
+// its products are all NaN.  Bound by the read of x.
+template <int DT, int WAVES>
+__global__ __launch_bounds__(256) void vx_k_quant_rows(const void *__restrict__ x, long long M, int K, long long xs,
+                                                       int8_t *__restrict__ q, long long qs, float *__restrict__ scale) {
     typedef typename vx_elem<DT>::type E;
+    constexpr int VEC = 16 / sizeof(E), U = 4, THREADS = WAVES * 64;
     __shared__ float s_max[4];
     __shared__ int s_bad[4];
-    const long long m = blockIdx.x;
+    const int w = threadIdx.x >> 6, tid = WAVES == 1 ? vx_lane() : (int)threadIdx.x;
+    const long long m = WAVES == 1 ? (long long)blockIdx.x * 4 + w : (long long)blockIdx.x;
+    if (m >= M) return;                                           // WAVES == 1 has no barrier behind this
     const E *row = (const E *)x + m * xs;
     float mx = 0.f;
     bool bad = false;
-    for (int k = threadIdx.x; k < K; k += 256) {
-        const float a = fabsf((float)row[k]);
-        bad |= !(a <= 3.4028234663852886e38f);
-        mx = fmaxf(mx, a);
+    vx_vec<DT> v[U];
+    const bool once = K <= THREADS * VEC * U;
+    auto look = [&](const vx_vec<DT> &a) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+            const float f = fabsf((float)a.e[k]);
+            bad |= !(f <= 3.4028234663852886e38f);
+            mx = fmaxf(mx, f);
+        }
+    };
+    if (once) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = vx_load_vec<DT>(row + (u * THREADS + tid) * VEC, K - (u * THREADS + tid) * VEC);
+#pragma unroll
+        for (int u = 0; u < U; ++u) look(v[u]);
+    } else {
+        for (int c = tid * VEC; c < K; c += THREADS * VEC) look(vx_load_vec<DT>(row + c, K - c));
     }
+#pragma unroll
     for (int i = 32; i >= 1; i >>= 1) mx = fmaxf(mx, __shfl_xor(mx, i, VX_WAVE));
-    const bool wbad = __any(bad);
-    if (vx_lane() == 0) { s_max[threadIdx.x >> 6] = mx; s_bad[threadIdx.x >> 6] = wbad; }
-    __syncthreads();
-    mx = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-    bad = s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3];
+    bad = __any(bad);
+    if (WAVES > 1) {
+        if (vx_lane() == 0) { s_max[w] = mx; s_bad[w] = bad; }
+        __syncthreads();
+        mx = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+        bad = s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3];
+    }
     int8_t *dst = q + m * qs;
     const bool zero = bad || mx == 0.f;
-    for (int k = threadIdx.x; k < qs; k += 256) dst[k] = (zero || k >= K) ? 0 : (int8_t)vx_quant1<DT>((float)row[k], mx);
-    if (threadIdx.x == 0) scale[m] = bad ? __builtin_nanf("") : mx / 127.0f;
+    auto put = [&](const vx_vec<DT> &a, int c) {
+        union { int8_t b[VEC]; unsigned w[VEC / 4]; } o;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) o.b[k] = zero ? 0 : (int8_t)vx_quant1<DT>((float)a.e[k], mx);
+        if (c + VEC <= qs) {                                      // columns K .. qs - 1 come out as 0
+            typedef unsigned u32_at1 __attribute__((aligned(1)));
+#pragma unroll
+            for (int k = 0; k < VEC / 4; ++k) *(u32_at1 *)(dst + c + 4 * k) = o.w[k];
+        } else {
+#pragma unroll
+            for (int k = 0; k < VEC; ++k)
+                if (c + k < qs) dst[c + k] = o.b[k];
+        }
+    };
+    if (once) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) put(v[u], (u * THREADS + tid) * VEC);
+    }
+    for (long long c = (once ? THREADS * VEC * U : 0) + tid * VEC; c < qs; c += THREADS * VEC)
+        put(vx_load_vec<DT>(row + c, K - (int)c), (int)c);
+    if (tid == 0) scale[m] = bad ? __builtin_nanf("") : mx / 127.0f;
 }
 
 static int vx_quant_launch(const void *x, int dtype, long long M, int K, long long xs, int8_t *q, long long qs, float *s, hipStream_t st) {
     vx_prof_begin(VX_PROF_QUANT, st);
-    VX_DISPATCH_DTYPE(dtype, hipLaunchKernelGGL((vx_k_quant_rows<DT>), dim3((unsigned)M), dim3(256), 0, st, x, K, xs, q, qs, s));
+    // a row that one wave holds needs no barrier
+    VX_DISPATCH_DTYPE(dtype, {
+        if (K <= 64 * 4 * 16 / vx_elem_size(DT))
+            hipLaunchKernelGGL((vx_k_quant_rows<DT, 1>), dim3((unsigned)((M + 3) / 4)), dim3(256), 0, st, x, M, K, xs, q, qs, s);
+        else
+            hipLaunchKernelGGL((vx_k_quant_rows<DT, 4>), dim3((unsigned)M), dim3(256), 0, st, x, M, K, xs, q, qs, s);
+    });
     vx_prof_end(VX_PROF_QUANT, st);
     return hipGetLastError() == hipSuccess ? VX_OK : VX_ERR_LAUNCH;
 }
@@ -57,50 +103,297 @@ extern "C" int vx_quantize_rows_i8(const void *d_x, int dtype, int64_t M, int K,
     return vx_quant_launch(d_x, dtype, M, K, x_stride, d_q, q_stride, d_scale, (hipStream_t)stream);
 }
 
-// 64 x 64 outputs for each workgroup, 64 bytes of K staged at a time; a thread owns 4 x 4 outputs (4-byte dot products).
-template <int DT>
-__global__ __launch_bounds__(256) void vx_k_linear_i8(const int8_t *__restrict__ q, long long qs, const float *__restrict__ s,
-                                                      long long M, const int8_t *__restrict__ w, long long ws,
-                                                      const float *__restrict__ sw, long long N, int K,
-                                                      const float *__restrict__ bias, void *__restrict__ out, long long os) {
-    typedef typename vx_elem<DT>::type E;
-    __shared__ int s_q[64][17], s_w[64][17];
-    const long long m0 = (long long)blockIdx.y * 64, n0 = (long long)blockIdx.x * 64;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    int acc[4][4] = {};
-    for (int k0 = 0; k0 < K; k0 += 64) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-            const int r = i >> 6, k = i & 63;
-            ((int8_t *)&s_q[r][0])[k] = (m0 + r < M && k0 + k < K) ? q[(m0 + r) * qs + k0 + k] : 0;
-            ((int8_t *)&s_w[r][0])[k] = (n0 + r < N && k0 + k < K) ? w[(n0 + r) * ws + k0 + k] : 0;
-        }
-        __syncthreads();
-        for (int k = 0; k < 16; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    acc[i][j] = __builtin_amdgcn_sdot4(s_q[ty + 16 * i][k], s_w[tx + 16 * j][k], acc[i][j], false);
-    }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const long long m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-            if (m < M && n < N) {
-                float y = (float)acc[i][j] * (s[m] * sw[n]);
-                if (bias) y = y + bias[n];
-                ((E *)out)[m * os + n] = vx_store_cast<DT>(y);
-            }
-        }
+typedef int vx_i4 __attribute__((ext_vector_type(4)));
+typedef int vx_i16 __attribute__((ext_vector_type(16)));
+typedef vx_i4 vx_i4_at1 __attribute__((aligned(1)));
+
+// y for one output; the same expression in every kernel, so that all variants give the same bits
+__device__ __forceinline__ float vx_linear_out(int acc, float s, float sw, const float *bias, long long n) {
+    float y = (float)acc * (s * sw);
+    if (bias) y = y + bias[n];
+    return y;
 }
 
-static int vx_linear_launch(const int8_t *q, long long qs, const float *s, long long M, const int8_t *w, long long ws,
+// ---- few tokens: the weights stream once from memory into registers, no LDS between.
+// One workgroup per 16 channels, its waves share K; mfma 16x16x64 with the weights as rows: lane l holds 16 bytes of channel
+// l % 16 at k = 64 b + 16 (l / 16), and MT tiles of 16 tokens stand against them.
+__device__ __forceinline__ vx_i4 vx_i8_tail(const int8_t *row, int k, int K) {      // bytes k .. k+15, 0 from K on
+    union { vx_i4 v; int8_t b[16]; } o;
+    o.v = vx_i4{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        if (k + i < K) o.b[i] = row[k + i];
+    return o.v;
+}
+
+template <int DT, int MT>
+__global__ __launch_bounds__(1024) void vx_k_linear_stream(const int8_t *__restrict__ q, long long qs, const float *__restrict__ s,
+                                                          long long M, const int8_t *__restrict__ w, long long ws,
+                                                          const float *__restrict__ sw, long long N, int K,
+                                                          const float *__restrict__ bias, void *__restrict__ out, long long os) {
+    typedef typename vx_elem<DT>::type E;
+    constexpr int UN = MT == 1 ? 8 : 4;
+    extern __shared__ int s_part[];                               // [waves][MT][16 tokens][16 channels]
+    const int lane = vx_lane(), wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const long long n0 = (long long)blockIdx.x * 16, m0 = (long long)blockIdx.y * 16 * MT;
+    const int8_t *wrow = w + min(n0 + (lane & 15), N - 1) * ws;
+    const int8_t *qrow[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) qrow[t] = q + min(m0 + t * 16 + (lane & 15), M - 1) * qs;
+    vx_i4 acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = vx_i4{0, 0, 0, 0};
+    const int blocks = (K + 63) >> 6, per = (blocks + waves - 1) / waves, full = K >> 6;
+    int b = min(blocks, wave * per);
+    const int end = min(blocks, b + per), end_full = min(end, full);
+    const int koff = (lane >> 4) * 16;
+    for (; b + UN <= end_full; b += UN) {
+        vx_i4 a[UN], x[UN][MT];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) a[u] = *(const vx_i4_at1 *)(wrow + (b + u) * 64 + koff);
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) x[u][t] = *(const vx_i4_at1 *)(qrow[t] + (b + u) * 64 + koff);
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u], x[u][t], acc[t], 0, 0, 0);
+    }
+    for (; b < end_full; ++b) {
+        const vx_i4 a = *(const vx_i4_at1 *)(wrow + b * 64 + koff);
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+            acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, *(const vx_i4_at1 *)(qrow[t] + b * 64 + koff), acc[t], 0, 0, 0);
+    }
+    if (b < end) {                                                // the last 64 bytes stick out of the rows
+        const vx_i4 a = vx_i8_tail(wrow, b * 64 + koff, K);
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+            acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, vx_i8_tail(qrow[t], b * 64 + koff, K), acc[t], 0, 0, 0);
+    }
+    // lane l holds token l % 16, channels 4 (l / 16) .. + 3
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+        *(vx_i4 *)&s_part[((wave * MT + t) * 16 + (lane & 15)) * 16 + (lane >> 4) * 4] = acc[t];
+    __syncthreads();
+    for (int i = threadIdx.x; i < MT * 256; i += blockDim.x) {
+        int sum = 0;
+        for (int k = 0; k < waves; ++k) sum += s_part[k * MT * 256 + i];
+        const long long m = m0 + (i >> 4), n = n0 + (i & 15);
+        if (m < M && n < N) ((E *)out)[m * os + n] = vx_store_cast<DT>(vx_linear_out(sum, s[m], sw[n], bias, n));
+    }
+}
+
+// ---- many tokens: TM x TN outputs for each workgroup, WM x WN waves of 32x32x32 mfma tiles (weights as rows, tokens as
+// columns, so a lane's four accumulators in a row are four neighbouring channels of one token).
+// K goes by 64 bytes through a ring of four LDS stages that the loads fill directly; each wave's operands of step t + 1 are
+// read into registers while the matrix instructions of step t run, and step t + 4 is requested once step t's slot is free.
+// An LDS row is 64 bytes; its 16-byte pieces are stored at piece ^ ((row >> 1) & 3), so the eight rows that one quarter of a
+// 16-byte LDS read covers lie in all banks.
+// Needs 16-byte aligned rows; q padded with zeros to a multiple of 64, w's pieces beyond K read as piece 0 (K % 16 == 0).
+template <int N>
+__device__ __forceinline__ void vx_wait_stage() {                 // at most N loads and no LDS read outstanding, then the barrier
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+template <int DT, int TM, int TN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64) void vx_k_linear_tile(const int8_t *__restrict__ q, long long qs,
+                                                                 const float *__restrict__ s, long long M,
+                                                                 const int8_t *__restrict__ w, long long ws,
+                                                                 const float *__restrict__ sw, long long N, int K,
+                                                                 const float *__restrict__ bias, void *__restrict__ out,
+                                                                 long long os, int gm, int gn) {
+    typedef typename vx_elem<DT>::type E;
+    constexpr int WAVES = WM * WN, NI = TN / WN / 32, MJ = TM / WM / 32, STAGE = (TM + TN) * 64, LOADS = (TM + TN) / 16 / WAVES;
+    __shared__ __attribute__((aligned(1024))) int8_t s_ring[4 * STAGE];
+    const int tile = vx_xcd_tile(blockIdx.x, gm * gn);
+    if (tile < 0) return;
+    // eight tiles of tokens by four of channels are in flight on an XCD: its L2 holds what they share
+    const int band = tile / (8 * gn), in_band = tile - band * 8 * gn, bh = min(8, gm - band * 8);
+    const long long m0 = (long long)(band * 8 + in_band % bh) * TM, n0 = (long long)(in_band / bh) * TN;
+    const int lane = vx_lane(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+    const int steps = (K + 63) >> 6;
+
+    // rows of the stage that this wave loads: 16 for each of its LOADS instructions, 4 lanes a row
+    const int8_t *src[LOADS];
+    int piece[LOADS];                                             // the piece of the row that lands in the lane's slot
+    bool is_w[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const int r = (i * WAVES + wave) * 16 + (lane >> 2);
+        is_w[i] = (i * WAVES + wave) * 16 < TN;
+        piece[i] = (((lane & 3) ^ ((r >> 1) & 3))) * 16;
+        src[i] = is_w[i] ? w + min(n0 + r, N - 1) * ws : q + min(m0 + r - TN, M - 1) * qs;
+    }
+    auto request = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int k = t * 64 + piece[i];
+            const int8_t *g = src[i] + (is_w[i] && k >= K ? 0 : k);
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)g,
+                                             (__attribute__((address_space(3))) void *)(s_ring + (t & 3) * STAGE + (i * WAVES + wave) * 1024),
+                                             16, 0, 0);
+        }
+    };
+    // lane's byte offsets of its operands inside a stage, for the two halves of 32 bytes
+    const int lr = lane & 31;
+    int at_w[2], at_q[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int p = ((2 * h + (lane >> 5)) ^ ((lr >> 1) & 3)) * 16;
+        at_w[h] = (wn * (TN / WN) + lr) * 64 + p;
+        at_q[h] = (TN + wm * (TM / WM) + lr) * 64 + p;
+    }
+    vx_i4 fw[2][2][NI], fq[2][2][MJ];
+    auto fetch = [&](int t, int set) {
+        const int8_t *base = s_ring + (t & 3) * STAGE;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) fw[set][h][i] = *(const vx_i4 *)(base + at_w[h] + i * 2048);
+#pragma unroll
+            for (int j = 0; j < MJ; ++j) fq[set][h][j] = *(const vx_i4 *)(base + at_q[h] + j * 2048);
+        }
+    };
+    vx_i16 acc[NI][MJ];
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < MJ; ++j)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) acc[i][j][k] = 0;
+    auto multiply = [&](int set) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+#pragma unroll
+                for (int j = 0; j < MJ; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[set][h][i], fq[set][h][j], acc[i][j], 0, 0, 0);
+    };
+    // waits until step t is in LDS for every wave; steps t + 1 .. may still be on their way
+    auto arrive = [&](int t) {
+        const int later = min(steps - 1, t + 2) - t;              // steps requested behind t
+        if (later >= 2) vx_wait_stage<2 * LOADS>();
+        else if (later == 1) vx_wait_stage<LOADS>();
+        else vx_wait_stage<0>();
+    };
+
+#pragma unroll
+    for (int t = 0; t < 3; ++t)
+        if (t < steps) request(t);
+    arrive(0);
+    if (3 < steps) request(3);
+    fetch(0, 0);
+    auto step = [&](int t, int set) {
+        if (t + 1 < steps) {
+            arrive(t + 1);                                        // and every wave holds its operands of step t: the slot is free
+            if (t + 4 < steps) request(t + 4);
+            fetch(t + 1, set ^ 1);
+        }
+        multiply(set);
+    };
+    for (int t = 0; t < steps; t += 2) {
+        step(t, 0);
+        if (t + 1 < steps) step(t + 1, 1);
+    }
+
+    // accumulator r of a tile: channel 8 (r / 4) + 4 (lane / 32) + r % 4, token lane % 32
+#pragma unroll
+    for (int j = 0; j < MJ; ++j) {
+        const long long m = m0 + wm * (TM / WM) + j * 32 + lr;
+        if (m >= M) continue;
+        const float sm = s[m];
+        E *row = (E *)out + m * os;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const long long n = n0 + wn * (TN / WN) + i * 32 + 8 * g + 4 * (lane >> 5);
+                union { E e[4]; vx_v2 v2; vx_v4 v4; } o;
+                if (n + 4 <= N) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) o.e[k] = vx_store_cast<DT>(vx_linear_out(acc[i][j][4 * g + k], sm, sw[n + k], bias, n + k));
+                    if (sizeof(E) == 2) *(vx_v2_at2 *)(row + n) = o.v2;
+                    else *(vx_v4_at4 *)(row + n) = o.v4;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (n + k < N) row[n + k] = vx_store_cast<DT>(vx_linear_out(acc[i][j][4 * g + k], sm, sw[n + k], bias, n + k));
+                }
+            }
+    }
+}
+
+// rows of K bytes to rows of `pitch` (a multiple of 64), padded with zeros
+__global__ __launch_bounds__(256) void vx_k_pad_rows(const int8_t *__restrict__ src, long long stride, long long rows, int K,
+                                                     int8_t *__restrict__ dst, int pitch) {
+    const int pieces = pitch / 16;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= rows * pieces) return;
+    const long long r = i / pieces;
+    const int k = (int)(i - r * pieces) * 16;
+    const int8_t *row = src + r * stride;
+    *(vx_i4 *)(dst + r * pitch + k) = k + 16 <= K ? (vx_i4)*(const vx_i4_at1 *)(row + k) : vx_i8_tail(row, k, K);
+}
+
+#define VX_STREAM_MAX 64          // tokens of the streaming kernel
+
+static size_t vx_up256(size_t n) { return (n + 255) & ~(size_t)255; }
+static long long vx_k_pitch(int K) { return ((long long)K + 63) / 64 * 64; }
+
+// q_padded: columns K .. vx_k_pitch(K) - 1 of q are zeros.  pad: 256-byte aligned room for the padded copies that
+// vx_linear_i8_workspace_bytes counts.
+static int vx_linear_launch(const int8_t *q, long long qs, bool q_padded, const float *s, long long M, const int8_t *w, long long ws,
                             const float *sw, long long N, int K, const float *bias, void *out, int out_dtype, long long os,
-                            hipStream_t st) {
-    const dim3 grid((unsigned)((N + 63) / 64), (unsigned)((M + 63) / 64));
+                            int8_t *pad, hipStream_t st) {
+    const long long pitch = vx_k_pitch(K);
+    bool tiles = M > VX_STREAM_MAX;
     vx_prof_begin(VX_PROF_LINEAR, st);
-    VX_DISPATCH_DTYPE(out_dtype, hipLaunchKernelGGL((vx_k_linear_i8<DT>), grid, dim3(256), 0, st, q, qs, s, M, w, ws, sw, N, K,
-                                                    bias, out, os));
+    if (tiles) {
+        if (K % 64 && !q_padded) {
+            const long long n = M * (pitch / 16);
+            hipLaunchKernelGGL(vx_k_pad_rows, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, q, qs, M, K, pad, (int)pitch);
+            q = pad;
+            qs = pitch;
+            pad += vx_up256((size_t)(M * pitch));
+        }
+        if (K % 16) {
+            const long long n = N * (pitch / 16);
+            hipLaunchKernelGGL(vx_k_pad_rows, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, w, ws, N, K, pad, (int)pitch);
+            w = pad;
+            ws = pitch;
+        }
+        // rows at odd addresses go by the streaming kernel, 64 tokens at a time
+        tiles = !(((uintptr_t)q | (uintptr_t)w) & 15) && !((qs | ws) & 15);
+    }
+    if (tiles) {
+        const long long big = ((M + 255) / 256) * ((N + 255) / 256);
+        VX_DISPATCH_DTYPE(out_dtype, {
+            if (big >= 256) {
+                const int gm = (int)((M + 255) / 256), gn = (int)((N + 255) / 256);
+                hipLaunchKernelGGL((vx_k_linear_tile<DT, 256, 256, 2, 4>), dim3((unsigned)(8 * ((big + 7) / 8))), dim3(512), 0, st, q, qs, s,
+                                   M, w, ws, sw, N, K, bias, out, os, gm, gn);
+            } else {
+                const int gm = (int)((M + 127) / 128), gn = (int)((N + 127) / 128);
+                hipLaunchKernelGGL((vx_k_linear_tile<DT, 128, 128, 2, 2>), dim3((unsigned)(8 * (((long long)gm * gn + 7) / 8))), dim3(256), 0,
+                                   st, q, qs, s, M, w, ws, sw, N, K, bias, out, os, gm, gn);
+            }
+        });
+    } else {
+        const int mt = (int)min(4LL, (M + 15) / 16);
+        const int waves = N <= 4096 ? 16 : 4;                     // few channels: more of K side by side
+        const dim3 grid((unsigned)((N + 15) / 16), (unsigned)((M + 16 * mt - 1) / (16 * mt)));
+        const size_t lds = (size_t)waves * mt * 1024;
+        VX_DISPATCH_DTYPE(out_dtype, {
+            if (mt == 1) hipLaunchKernelGGL((vx_k_linear_stream<DT, 1>), grid, dim3(waves * 64), lds, st, q, qs, s, M, w, ws, sw, N, K, bias, out, os);
+            else if (mt == 2) hipLaunchKernelGGL((vx_k_linear_stream<DT, 2>), grid, dim3(waves * 64), lds, st, q, qs, s, M, w, ws, sw, N, K, bias, out, os);
+            else if (mt == 3) hipLaunchKernelGGL((vx_k_linear_stream<DT, 3>), grid, dim3(waves * 64), lds, st, q, qs, s, M, w, ws, sw, N, K, bias, out, os);
+            else hipLaunchKernelGGL((vx_k_linear_stream<DT, 4>), grid, dim3(waves * 64), lds, st, q, qs, s, M, w, ws, sw, N, K, bias, out, os);
+        });
+    }
     vx_prof_end(VX_PROF_LINEAR, st);
     return hipGetLastError() == hipSuccess ? VX_OK : VX_ERR_LAUNCH;
 }
@@ -113,8 +406,19 @@ static int vx_linear_check(const void *a, long long as, const int8_t *w, long lo
     return VX_OK;
 }
 
+static bool vx_linear_sizes_ok(int64_t M, int64_t N, int K) {
+    return M > 0 && N > 0 && K > 0 && M <= VX_MAX_LINEAR_ROWS && N <= VX_MAX_LINEAR_ROWS && K <= VX_MAX_I8_DEPTH;
+}
+
+// the padded copies of vx_linear_launch
+static size_t vx_linear_pad_bytes(int64_t M, int64_t N, int K, bool q_padded) {
+    if (M <= VX_STREAM_MAX) return 0;
+    const size_t pitch = (size_t)vx_k_pitch(K);
+    return (K % 64 && !q_padded ? vx_up256((size_t)M * pitch) : 0) + (K % 16 ? vx_up256((size_t)N * pitch) : 0);
+}
+
 extern "C" size_t vx_linear_i8_workspace_bytes(int64_t M, int64_t N, int K) {
-    return M <= 0 || N <= 0 || K <= 0 || M > VX_MAX_LINEAR_ROWS || N > VX_MAX_LINEAR_ROWS || K > VX_MAX_I8_DEPTH ? 0 : 256;
+    return vx_linear_sizes_ok(M, N, K) ? 256 + vx_linear_pad_bytes(M, N, K, false) : 0;
 }
 
 extern "C" int vx_linear_i8(const int8_t *d_q, int64_t q_stride, const float *d_scale, int64_t M, const int8_t *d_w,
@@ -125,15 +429,13 @@ extern "C" int vx_linear_i8(const int8_t *d_q, int64_t q_stride, const float *d_
     if (rc != VX_OK) return rc;
     if (((uintptr_t)d_scale & 3) || ((uintptr_t)d_workspace & 255)) return VX_ERR_ALIGNMENT;
     if (workspace_bytes < vx_linear_i8_workspace_bytes(M, N, K)) return VX_ERR_WORKSPACE;
-    return vx_linear_launch(d_q, q_stride, d_scale, M, d_w, w_stride, d_w_scale, N, K, d_bias, d_out, out_dtype, out_stride,
-                            (hipStream_t)stream);
+    return vx_linear_launch(d_q, q_stride, false, d_scale, M, d_w, w_stride, d_w_scale, N, K, d_bias, d_out, out_dtype, out_stride,
+                            (int8_t *)d_workspace, (hipStream_t)stream);
 }
 
-static size_t vx_up256(size_t n) { return (n + 255) & ~(size_t)255; }
-
 extern "C" size_t vx_linear_w8a8_workspace_bytes(int64_t M, int64_t N, int K) {
-    const size_t rest = vx_linear_i8_workspace_bytes(M, N, K);
-    return rest ? rest + vx_up256((size_t)M * 4) + vx_up256((size_t)M * (size_t)K) : 0;
+    if (!vx_linear_sizes_ok(M, N, K)) return 0;
+    return 256 + vx_up256((size_t)M * 4) + vx_up256((size_t)(M * vx_k_pitch(K))) + vx_linear_pad_bytes(M, N, K, true);
 }
 
 extern "C" int vx_linear_w8a8(const void *d_x, int x_dtype, int64_t x_stride, int64_t M, const int8_t *d_w, int64_t w_stride,
@@ -145,9 +447,10 @@ extern "C" int vx_linear_w8a8(const void *d_x, int x_dtype, int64_t x_stride, in
     if (((uintptr_t)d_x & (vx_elem_size(x_dtype) - 1)) || ((uintptr_t)d_workspace & 255)) return VX_ERR_ALIGNMENT;
     if (workspace_bytes < vx_linear_w8a8_workspace_bytes(M, N, K)) return VX_ERR_WORKSPACE;
     hipStream_t st = (hipStream_t)stream;
+    const long long pitch = vx_k_pitch(K);
     float *s = (float *)d_workspace;
-    int8_t *q = (int8_t *)d_workspace + vx_up256((size_t)M * 4);
-    rc = vx_quant_launch(d_x, x_dtype, M, K, x_stride, q, K, s, st);
+    int8_t *q = (int8_t *)d_workspace + vx_up256((size_t)M * 4), *pad = q + vx_up256((size_t)(M * pitch));
+    rc = vx_quant_launch(d_x, x_dtype, M, K, x_stride, q, pitch, s, st);
     if (rc != VX_OK) return rc;
-    return vx_linear_launch(q, K, s, M, d_w, w_stride, d_w_scale, N, K, d_bias, d_out, out_dtype, out_stride, st);
+    return vx_linear_launch(q, pitch, true, s, M, d_w, w_stride, d_w_scale, N, K, d_bias, d_out, out_dtype, out_stride, pad, st);
 }

@@ -520,7 +520,10 @@ def _linear_weights(qw, w_scale, bias, K: int, dev):
         _tensor(bias, "bias", dev, (torch.float32,), 1)
         _need(bias.numel() == N, "bias has %d values for %d channels" % (bias.numel(), N))
         bias = bias.contiguous()
-    return _rows(qw, "qw"), w_scale.contiguous(), bias, N
+    qw = _rows(qw, "qw")
+    if K % 16 == 0 and (qw.data_ptr() % 16 or qw.stride(0) % 16):
+        qw = qw.contiguous()                     # a slice of wider rows: the tile kernel takes 16-byte aligned ones
+    return qw, w_scale.contiguous(), bias, N
 
 
 @_on_device
