@@ -108,10 +108,9 @@ typedef int vx_i16 __attribute__((ext_vector_type(16)));
 typedef vx_i4 vx_i4_at1 __attribute__((aligned(1)));
 
 // y for one output; the same expression in every kernel, so that all variants give the same bits
-__device__ __forceinline__ float vx_linear_out(int acc, float s, float sw, const float *bias, long long n) {
-    float y = (float)acc * (s * sw);
-    if (bias) y = y + bias[n];
-    return y;
+__device__ __forceinline__ float vx_linear_out(int acc, float s, float sw, bool has_bias, float bias) {
+    const float y = (float)acc * (s * sw);
+    return has_bias ? y + bias : y;
 }
 
 // ---- few tokens: the weights stream once from memory into registers, no LDS between.
@@ -181,7 +180,7 @@ __global__ __launch_bounds__(1024) void vx_k_linear_stream(const int8_t *__restr
         int sum = 0;
         for (int k = 0; k < waves; ++k) sum += s_part[k * MT * 256 + i];
         const long long m = m0 + (i >> 4), n = n0 + (i & 15);
-        if (m < M && n < N) ((E *)out)[m * os + n] = vx_store_cast<DT>(vx_linear_out(sum, s[m], sw[n], bias, n));
+        if (m < M && n < N) ((E *)out)[m * os + n] = vx_store_cast<DT>(vx_linear_out(sum, s[m], sw[n], bias != nullptr, bias ? bias[n] : 0.f));
     }
 }
 
@@ -194,7 +193,10 @@ __global__ __launch_bounds__(1024) void vx_k_linear_stream(const int8_t *__restr
 // Needs 16-byte aligned rows; q padded with zeros to a multiple of 64, w's pieces beyond K read as piece 0 (K % 16 == 0).
 template <int N>
 __device__ __forceinline__ void vx_wait_stage() {                 // at most N loads and no LDS read outstanding, then the barrier
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+    __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (0 << 8) | ((N >> 4) << 14));
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
 template <int DT, int TM, int TN, int WM, int WN>
@@ -227,15 +229,16 @@ __global__ __launch_bounds__(WM * WN * 64) void vx_k_linear_tile(const int8_t *_
         piece[i] = (((lane & 3) ^ ((r >> 1) & 3))) * 16;
         src[i] = is_w[i] ? w + min(n0 + r, N - 1) * ws : q + min(m0 + r - TN, M - 1) * qs;
     }
+    auto request1 = [&](int t, int i) {
+        const int k = t * 64 + piece[i];
+        const int8_t *g = src[i] + (is_w[i] && k >= K ? 0 : k);
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)g,
+                                         (__attribute__((address_space(3))) void *)(s_ring + (t & 3) * STAGE + (i * WAVES + wave) * 1024),
+                                         16, 0, 0);
+    };
     auto request = [&](int t) {
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const int k = t * 64 + piece[i];
-            const int8_t *g = src[i] + (is_w[i] && k >= K ? 0 : k);
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)g,
-                                             (__attribute__((address_space(3))) void *)(s_ring + (t & 3) * STAGE + (i * WAVES + wave) * 1024),
-                                             16, 0, 0);
-        }
+        for (int i = 0; i < LOADS; ++i) request1(t, i);
     };
     // lane's byte offsets of its operands inside a stage, for the two halves of 32 bytes
     const int lr = lane & 31;
@@ -295,35 +298,94 @@ __global__ __launch_bounds__(WM * WN * 64) void vx_k_linear_tile(const int8_t *_
         }
         multiply(set);
     };
-    for (int t = 0; t < steps; t += 2) {
+    // the same without a branch: an LDS read or a request in front of each matrix instruction, in this order
+    auto steady = [&](int t, int set) {
+        constexpr int READS = 2 * (NI + MJ), MULS = 2 * NI * MJ;
+        vx_wait_stage<2 * LOADS>();
+        const int8_t *base = s_ring + ((t + 1) & 3) * STAGE;
+#pragma unroll
+        for (int k = 0; k < (MULS > READS + LOADS ? MULS : READS + LOADS); ++k) {
+            if (k < READS) {
+                const int h = k / (NI + MJ), r = k % (NI + MJ);
+                if (r < NI) fw[set ^ 1][h][r] = *(const vx_i4 *)(base + at_w[h] + r * 2048);
+                else fq[set ^ 1][h][r - NI] = *(const vx_i4 *)(base + at_q[h] + (r - NI) * 2048);
+            } else if (k < READS + LOADS) {
+                request1(t + 4, k - READS);
+            }
+            if (k < MULS) {
+                const int h = k / (NI * MJ), i = k / MJ % NI, j = k % MJ;
+                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[set][h][i], fq[set][h][j], acc[i][j], 0, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    int t = 0;
+    for (; t + 5 < steps; t += 2) {
+        steady(t, 0);
+        steady(t + 1, 1);
+    }
+    for (; t < steps; t += 2) {
         step(t, 0);
         if (t + 1 < steps) step(t + 1, 1);
     }
 
-    // accumulator r of a tile: channel 8 (r / 4) + 4 (lane / 32) + r % 4, token lane % 32
+    // Results.  Accumulator r of a tile: channel 8 (r / 4) + 4 (lane / 32) + r % 4, token lane % 32.  Stored from there, a
+    // wave's store would touch 32 rows with 16 bytes each (400 of 900 us at 8192 x 16384 x 4096); instead they go through
+    // the wave's part of the ring, 32 tokens at a time, and leave as whole rows of its channels.  A row's 16-byte pieces are
+    // stored at piece ^ (row & 7): writes and reads both spread over all banks.
+    constexpr int CH = TN / WN, PIECES = CH * (int)sizeof(E) / 16, ROWS = 64 / PIECES;       // rows of one store instruction
+    static_assert(WAVES * 32 * CH * 4 <= 4 * STAGE, "a wave's 32 rows of results fit its part of the ring");
+    vx_wait_stage<0>();                                           // every wave is done with the ring
+    int8_t *mine = s_ring + wave * (32 * CH * 4);
+    const long long nw = n0 + wn * CH;
+    float scale[NI][4][4], plus[NI][4][4];
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const long long n = min(nw + i * 32 + 8 * g + 4 * (lane >> 5) + k, N - 1);
+                scale[i][g][k] = sw[n];
+                plus[i][g][k] = bias ? bias[n] : 0.f;
+            }
 #pragma unroll
     for (int j = 0; j < MJ; ++j) {
-        const long long m = m0 + wm * (TM / WM) + j * 32 + lr;
-        if (m >= M) continue;
-        const float sm = s[m];
-        E *row = (E *)out + m * os;
+        const long long mj = m0 + wm * (TM / WM) + j * 32;
+        const float sm = s[min(mj + lr, M - 1)];
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const long long n = n0 + wn * (TN / WN) + i * 32 + 8 * g + 4 * (lane >> 5);
                 union { E e[4]; vx_v2 v2; vx_v4 v4; } o;
-                if (n + 4 <= N) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) o.e[k] = vx_store_cast<DT>(vx_linear_out(acc[i][j][4 * g + k], sm, sw[n + k], bias, n + k));
-                    if (sizeof(E) == 2) *(vx_v2_at2 *)(row + n) = o.v2;
-                    else *(vx_v4_at4 *)(row + n) = o.v4;
+                for (int k = 0; k < 4; ++k)
+                    o.e[k] = vx_store_cast<DT>(vx_linear_out(acc[i][j][4 * g + k], sm, scale[i][g][k], bias != nullptr, plus[i][g][k]));
+                const int col = (i * 32 + 8 * g + 4 * (lane >> 5)) * (int)sizeof(E), piece = (col >> 4) ^ (lr & (PIECES < 8 ? PIECES - 1 : 7));
+                int8_t *to = mine + lr * (CH * (int)sizeof(E)) + piece * 16 + (col & 15);
+                if (sizeof(E) == 2) *(vx_v2 *)to = o.v2;
+                else *(vx_v4 *)to = o.v4;
+            }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int r0 = 0; r0 < 32; r0 += ROWS) {
+            const int r = r0 + lane / PIECES, p = lane % PIECES;
+            union { vx_v4 v; E e[16 / sizeof(E)]; } o;
+            o.v = *(const vx_v4 *)(mine + r * (CH * (int)sizeof(E)) + (p ^ (r & (PIECES < 8 ? PIECES - 1 : 7))) * 16);
+            const long long m = mj + r, n = nw + p * (16 / (int)sizeof(E));
+            if (m < M) {
+                E *to = (E *)out + m * os + n;
+                if (n + 16 / (int)sizeof(E) <= N) {
+                    if (sizeof(E) == 2) *(vx_v4_at2 *)to = o.v;
+                    else *(vx_v4_at4 *)to = o.v;
                 } else {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (n + k < N) row[n + k] = vx_store_cast<DT>(vx_linear_out(acc[i][j][4 * g + k], sm, sw[n + k], bias, n + k));
+                    for (int k = 0; k < 16 / (int)sizeof(E); ++k)
+                        if (n + k < N) to[k] = o.e[k];
                 }
             }
+        }
     }
 }
 
