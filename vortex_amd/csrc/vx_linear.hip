@@ -186,11 +186,14 @@ __global__ __launch_bounds__(1024) void vx_k_linear_stream(const int8_t *__restr
 
 // ---- many tokens: TM x TN outputs for each workgroup, WM x WN waves of 32x32x32 mfma tiles (weights as rows, tokens as
 // columns, so a lane's four accumulators in a row are four neighbouring channels of one token).
-// K goes by 64 bytes through a ring of four LDS stages that the loads fill directly; each wave's operands of step t + 1 are
-// read into registers while the matrix instructions of step t run, and step t + 4 is requested once step t's slot is free.
-// An LDS row is 64 bytes; its 16-byte pieces are stored at piece ^ ((row >> 1) & 3), so the eight rows that one quarter of a
-// 16-byte LDS read covers lie in all banks.
-// Needs 16-byte aligned rows; q padded with zeros to a multiple of 64, w's pieces beyond K read as piece 0 (K % 16 == 0).
+// K goes by stages of 128 bytes, a whole cache line of each row (requests of 64 bytes found the line of the request before
+// still on its way), through LDS that the loads fill directly: three stages of weights, two of tokens, all 160 KB of a
+// compute unit.  A stage is worked off in two halves; each wave reads its operands of the next half into registers while
+// the matrix instructions of this one run.  One barrier a stage: behind it stage d + 1 is there for every wave and nobody
+// reads stage d any more.
+// The 16-byte pieces of an LDS row are stored at piece ^ ((row >> 1) & 7), so the 16 rows that a quarter of a wave's 16-byte
+// LDS read covers lie in all 64 banks.
+// Needs 16-byte aligned rows; q padded with zeros to a multiple of 128, w's pieces beyond K read as piece 0 (K % 16 == 0).
 template <int N>
 __device__ __forceinline__ void vx_wait_stage() {                 // at most N loads and no LDS read outstanding, then the barrier
     __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (0 << 8) | ((N >> 4) << 14));
@@ -207,8 +210,10 @@ __global__ __launch_bounds__(WM * WN * 64) void vx_k_linear_tile(const int8_t *_
                                                                  const float *__restrict__ bias, void *__restrict__ out,
                                                                  long long os, int gm, int gn) {
     typedef typename vx_elem<DT>::type E;
-    constexpr int WAVES = WM * WN, NI = TN / WN / 32, MJ = TM / WM / 32, STAGE = (TM + TN) * 64, LOADS = (TM + TN) / 16 / WAVES;
-    __shared__ __attribute__((aligned(1024))) int8_t s_ring[4 * STAGE];
+    constexpr int WAVES = WM * WN, NI = TN / WN / 32, MJ = TM / WM / 32;
+    constexpr int LW = TN / 8 / WAVES, LQ = TM / 8 / WAVES;       // loads of one wave for a stage, 8 rows each
+    constexpr int RING = 3 * TN * 128 + 2 * TM * 128;
+    __shared__ __attribute__((aligned(1024))) int8_t s_ring[RING];
     const int tile = vx_xcd_tile(blockIdx.x, gm * gn);
     if (tile < 0) return;
     // eight tiles of tokens by four of channels are in flight on an XCD: its L2 holds what they share
@@ -216,50 +221,35 @@ __global__ __launch_bounds__(WM * WN * 64) void vx_k_linear_tile(const int8_t *_
     const long long m0 = (long long)(band * 8 + in_band % bh) * TM, n0 = (long long)(in_band / bh) * TN;
     const int lane = vx_lane(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
-    const int steps = (K + 63) >> 6;
+    const int stages = (K + 127) >> 7;
 
-    // rows of the stage that this wave loads: 16 for each of its LOADS instructions, 4 lanes a row
-    const int8_t *src[LOADS];
-    int piece[LOADS];                                             // the piece of the row that lands in the lane's slot
-    bool is_w[LOADS];
+    // what this wave loads of a stage: 8 rows with each instruction, 8 lanes a row; the lane's slot holds piece `piece`
+    const int8_t *src_w[LW], *src_q[LQ];
+    const int row8 = wave * 8 + (lane >> 3), piece = ((lane & 7) ^ ((row8 >> 1) & 7)) * 16;  // the same for rows 8 WAVES further
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-        const int r = (i * WAVES + wave) * 16 + (lane >> 2);
-        is_w[i] = (i * WAVES + wave) * 16 < TN;
-        piece[i] = (((lane & 3) ^ ((r >> 1) & 3))) * 16;
-        src[i] = is_w[i] ? w + min(n0 + r, N - 1) * ws : q + min(m0 + r - TN, M - 1) * qs;
-    }
-    auto request1 = [&](int t, int i) {
-        const int k = t * 64 + piece[i];
-        const int8_t *g = src[i] + (is_w[i] && k >= K ? 0 : k);
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)g,
-                                         (__attribute__((address_space(3))) void *)(s_ring + (t & 3) * STAGE + (i * WAVES + wave) * 1024),
+    for (int i = 0; i < LW; ++i) src_w[i] = w + min(n0 + i * WAVES * 8 + row8, N - 1) * ws;
+#pragma unroll
+    for (int i = 0; i < LQ; ++i) src_q[i] = q + min(m0 + i * WAVES * 8 + row8, M - 1) * qs + piece;
+    auto request_w = [&](int d, int slot, int i) {
+        const int k = d * 128 + piece;
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src_w[i] + (k < K ? k : 0)),
+                                         (__attribute__((address_space(3))) void *)(s_ring + slot + (i * WAVES + wave) * 1024), 16, 0, 0);
+    };
+    auto request_q = [&](int d, int i) {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src_q[i] + d * 128),
+                                         (__attribute__((address_space(3))) void *)(s_ring + 3 * TN * 128 + (d & 1) * TM * 128 + (i * WAVES + wave) * 1024),
                                          16, 0, 0);
     };
-    auto request = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) request1(t, i);
-    };
-    // lane's byte offsets of its operands inside a stage, for the two halves of 32 bytes
+    // the lane's byte offsets of its operands inside a stage, for its four quarters of 32 bytes
     const int lr = lane & 31;
-    int at_w[2], at_q[2];
+    int at_w[4], at_q[4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int p = ((2 * h + (lane >> 5)) ^ ((lr >> 1) & 3)) * 16;
-        at_w[h] = (wn * (TN / WN) + lr) * 64 + p;
-        at_q[h] = (TN + wm * (TM / WM) + lr) * 64 + p;
+    for (int h = 0; h < 4; ++h) {
+        const int p = ((2 * h + (lane >> 5)) ^ ((lr >> 1) & 7)) * 16;
+        at_w[h] = (wn * (TN / WN) + lr) * 128 + p;
+        at_q[h] = 3 * TN * 128 + (wm * (TM / WM) + lr) * 128 + p;
     }
-    vx_i4 fw[2][2][NI], fq[2][2][MJ];
-    auto fetch = [&](int t, int set) {
-        const int8_t *base = s_ring + (t & 3) * STAGE;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int i = 0; i < NI; ++i) fw[set][h][i] = *(const vx_i4 *)(base + at_w[h] + i * 2048);
-#pragma unroll
-            for (int j = 0; j < MJ; ++j) fq[set][h][j] = *(const vx_i4 *)(base + at_q[h] + j * 2048);
-        }
-    };
+    vx_i4 fw[2][2][NI], fq[2][2][MJ];                             // operands of the two halves of a stage
     vx_i16 acc[NI][MJ];
 #pragma unroll
     for (int i = 0; i < NI; ++i)
@@ -267,50 +257,20 @@ __global__ __launch_bounds__(WM * WN * 64) void vx_k_linear_tile(const int8_t *_
         for (int j = 0; j < MJ; ++j)
 #pragma unroll
             for (int k = 0; k < 16; ++k) acc[i][j][k] = 0;
-    auto multiply = [&](int set) {
+    // Half `set` of a stage: its matrix instructions, with an LDS read (of half set ^ 1: of this stage, or of the next one)
+    // or a request in front of each, in this order.
+    auto half = [&](int set, bool read, int base_w, int base_q, auto request, int requests) {
+        constexpr int READS = 2 * (NI + MJ), MULS = 2 * NI * MJ, TOTAL = READS + (LW > LQ ? LW : LQ);
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < NI; ++i)
-#pragma unroll
-                for (int j = 0; j < MJ; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[set][h][i], fq[set][h][j], acc[i][j], 0, 0, 0);
-    };
-    // waits until step t is in LDS for every wave; steps t + 1 .. may still be on their way
-    auto arrive = [&](int t) {
-        const int later = min(steps - 1, t + 2) - t;              // steps requested behind t
-        if (later >= 2) vx_wait_stage<2 * LOADS>();
-        else if (later == 1) vx_wait_stage<LOADS>();
-        else vx_wait_stage<0>();
-    };
-
-#pragma unroll
-    for (int t = 0; t < 3; ++t)
-        if (t < steps) request(t);
-    arrive(0);
-    if (3 < steps) request(3);
-    fetch(0, 0);
-    auto step = [&](int t, int set) {
-        if (t + 1 < steps) {
-            arrive(t + 1);                                        // and every wave holds its operands of step t: the slot is free
-            if (t + 4 < steps) request(t + 4);
-            fetch(t + 1, set ^ 1);
-        }
-        multiply(set);
-    };
-    // the same without a branch: an LDS read or a request in front of each matrix instruction, in this order
-    auto steady = [&](int t, int set) {
-        constexpr int READS = 2 * (NI + MJ), MULS = 2 * NI * MJ;
-        vx_wait_stage<2 * LOADS>();
-        const int8_t *base = s_ring + ((t + 1) & 3) * STAGE;
-#pragma unroll
-        for (int k = 0; k < (MULS > READS + LOADS ? MULS : READS + LOADS); ++k) {
+        for (int k = 0; k < (MULS > TOTAL ? MULS : TOTAL); ++k) {
             if (k < READS) {
-                const int h = k / (NI + MJ), r = k % (NI + MJ);
-                if (r < NI) fw[set ^ 1][h][r] = *(const vx_i4 *)(base + at_w[h] + r * 2048);
-                else fq[set ^ 1][h][r - NI] = *(const vx_i4 *)(base + at_q[h] + (r - NI) * 2048);
-            } else if (k < READS + LOADS) {
-                request1(t + 4, k - READS);
+                const int h = k / (NI + MJ), r = k % (NI + MJ), h4 = 2 * (set ^ 1) + h;
+                if (read) {
+                    if (r < NI) fw[set ^ 1][h][r] = *(const vx_i4 *)(s_ring + base_w + at_w[h4] + r * 4096);
+                    else fq[set ^ 1][h][r - NI] = *(const vx_i4 *)(s_ring + base_q + at_q[h4] + (r - NI) * 4096);
+                }
+            } else if (k - READS < requests) {
+                request(k - READS);
             }
             if (k < MULS) {
                 const int h = k / (NI * MJ), i = k / MJ % NI, j = k % MJ;
@@ -319,22 +279,52 @@ __global__ __launch_bounds__(WM * WN * 64) void vx_k_linear_tile(const int8_t *_
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    int t = 0;
-    for (; t + 5 < steps; t += 2) {
-        steady(t, 0);
-        steady(t + 1, 1);
+    auto nothing = [](int) {};
+
+    int slot = 0, slot1 = TN * 128, slot2 = 2 * TN * 128;         // of the weights of stages d, d + 1, d + 2
+#pragma unroll
+    for (int i = 0; i < LW; ++i) request_w(0, slot, i);
+#pragma unroll
+    for (int i = 0; i < LQ; ++i) request_q(0, i);
+    if (stages > 1) {
+#pragma unroll
+        for (int i = 0; i < LW; ++i) request_w(1, slot1, i);
+#pragma unroll
+        for (int i = 0; i < LQ; ++i) request_q(1, i);
+        vx_wait_stage<LW + LQ>();
+    } else {
+        vx_wait_stage<0>();
     }
-    for (; t < steps; t += 2) {
-        step(t, 0);
-        if (t + 1 < steps) step(t + 1, 1);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) fw[0][h][i] = *(const vx_i4 *)(s_ring + at_w[h] + i * 4096);
+#pragma unroll
+        for (int j = 0; j < MJ; ++j) fq[0][h][j] = *(const vx_i4 *)(s_ring + at_q[h] + j * 4096);
+    }
+    int d = 0;
+    for (; d + 2 < stages; ++d) {
+        const int here = (d & 1) * TM * 128, next = TM * 128 - here;
+        half(0, true, slot, here, [&](int i) { request_w(d + 2, slot2, i); }, LW);   // slot2: stage d - 1's, done with since the last barrier
+        vx_wait_stage<LW>();
+        half(1, true, slot1, next, [&](int i) { request_q(d + 2, i); }, LQ);         // into stage d's place
+        const int s0 = slot;
+        slot = slot1; slot1 = slot2; slot2 = s0;
+    }
+    for (; d < stages; ++d) {
+        const int here = (d & 1) * TM * 128, next = TM * 128 - here;
+        half(0, true, slot, here, nothing, 0);
+        vx_wait_stage<0>();
+        half(1, d + 1 < stages, slot1, next, nothing, 0);
+        slot = slot1; slot1 = slot2;
     }
 
     // Results.  Accumulator r of a tile: channel 8 (r / 4) + 4 (lane / 32) + r % 4, token lane % 32.  Stored from there, a
     // wave's store would touch 32 rows with 16 bytes each (400 of 900 us at 8192 x 16384 x 4096); instead they go through
     // the wave's part of the ring, 32 tokens at a time, and leave as whole rows of its channels.  A row's 16-byte pieces are
-    // stored at piece ^ (row & 7): writes and reads both spread over all banks.
+    // stored at piece ^ ((row >> 1) & 7): writes and reads both spread over all banks.
     constexpr int CH = TN / WN, PIECES = CH * (int)sizeof(E) / 16, ROWS = 64 / PIECES;       // rows of one store instruction
-    static_assert(WAVES * 32 * CH * 4 <= 4 * STAGE, "a wave's 32 rows of results fit its part of the ring");
+    static_assert(WAVES * 32 * CH * 4 <= RING, "a wave's 32 rows of results fit its part of the ring");
     vx_wait_stage<0>();                                           // every wave is done with the ring
     int8_t *mine = s_ring + wave * (32 * CH * 4);
     const long long nw = n0 + wn * CH;
@@ -362,7 +352,7 @@ __global__ __launch_bounds__(WM * WN * 64) void vx_k_linear_tile(const int8_t *_
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                     o.e[k] = vx_store_cast<DT>(vx_linear_out(acc[i][j][4 * g + k], sm, scale[i][g][k], bias != nullptr, plus[i][g][k]));
-                const int col = (i * 32 + 8 * g + 4 * (lane >> 5)) * (int)sizeof(E), piece = (col >> 4) ^ (lr & (PIECES < 8 ? PIECES - 1 : 7));
+                const int col = (i * 32 + 8 * g + 4 * (lane >> 5)) * (int)sizeof(E), piece = (col >> 4) ^ ((lr >> 1) & (PIECES < 8 ? PIECES - 1 : 7));
                 int8_t *to = mine + lr * (CH * (int)sizeof(E)) + piece * 16 + (col & 15);
                 if (sizeof(E) == 2) *(vx_v2 *)to = o.v2;
                 else *(vx_v4 *)to = o.v4;
@@ -372,7 +362,7 @@ __global__ __launch_bounds__(WM * WN * 64) void vx_k_linear_tile(const int8_t *_
         for (int r0 = 0; r0 < 32; r0 += ROWS) {
             const int r = r0 + lane / PIECES, p = lane % PIECES;
             union { vx_v4 v; E e[16 / sizeof(E)]; } o;
-            o.v = *(const vx_v4 *)(mine + r * (CH * (int)sizeof(E)) + (p ^ (r & (PIECES < 8 ? PIECES - 1 : 7))) * 16);
+            o.v = *(const vx_v4 *)(mine + r * (CH * (int)sizeof(E)) + (p ^ ((r >> 1) & (PIECES < 8 ? PIECES - 1 : 7))) * 16);
             const long long m = mj + r, n = nw + p * (16 / (int)sizeof(E));
             if (m < M) {
                 E *to = (E *)out + m * os + n;
@@ -389,7 +379,7 @@ __global__ __launch_bounds__(WM * WN * 64) void vx_k_linear_tile(const int8_t *_
     }
 }
 
-// rows of K bytes to rows of `pitch` (a multiple of 64), padded with zeros
+// rows of K bytes to rows of `pitch` (a multiple of 128), padded with zeros
 __global__ __launch_bounds__(256) void vx_k_pad_rows(const int8_t *__restrict__ src, long long stride, long long rows, int K,
                                                      int8_t *__restrict__ dst, int pitch) {
     const int pieces = pitch / 16;
@@ -404,7 +394,7 @@ __global__ __launch_bounds__(256) void vx_k_pad_rows(const int8_t *__restrict__ 
 #define VX_STREAM_MAX 64          // tokens of the streaming kernel
 
 static size_t vx_up256(size_t n) { return (n + 255) & ~(size_t)255; }
-static long long vx_k_pitch(int K) { return ((long long)K + 63) / 64 * 64; }
+static long long vx_k_pitch(int K) { return ((long long)K + 127) / 128 * 128; }
 
 // q_padded: columns K .. vx_k_pitch(K) - 1 of q are zeros.  pad: 256-byte aligned room for the padded copies that
 // vx_linear_i8_workspace_bytes counts.
@@ -415,7 +405,7 @@ static int vx_linear_launch(const int8_t *q, long long qs, bool q_padded, const 
     bool tiles = M > VX_STREAM_MAX;
     vx_prof_begin(VX_PROF_LINEAR, st);
     if (tiles) {
-        if (K % 64 && !q_padded) {
+        if (K % 128 && !q_padded) {
             const long long n = M * (pitch / 16);
             hipLaunchKernelGGL(vx_k_pad_rows, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, q, qs, M, K, pad, (int)pitch);
             q = pad;
@@ -476,7 +466,7 @@ static bool vx_linear_sizes_ok(int64_t M, int64_t N, int K) {
 static size_t vx_linear_pad_bytes(int64_t M, int64_t N, int K, bool q_padded) {
     if (M <= VX_STREAM_MAX) return 0;
     const size_t pitch = (size_t)vx_k_pitch(K);
-    return (K % 64 && !q_padded ? vx_up256((size_t)M * pitch) : 0) + (K % 16 ? vx_up256((size_t)N * pitch) : 0);
+    return (K % 128 && !q_padded ? vx_up256((size_t)M * pitch) : 0) + (K % 16 ? vx_up256((size_t)N * pitch) : 0);
 }
 
 extern "C" size_t vx_linear_i8_workspace_bytes(int64_t M, int64_t N, int K) {
