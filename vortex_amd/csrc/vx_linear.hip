@@ -4,41 +4,38 @@
 #include "vx_dtype.h"
 #include "vx_profile.h"
 
-// rint(127 x / amax), exactly (ties to even), for x and amax of the input type.
+// rint(127 x / amax), exactly (ties to even), for x and amax of the input type, by division:
 //  16-bit types: 127 x is exact in fp32 (11 + 7 bits) and the quotient of an (11+7)-bit by an 11-bit number, at most 127,
 //  is either a tie itself or further than 2^-12 from one: the rounded fp32 quotient falls on the same side.
 //  fp32: the same argument holds for fp64 (24 + 7 bits over 24 bits: at least 2^-25 from a tie, rounding 2^-47).
 template <int DT>
-__device__ __forceinline__ int vx_quant1(float x, float amax) {
-    if (DT == VX_DTYPE_F32) return (int)rint(((double)x * 127.0) / (double)amax);
-    return (int)rintf((x * 127.0f) / amax);
+__device__ __forceinline__ float vx_quant_exact(float x, float amax) {
+    if (DT == VX_DTYPE_F32) return (float)rint(((double)x * 127.0) / (double)amax);
+    return rintf((x * 127.0f) / amax);
 }
 
-// WAVES waves per row.  The row's values stay in registers between the two passes (maximum, quotients) up to
-// WAVES * 64 * VEC * U of them; longer rows are read again.  A row with a NaN or an infinity gets the scale NaN (and q = 0):
-// its products are all NaN.  Bound by the read of x.
-template <int DT, int WAVES>
+// WAVES waves per row, U 16-byte pieces of it in the registers of each lane between the two passes (maximum, quotients);
+// longer rows are read again.  The quotient is a product with r = 127 / amax, off by at most 3 roundings of a value up to
+// 127 (127 * 3 * 2^-24 < 2.3e-5); where that could change the integer (closer than 1e-4 to a tie) it is divided: 46 -> 24 us
+// for 8192 x 4096 bf16.  r overflows for amax below 127 / FLT_MAX: such rows are divided throughout.
+// |x| is compared by its bits: they order as the values do, with infinity and NaN above all.  A row that holds one gets the
+// scale NaN (and q = 0): its products are all NaN.
+template <int DT, int WAVES, int U>
 __global__ __launch_bounds__(256) void vx_k_quant_rows(const void *__restrict__ x, long long M, int K, long long xs,
                                                        int8_t *__restrict__ q, long long qs, float *__restrict__ scale) {
     typedef typename vx_elem<DT>::type E;
-    constexpr int VEC = 16 / sizeof(E), U = 4, THREADS = WAVES * 64;
-    __shared__ float s_max[4];
-    __shared__ int s_bad[4];
+    constexpr int VEC = 16 / sizeof(E), THREADS = WAVES * 64;
+    __shared__ unsigned s_max[4];
     const int w = threadIdx.x >> 6, tid = WAVES == 1 ? vx_lane() : (int)threadIdx.x;
     const long long m = WAVES == 1 ? (long long)blockIdx.x * 4 + w : (long long)blockIdx.x;
     if (m >= M) return;                                           // WAVES == 1 has no barrier behind this
     const E *row = (const E *)x + m * xs;
-    float mx = 0.f;
-    bool bad = false;
+    unsigned top = 0;
     vx_vec<DT> v[U];
     const bool once = K <= THREADS * VEC * U;
     auto look = [&](const vx_vec<DT> &a) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-            const float f = fabsf((float)a.e[k]);
-            bad |= !(f <= 3.4028234663852886e38f);
-            mx = fmaxf(mx, f);
-        }
+        for (int k = 0; k < VEC; ++k) top = max(top, __float_as_uint((float)a.e[k]) & 0x7fffffffu);
     };
     if (once) {
 #pragma unroll
@@ -49,20 +46,32 @@ __global__ __launch_bounds__(256) void vx_k_quant_rows(const void *__restrict__ 
         for (int c = tid * VEC; c < K; c += THREADS * VEC) look(vx_load_vec<DT>(row + c, K - c));
     }
 #pragma unroll
-    for (int i = 32; i >= 1; i >>= 1) mx = fmaxf(mx, __shfl_xor(mx, i, VX_WAVE));
-    bad = __any(bad);
+    for (int i = 32; i >= 1; i >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, i, VX_WAVE));
     if (WAVES > 1) {
-        if (vx_lane() == 0) { s_max[w] = mx; s_bad[w] = bad; }
+        if (vx_lane() == 0) s_max[w] = top;
         __syncthreads();
-        mx = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-        bad = s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3];
+        top = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
     }
+    const bool bad = top >= 0x7f800000u, zero = bad || top == 0;
+    const float mx = __uint_as_float(top), r = zero ? 0.f : 127.0f / mx;
+    const bool divide = !zero && !(r <= 3.4028234663852886e38f);
     int8_t *dst = q + m * qs;
-    const bool zero = bad || mx == 0.f;
     auto put = [&](const vx_vec<DT> &a, int c) {
         union { int8_t b[VEC]; unsigned w[VEC / 4]; } o;
+        float t[VEC];
+        bool near = divide;
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) o.b[k] = zero ? 0 : (int8_t)vx_quant1<DT>((float)a.e[k], mx);
+        for (int k = 0; k < VEC; ++k) {
+            const float y = zero ? 0.f : (float)a.e[k] * r;
+            t[k] = rintf(y);
+            near |= fabsf(y - t[k]) > 0.4999f;
+        }
+        if (near) {
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) t[k] = vx_quant_exact<DT>((float)a.e[k], mx);
+        }
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) o.b[k] = (int8_t)(int)t[k];
         if (c + VEC <= qs) {                                      // columns K .. qs - 1 come out as 0
             typedef unsigned u32_at1 __attribute__((aligned(1)));
 #pragma unroll
@@ -84,12 +93,15 @@ __global__ __launch_bounds__(256) void vx_k_quant_rows(const void *__restrict__ 
 
 static int vx_quant_launch(const void *x, int dtype, long long M, int K, long long xs, int8_t *q, long long qs, float *s, hipStream_t st) {
     vx_prof_begin(VX_PROF_QUANT, st);
-    // a row that one wave holds needs no barrier
+    // a row that one wave holds needs no barrier; with few rows four waves share one
     VX_DISPATCH_DTYPE(dtype, {
-        if (K <= 64 * 4 * 16 / vx_elem_size(DT))
-            hipLaunchKernelGGL((vx_k_quant_rows<DT, 1>), dim3((unsigned)((M + 3) / 4)), dim3(256), 0, st, x, M, K, xs, q, qs, s);
+        constexpr int PIECE = 64 * 16 / (int)sizeof(typename vx_elem<DT>::type);
+        if (K <= 4 * PIECE && M >= 256)
+            hipLaunchKernelGGL((vx_k_quant_rows<DT, 1, 4>), dim3((unsigned)((M + 3) / 4)), dim3(256), 0, st, x, M, K, xs, q, qs, s);
+        else if (K <= 8 * PIECE && M >= 256)
+            hipLaunchKernelGGL((vx_k_quant_rows<DT, 1, 8>), dim3((unsigned)((M + 3) / 4)), dim3(256), 0, st, x, M, K, xs, q, qs, s);
         else
-            hipLaunchKernelGGL((vx_k_quant_rows<DT, 4>), dim3((unsigned)M), dim3(256), 0, st, x, M, K, xs, q, qs, s);
+            hipLaunchKernelGGL((vx_k_quant_rows<DT, 4, 4>), dim3((unsigned)M), dim3(256), 0, st, x, M, K, xs, q, qs, s);
     });
     vx_prof_end(VX_PROF_QUANT, st);
     return hipGetLastError() == hipSuccess ? VX_OK : VX_ERR_LAUNCH;
