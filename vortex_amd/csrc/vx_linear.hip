@@ -177,11 +177,21 @@ __global__ __launch_bounds__(1024) void vx_k_linear_stream(const int8_t *__restr
         for (int t = 0; t < MT; ++t)
             acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, *(const vx_i4_at1 *)(qrow[t] + b * 64 + koff), acc[t], 0, 0, 0);
     }
-    if (b < end) {                                                // the last 64 bytes stick out of the rows
-        const vx_i4 a = vx_i8_tail(wrow, b * 64 + koff, K);
+    if (b < end) {
+        // The last 64 bytes stick out of the rows.  The tokens' bytes from K on are made 0, so the channels' may be anything
+        // that lies inside the matrix: only its last rows are read byte by byte.
+        const int k = b * 64 + koff;
+        const vx_i4 a = wrow + k + 16 <= w + (N - 1) * ws + K ? (vx_i4)*(const vx_i4_at1 *)(wrow + k) : vx_i8_tail(wrow, k, K);
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
-            acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, vx_i8_tail(qrow[t], b * 64 + koff, K), acc[t], 0, 0, 0);
+        for (int t = 0; t < MT; ++t) {
+            vx_i4 x = qrow[t] + k + 16 <= q + (M - 1) * qs + K ? (vx_i4)*(const vx_i4_at1 *)(qrow[t] + k) : vx_i8_tail(qrow[t], k, K);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int left = K - k - 4 * i;                   // bytes of this word inside the row
+                x[i] = left >= 4 ? x[i] : (left <= 0 ? 0 : x[i] & (int)(0xffffffffu >> (32 - 8 * left)));
+            }
+            acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, x, acc[t], 0, 0, 0);
+        }
     }
     // lane l holds token l % 16, channels 4 (l / 16) .. + 3
 #pragma unroll
