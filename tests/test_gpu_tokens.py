@@ -252,7 +252,8 @@ def product_ref(q, s, qw, sw, bias, dt):
 
 LINEAR_SHAPES = [(1, 1, 1), (1, 3, 16), (1, 1000, 64), (2, 257, 1000), (5, 130, 127), (15, 64, 2048), (16, 1024, 1024), (17, 255, 1024), (31, 1000, 513),
                  (32, 96, 4096), (33, 2048, 96), (64, 64, 64), (65, 129, 192), (100, 300, 1025), (128, 512, 256), (200, 255, 1024), (257, 259, 321),
-                 (300, 1000, 4096), (513, 70, 128), (1030, 515, 640)]
+                 (300, 1000, 4096), (513, 70, 128), (1030, 515, 640),
+                 (33, 16400, 64), (9, 16384, 160), (16, 16385, 320), (8, 20000, 100), (17, 16385, 144), (64, 17000, 272), (2049, 2100, 192), (4000, 3000, 16), (130, 12300, 80), (48, 20001, 200)]
 
 
 @pytest.mark.parametrize("M,N,K", LINEAR_SHAPES)

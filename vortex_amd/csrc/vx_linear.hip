@@ -3,6 +3,7 @@
 //   y[m,n] = s_m * sw_n * (sum_k q[m,k] w[n,k]) + bias_n          (the sum is exact in 32-bit integers: K <= 131072)
 #include "vx_dtype.h"
 #include "vx_profile.h"
+#include <type_traits>
 
 // rint(127 x / amax), exactly (ties to even), for x and amax of the input type, by division:
 //  16-bit types: 127 x is exact in fp32 (11 + 7 bits) and the quotient of an (11+7)-bit by an 11-bit number, at most 127,
@@ -126,8 +127,9 @@ __device__ __forceinline__ float vx_linear_out(int acc, float s, float sw, bool 
 }
 
 // ---- few tokens: the weights stream once from memory into registers, no LDS between.
-// One workgroup per 16 channels, its waves share K; mfma 16x16x64 with the weights as rows: lane l holds 16 bytes of channel
-// l % 16 at k = 64 b + 16 (l / 16), and MT tiles of 16 tokens stand against them.
+// One workgroup per 16 NT channels, its waves share K; mfma 16x16x64 with the weights as rows: lane l holds 16 bytes of
+// channel l % 16 at k = 64 b + 16 (l / 16), and MT tiles of 16 tokens stand against them.  Bound by the read of the weights:
+// 131 MB in 21 us (6.2 TB/s) for one token against 32000 x 4096.
 __device__ __forceinline__ vx_i4 vx_i8_tail(const int8_t *row, int k, int K) {      // bytes k .. k+15, 0 from K on
     union { vx_i4 v; int8_t b[16]; } o;
     o.v = vx_i4{0, 0, 0, 0};
@@ -137,71 +139,86 @@ __device__ __forceinline__ vx_i4 vx_i8_tail(const int8_t *row, int k, int K) {  
     return o.v;
 }
 
-template <int DT, int MT>
+template <int DT, int MT, int NT>
 __global__ __launch_bounds__(1024) void vx_k_linear_stream(const int8_t *__restrict__ q, long long qs, const float *__restrict__ s,
                                                           long long M, const int8_t *__restrict__ w, long long ws,
                                                           const float *__restrict__ sw, long long N, int K,
                                                           const float *__restrict__ bias, void *__restrict__ out, long long os) {
     typedef typename vx_elem<DT>::type E;
-    constexpr int UN = MT == 1 ? 8 : 4;
-    extern __shared__ int s_part[];                               // [waves][MT][16 tokens][16 channels]
+    constexpr int UN = MT * NT == 1 ? 8 : (MT + NT <= 4 ? 4 : 2);
+    extern __shared__ int s_part[];                               // [waves][MT][16 tokens][16 NT channels]
     const int lane = vx_lane(), wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const long long n0 = (long long)blockIdx.x * 16, m0 = (long long)blockIdx.y * 16 * MT;
-    const int8_t *wrow = w + min(n0 + (lane & 15), N - 1) * ws;
-    const int8_t *qrow[MT];
+    const long long n0 = (long long)blockIdx.x * 16 * NT, m0 = (long long)blockIdx.y * 16 * MT;
+    const int8_t *wrow[NT], *qrow[MT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) wrow[i] = w + min(n0 + i * 16 + (lane & 15), N - 1) * ws;
 #pragma unroll
     for (int t = 0; t < MT; ++t) qrow[t] = q + min(m0 + t * 16 + (lane & 15), M - 1) * qs;
-    vx_i4 acc[MT];
+    vx_i4 acc[NT][MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) acc[t] = vx_i4{0, 0, 0, 0};
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[i][t] = vx_i4{0, 0, 0, 0};
     const int blocks = (K + 63) >> 6, per = (blocks + waves - 1) / waves, full = K >> 6;
     int b = min(blocks, wave * per);
     const int end = min(blocks, b + per), end_full = min(end, full);
     const int koff = (lane >> 4) * 16;
-    for (; b + UN <= end_full; b += UN) {
-        vx_i4 a[UN], x[UN][MT];
+    auto run = [&](auto un) {
+        constexpr int N_ = decltype(un)::value;
+        vx_i4 a[N_][NT], x[N_][MT];
 #pragma unroll
-        for (int u = 0; u < UN; ++u) a[u] = *(const vx_i4_at1 *)(wrow + (b + u) * 64 + koff);
+        for (int u = 0; u < N_; ++u) {
 #pragma unroll
-        for (int u = 0; u < UN; ++u)
+            for (int i = 0; i < NT; ++i) a[u][i] = *(const vx_i4_at1 *)(wrow[i] + (b + u) * 64 + koff);
+        }
+#pragma unroll
+        for (int u = 0; u < N_; ++u) {
 #pragma unroll
             for (int t = 0; t < MT; ++t) x[u][t] = *(const vx_i4_at1 *)(qrow[t] + (b + u) * 64 + koff);
+        }
 #pragma unroll
-        for (int u = 0; u < UN; ++u)
+        for (int u = 0; u < N_; ++u)
 #pragma unroll
-            for (int t = 0; t < MT; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u], x[u][t], acc[t], 0, 0, 0);
-    }
-    for (; b < end_full; ++b) {
-        const vx_i4 a = *(const vx_i4_at1 *)(wrow + b * 64 + koff);
+            for (int i = 0; i < NT; ++i)
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
-            acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, *(const vx_i4_at1 *)(qrow[t] + b * 64 + koff), acc[t], 0, 0, 0);
-    }
+                for (int t = 0; t < MT; ++t) acc[i][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u][i], x[u][t], acc[i][t], 0, 0, 0);
+        b += N_;
+    };
+    while (b + UN <= end_full) run(std::integral_constant<int, UN>());
+    while (b < end_full) run(std::integral_constant<int, 1>());
     if (b < end) {
         // The last 64 bytes stick out of the rows.  The tokens' bytes from K on are made 0, so the channels' may be anything
         // that lies inside the matrix: only its last rows are read byte by byte.
         const int k = b * 64 + koff;
-        const vx_i4 a = wrow + k + 16 <= w + (N - 1) * ws + K ? (vx_i4)*(const vx_i4_at1 *)(wrow + k) : vx_i8_tail(wrow, k, K);
+        vx_i4 a[NT], x[MT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+            a[i] = wrow[i] + k + 16 <= w + (N - 1) * ws + K ? (vx_i4)*(const vx_i4_at1 *)(wrow[i] + k) : vx_i8_tail(wrow[i], k, K);
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-            vx_i4 x = qrow[t] + k + 16 <= q + (M - 1) * qs + K ? (vx_i4)*(const vx_i4_at1 *)(qrow[t] + k) : vx_i8_tail(qrow[t], k, K);
+            x[t] = qrow[t] + k + 16 <= q + (M - 1) * qs + K ? (vx_i4)*(const vx_i4_at1 *)(qrow[t] + k) : vx_i8_tail(qrow[t], k, K);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int left = K - k - 4 * i;                   // bytes of this word inside the row
-                x[i] = left >= 4 ? x[i] : (left <= 0 ? 0 : x[i] & (int)(0xffffffffu >> (32 - 8 * left)));
+                x[t][i] = left >= 4 ? x[t][i] : (left <= 0 ? 0 : x[t][i] & (int)(0xffffffffu >> (32 - 8 * left)));
             }
-            acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, x, acc[t], 0, 0, 0);
         }
-    }
-    // lane l holds token l % 16, channels 4 (l / 16) .. + 3
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
-        *(vx_i4 *)&s_part[((wave * MT + t) * 16 + (lane & 15)) * 16 + (lane >> 4) * 4] = acc[t];
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[i][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i], x[t], acc[i][t], 0, 0, 0);
+    }
+    // lane l holds token l % 16, channels 4 (l / 16) .. + 3 of each tile
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+            *(vx_i4 *)&s_part[((wave * MT + t) * 16 + (lane & 15)) * 16 * NT + i * 16 + (lane >> 4) * 4] = acc[i][t];
     __syncthreads();
-    for (int i = threadIdx.x; i < MT * 256; i += blockDim.x) {
+    for (int i = threadIdx.x; i < MT * NT * 256; i += blockDim.x) {
         int sum = 0;
-        for (int k = 0; k < waves; ++k) sum += s_part[k * MT * 256 + i];
-        const long long m = m0 + (i >> 4), n = n0 + (i & 15);
+        for (int k = 0; k < waves; ++k) sum += s_part[k * MT * NT * 256 + i];
+        const long long m = m0 + i / (16 * NT), n = n0 + i % (16 * NT);
         if (m < M && n < N) ((E *)out)[m * os + n] = vx_store_cast<DT>(vx_linear_out(sum, s[m], sw[n], bias != nullptr, bias ? bias[n] : 0.f));
     }
 }
@@ -215,6 +232,8 @@ __global__ __launch_bounds__(1024) void vx_k_linear_stream(const int8_t *__restr
 // reads stage d any more.
 // The 16-byte pieces of an LDS row are stored at piece ^ ((row >> 1) & 7), so the 16 rows that a quarter of a wave's 16-byte
 // LDS read covers lie in all 64 banks.
+// 8192 x 16384 x 4096: 500 us, 2.2 PFLOP/s of int8; the matrix instructions are busy 57 % of the cycles, at a clock that the
+// card has brought down to 1.7 GHz.
 // Needs 16-byte aligned rows; q padded with zeros to a multiple of 128, w's pieces beyond K read as piece 0 (K % 16 == 0).
 template <int N>
 __device__ __forceinline__ void vx_wait_stage() {                 // at most N loads and no LDS read outstanding, then the barrier
@@ -413,10 +432,28 @@ __global__ __launch_bounds__(256) void vx_k_pad_rows(const int8_t *__restrict__ 
     *(vx_i4 *)(dst + r * pitch + k) = k + 16 <= K ? (vx_i4)*(const vx_i4_at1 *)(row + k) : vx_i8_tail(row, k, K);
 }
 
-#define VX_STREAM_MAX 64          // tokens of the streaming kernel
+// Which kernel takes M tokens (us of the product alone; N x K, weights from memory):
+//   M <= 8: streaming (32000 x 4096: 30 against 33 by 64 x 64 tiles; at M = 16 36 against 33)
+//   M <= 64: streaming with few channels or an odd K, which the tiles would have to copy (8192 x 8192, M = 32: 27 against 30;
+//            50021 x 1000, M = 37: 23), 64 x 64 tiles from 16384 channels on (32000 x 4096, M = 32: 33 against 43)
+//   more: the largest tile that gives at least 192 workgroups, three for four compute units (8192 x 4096: M = 1536, 192 tiles
+//   of 256: 54 against 60 by 128; M = 1024, 128 tiles: 48 against 41.  8192 x 8192, M = 128, 64 tiles of 128: 43 against 33 by
+//   64; M = 512, 256 tiles: 47 against 58)
+#define VX_STREAM_MAX 64
+static bool vx_linear_streams(int64_t M, int64_t N, int K) {
+    return M <= 8 || (M <= VX_STREAM_MAX && (N < 16384 || K % 16 != 0));
+}
 
 static size_t vx_up256(size_t n) { return (n + 255) & ~(size_t)255; }
 static long long vx_k_pitch(int K) { return ((long long)K + 127) / 128 * 128; }
+
+template <int DT, int T, int WM, int WN>
+static void vx_linear_tiles(const int8_t *q, long long qs, const float *s, long long M, const int8_t *w, long long ws, const float *sw,
+                            long long N, int K, const float *bias, void *out, long long os, hipStream_t st) {
+    const int gm = (int)((M + T - 1) / T), gn = (int)((N + T - 1) / T);
+    hipLaunchKernelGGL((vx_k_linear_tile<DT, T, T, WM, WN>), dim3((unsigned)(8 * (((long long)gm * gn + 7) / 8))), dim3(WM * WN * 64), 0, st,
+                       q, qs, s, M, w, ws, sw, N, K, bias, out, os, gm, gn);
+}
 
 // q_padded: columns K .. vx_k_pitch(K) - 1 of q are zeros.  pad: 256-byte aligned room for the padded copies that
 // vx_linear_i8_workspace_bytes counts.
@@ -424,7 +461,7 @@ static int vx_linear_launch(const int8_t *q, long long qs, bool q_padded, const 
                             const float *sw, long long N, int K, const float *bias, void *out, int out_dtype, long long os,
                             int8_t *pad, hipStream_t st) {
     const long long pitch = vx_k_pitch(K);
-    bool tiles = M > VX_STREAM_MAX;
+    bool tiles = !vx_linear_streams(M, N, K);
     vx_prof_begin(VX_PROF_LINEAR, st);
     if (tiles) {
         if (K % 128 && !q_padded) {
@@ -444,28 +481,24 @@ static int vx_linear_launch(const int8_t *q, long long qs, bool q_padded, const 
         tiles = !(((uintptr_t)q | (uintptr_t)w) & 15) && !((qs | ws) & 15);
     }
     if (tiles) {
-        const long long big = ((M + 255) / 256) * ((N + 255) / 256);
+        auto count = [&](int t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
         VX_DISPATCH_DTYPE(out_dtype, {
-            if (big >= 256) {
-                const int gm = (int)((M + 255) / 256), gn = (int)((N + 255) / 256);
-                hipLaunchKernelGGL((vx_k_linear_tile<DT, 256, 256, 2, 4>), dim3((unsigned)(8 * ((big + 7) / 8))), dim3(512), 0, st, q, qs, s,
-                                   M, w, ws, sw, N, K, bias, out, os, gm, gn);
-            } else {
-                const int gm = (int)((M + 127) / 128), gn = (int)((N + 127) / 128);
-                hipLaunchKernelGGL((vx_k_linear_tile<DT, 128, 128, 2, 2>), dim3((unsigned)(8 * (((long long)gm * gn + 7) / 8))), dim3(256), 0,
-                                   st, q, qs, s, M, w, ws, sw, N, K, bias, out, os, gm, gn);
-            }
+            if (count(256) >= 192) vx_linear_tiles<DT, 256, 2, 4>(q, qs, s, M, w, ws, sw, N, K, bias, out, os, st);
+            else if (count(128) >= 192) vx_linear_tiles<DT, 128, 2, 2>(q, qs, s, M, w, ws, sw, N, K, bias, out, os, st);
+            else vx_linear_tiles<DT, 64, 2, 2>(q, qs, s, M, w, ws, sw, N, K, bias, out, os, st);
         });
     } else {
-        const int mt = (int)min(4LL, (M + 15) / 16);
-        const int waves = N <= 4096 ? 16 : 4;                     // few channels: more of K side by side
-        const dim3 grid((unsigned)((N + 15) / 16), (unsigned)((M + 16 * mt - 1) / (16 * mt)));
-        const size_t lds = (size_t)waves * mt * 1024;
+        // two tiles of channels share the tokens' loads where there is more than one tile of tokens (37 x 50021 x 1000: 30 ->
+        // 23 us with two waves); few channels: more waves side by side along K
+        const int mt = (int)min(4LL, (M + 15) / 16), nt = mt == 1 ? 1 : 2;
+        const int waves = N <= 4096 ? 16 / nt : (K <= 2048 && mt > 1 ? 2 : 4);
+        const dim3 grid((unsigned)((N + 16 * nt - 1) / (16 * nt)), (unsigned)((M + 16 * mt - 1) / (16 * mt)));
+        const size_t lds = (size_t)waves * mt * nt * 1024;
         VX_DISPATCH_DTYPE(out_dtype, {
-            if (mt == 1) hipLaunchKernelGGL((vx_k_linear_stream<DT, 1>), grid, dim3(waves * 64), lds, st, q, qs, s, M, w, ws, sw, N, K, bias, out, os);
-            else if (mt == 2) hipLaunchKernelGGL((vx_k_linear_stream<DT, 2>), grid, dim3(waves * 64), lds, st, q, qs, s, M, w, ws, sw, N, K, bias, out, os);
-            else if (mt == 3) hipLaunchKernelGGL((vx_k_linear_stream<DT, 3>), grid, dim3(waves * 64), lds, st, q, qs, s, M, w, ws, sw, N, K, bias, out, os);
-            else hipLaunchKernelGGL((vx_k_linear_stream<DT, 4>), grid, dim3(waves * 64), lds, st, q, qs, s, M, w, ws, sw, N, K, bias, out, os);
+            if (mt == 1) hipLaunchKernelGGL((vx_k_linear_stream<DT, 1, 1>), grid, dim3(waves * 64), lds, st, q, qs, s, M, w, ws, sw, N, K, bias, out, os);
+            else if (mt == 2) hipLaunchKernelGGL((vx_k_linear_stream<DT, 2, 2>), grid, dim3(waves * 64), lds, st, q, qs, s, M, w, ws, sw, N, K, bias, out, os);
+            else if (mt == 3) hipLaunchKernelGGL((vx_k_linear_stream<DT, 3, 2>), grid, dim3(waves * 64), lds, st, q, qs, s, M, w, ws, sw, N, K, bias, out, os);
+            else hipLaunchKernelGGL((vx_k_linear_stream<DT, 4, 2>), grid, dim3(waves * 64), lds, st, q, qs, s, M, w, ws, sw, N, K, bias, out, os);
         });
     }
     vx_prof_end(VX_PROF_LINEAR, st);
@@ -486,7 +519,7 @@ static bool vx_linear_sizes_ok(int64_t M, int64_t N, int K) {
 
 // the padded copies of vx_linear_launch
 static size_t vx_linear_pad_bytes(int64_t M, int64_t N, int K, bool q_padded) {
-    if (M <= VX_STREAM_MAX) return 0;
+    if (vx_linear_streams(M, N, K)) return 0;
     const size_t pitch = (size_t)vx_k_pitch(K);
     return (K % 128 && !q_padded ? vx_up256((size_t)M * pitch) : 0) + (K % 16 ? vx_up256((size_t)N * pitch) : 0);
 }
