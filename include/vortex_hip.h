@@ -390,7 +390,8 @@ int vx_linear_w8a8(const void *d_x, int x_dtype, int64_t x_stride, int64_t M, co
  * d_temperature[b] not above 0: greedy -- x_j is accepted iff it is the first arg-max of target row j (d_accept 1 or 0), the
  * token behind is the arg-max of row n; the draft logits and d_uniforms are not used.  d_uniforms [B, K+1] in [0, 1).
  * -inf masks a token (in either distribution).  K = 0 draws one token from each row 0.
- * Everything is fp64 from the logits on.  d_status[b] (written, not ORed): VX_STATUS_NAN a NaN or +inf in a row that is used,
+ * The drawn token and every accepted / rejected are decided in fp64 from the logits on; d_accept is within 2^-15 relative.
+ * d_status[b] (written, not ORed): VX_STATUS_NAN a NaN or +inf in a row that is used,
  * VX_STATUS_EMPTY_ROW all of such a row is -inf, VX_STATUS_BAD_TOKEN a drafted token outside [0, V) (it is rejected).  A
  * draft is rejected at an invalid row; where the row that is drawn from is invalid, the token behind is -1.
  * Rows behind n_b, and their drafted tokens, are not read.  The workspace is 256-byte aligned. */

@@ -5,8 +5,18 @@
 //   n = the number accepted; the token behind them is the first i with sum_{<=i} r > u_{b,K} sum r,
 //       r = max(0, p_n - q_n) when a draft was rejected, r = p_n behind the last draft
 // T_b not above 0: greedy (x_j is accepted iff it is the first arg-max of its row; the token behind is the arg-max).
-// Exponentials, sums and the cumulative sum are fp64: the outcome is a whole number decided by where a cumulative sum
-// passes a border, and one step of a flat distribution is 1/V.
+//
+// Three launches over chunks of the vocabulary:
+//   stats   every used row: largest logit and fp32 sum of exponentials of each chunk (bound by the one read of the logits;
+//           fp64 exponentials here would take twice the time of the read)
+//   choose  the accepted drafts and the row to draw from; that row's (and the draft row's) chunk sums again in fp64
+//   draw    chunk sums of max(0, p - q) in fp64, the last workgroup of a sequence finds the token
+// The token that is drawn is a whole number, decided by where a cumulative sum passes a border, and one step of a flat
+// distribution is 1/V: everything it depends on is fp64.  The sums of the first launch are within 2^-17 of the true ones:
+//   an exponential is off by 2^-23 (the instruction) + ln2 |t| 3 * 2^-24 (difference, factor, product), t its exponent to
+//   base 2 below the largest; weighted with the distribution |t| averages at most log2 V <= 30 (it is the entropy less log2
+//   of the sum): 3.9e-6; at most 64 additions follow one another: 3.8e-6.
+// So a test u q < p is taken from them unless its sides are within 2^-15 of each other; then both rows are summed in fp64.
 #include "vx_dtype.h"
 #include "vx_profile.h"
 
@@ -17,210 +27,473 @@ struct vx_verify_args {
     const int *lens;                              // [B] or nullptr
     const float *uniforms;                        // [B, K + 1]
     const float *temperature;                     // [B]
-    int B, K, V;
+    int B, K, V, chunks;
+    // workspace
+    float2 *stats;                                // [B][2 K + 1][chunks]: largest logit (NaN: an invalid one), sum (greedy: index)
+    double2 *z;                                   // [B][chunks]: sums of the row that is drawn from, target and draft
+    double *r;                                    // [B][chunks]: sums of max(0, p - q)
+    struct vx_choice *choice;                     // [B]
+    int *ticket;                                  // [B]
+    // outputs
+    long long *out;                               // [B, K + 1]
+    int *counts, *status;
+    float *accept;
 };
 
-struct vx_row_stat {                              // of one row of logits
-    double z;                                     // sum of exp((x - m) / T)
-    float m;                                      // largest logit
-    int best;                                     // its first index
-    int status;
-    int pad;
+struct vx_choice {                                // what is left to do for a sequence
+    int row;                                      // number of accepted drafts = the row that is drawn from
+    int mode;                                     // 0: the token is known or there is none; 1: from p; 2: from p without `drop`; 3: from max(0, p - q)
+    float mp, mq;                                 // largest logits of the two rows
+    long long drop;
 };
+
+// chunk of a row: 256 threads x U pieces of 16 bytes
+#define VX_VERIFY_U 4
+template <int DT> __host__ __device__ constexpr int vx_verify_chunk() { return 256 * VX_VERIFY_U * 16 / (int)sizeof(typename vx_elem<DT>::type); }
 
 __device__ __forceinline__ int vx_verify_len(const vx_verify_args &a, int b) {
     return a.lens ? vx_clamp_count(a.lens[b], a.K) : a.K;
 }
-
-// weight of a logit against the row's largest one; T > 0.  A masked (-inf) logit weighs 0 whatever T is.
-__device__ __forceinline__ double vx_weight(float x, float m, double inv_t) {
-    return x == -INFINITY ? 0.0 : exp(((double)x - (double)m) * inv_t);
+template <int DT>
+__device__ __forceinline__ const typename vx_elem<DT>::type *vx_verify_target(const vx_verify_args &a, int b, int j) {
+    return (const typename vx_elem<DT>::type *)a.target + b * a.t_seq + j * a.t_row;
+}
+template <int DT>
+__device__ __forceinline__ const typename vx_elem<DT>::type *vx_verify_draft(const vx_verify_args &a, int b, int j) {
+    return (const typename vx_elem<DT>::type *)a.draft + b * a.d_seq + j * a.d_row;
 }
 
-// One workgroup per (sequence, row): target rows 0..K, then draft rows 0..K-1.
+// 2^t for t <= 0: t = n + f, |f| <= 1/2, and the series of e^(f ln 2) up to its 12th term (the 13th is below 2e-16).
+// Below -1000, and for the NaN of -inf * 0 (a masked logit at an infinite temperature), 0.
+__device__ __forceinline__ double vx_exp2_64(double t) {
+    t = fmax(t, -1000.0);
+    const double n = rint(t), f = (t - n) * 0.69314718055994530942;
+    double p = 1.0 / 479001600.0;
+    p = __builtin_fma(p, f, 1.0 / 39916800.0);
+    p = __builtin_fma(p, f, 1.0 / 3628800.0);
+    p = __builtin_fma(p, f, 1.0 / 362880.0);
+    p = __builtin_fma(p, f, 1.0 / 40320.0);
+    p = __builtin_fma(p, f, 1.0 / 5040.0);
+    p = __builtin_fma(p, f, 1.0 / 720.0);
+    p = __builtin_fma(p, f, 1.0 / 120.0);
+    p = __builtin_fma(p, f, 1.0 / 24.0);
+    p = __builtin_fma(p, f, 1.0 / 6.0);
+    p = __builtin_fma(p, f, 0.5);
+    p = __builtin_fma(p, f, 1.0);
+    p = __builtin_fma(p, f, 1.0);
+    p = ldexp(p, (int)n);
+    return t <= -1000.0 ? 0.0 : p;
+}
+// weight of a logit against the row's largest one; c = log2(e) / T
+__device__ __forceinline__ double vx_weight(float x, float m, double c) {
+    return vx_exp2_64(((double)x - (double)m) * c);
+}
+__device__ __forceinline__ double vx_verify_c(float T) { return 1.44269504088896340736 / (double)T; }
+
+// the thread's values of a chunk, -inf where the row has ended
 template <int DT>
-__global__ __launch_bounds__(256) void vx_k_verify_stats(vx_verify_args a, vx_row_stat *__restrict__ stats) {
-    typedef typename vx_elem<DT>::type E;
-    __shared__ float s_m[4];
-    __shared__ int s_i[4], s_bad[4];
-    __shared__ double s_z[4];
-    const int rows = 2 * a.K + 1, b = blockIdx.x / rows, j = blockIdx.x % rows, n = vx_verify_len(a, b);
+__device__ __forceinline__ void vx_verify_load(const typename vx_elem<DT>::type *row, int c0, int V,
+                                               float x[VX_VERIFY_U * 16 / sizeof(typename vx_elem<DT>::type)]) {
+    constexpr int VEC = 16 / sizeof(typename vx_elem<DT>::type);
+    vx_vec<DT> v[VX_VERIFY_U];
+    if (c0 + vx_verify_chunk<DT>() <= V) {
+#pragma unroll
+        for (int u = 0; u < VX_VERIFY_U; ++u) v[u].raw = vx_load16<DT>(row + c0 + (u * 256 + threadIdx.x) * VEC);
+#pragma unroll
+        for (int u = 0; u < VX_VERIFY_U; ++u)
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) x[u * VEC + k] = (float)v[u].e[k];
+    } else {
+#pragma unroll
+        for (int u = 0; u < VX_VERIFY_U; ++u) {
+            const int at = c0 + (u * 256 + threadIdx.x) * VEC;
+            v[u] = vx_load_vec<DT>(row + at, V - at);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) x[u * VEC + k] = at + k < V ? (float)v[u].e[k] : -INFINITY;
+        }
+    }
+}
+
+// One workgroup per (sequence, row, chunk): target rows 0..K, then draft rows 0..K-1.
+template <int DT>
+__global__ __launch_bounds__(256) void vx_k_verify_stats(vx_verify_args a) {
+    constexpr int VEC = 16 / sizeof(typename vx_elem<DT>::type), PER = VX_VERIFY_U * VEC;
+    __shared__ float s_m[4], s_z[4];
+    __shared__ int s_i[4];
+    const int rows = a.draft ? 2 * a.K + 1 : a.K + 1;
+    const int item = blockIdx.x / a.chunks, chunk = blockIdx.x - item * a.chunks;
+    const int b = item / rows, j = item - b * rows, n = vx_verify_len(a, b);
     const bool is_draft = j > a.K;
     const float T = a.temperature[b];
-    if (is_draft ? (!a.draft || j - a.K - 1 >= n || !(T > 0.f)) : j > n) return;
-    const E *row = is_draft ? (const E *)a.draft + b * a.d_seq + (j - a.K - 1) * a.d_row : (const E *)a.target + b * a.t_seq + j * a.t_row;
-    const int lane = vx_lane(), wave = threadIdx.x >> 6;
+    const bool greedy = !(T > 0.f);
+    if (j == 0 && chunk == 0 && threadIdx.x == 0) a.ticket[b] = 0;
+    if (is_draft ? (j - a.K - 1 >= n || greedy) : j > n) return;
+    float x[PER];
+    const int c0 = chunk * vx_verify_chunk<DT>();
+    vx_verify_load<DT>(is_draft ? vx_verify_draft<DT>(a, b, j - a.K - 1) : vx_verify_target<DT>(a, b, j), c0, a.V, x);
     float m = -INFINITY;
-    int best = 0x7fffffff;
     bool bad = false;
-    for (int i = threadIdx.x; i < a.V; i += 256) {
-        const float x = (float)row[i];
-        bad |= !(x < INFINITY);
-        if (x > m) { m = x; best = i; }
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        bad |= !(x[k] < INFINITY);
+        m = fmaxf(m, x[k]);
     }
-    for (int k = 32; k >= 1; k >>= 1) {
-        const float om = __shfl_xor(m, k, VX_WAVE);
-        const int oi = __shfl_xor(best, k, VX_WAVE);
-        if (om > m || (om == m && oi < best)) { m = om; best = oi; }
+#pragma unroll
+    for (int k = 32; k >= 1; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, VX_WAVE));
+    bad = __any(bad);
+    float z = 0.f;
+    int best = 0x7fffffff;
+    if (greedy) {
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int i = c0 + ((k / VEC) * 256 + threadIdx.x) * VEC + k % VEC;
+            if (x[k] == m) best = min(best, i);
+        }
+#pragma unroll
+        for (int k = 32; k >= 1; k >>= 1) best = min(best, __shfl_xor(best, k, VX_WAVE));
+    } else {
+        const float c = fminf((float)vx_verify_c(T), 3e38f);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) z += __builtin_amdgcn_exp2f(fmaxf((x[k] - m) * c, -200.f));   // -inf - -inf, 0 * inf: NaN, weighs 0
+#pragma unroll
+        for (int k = 32; k >= 1; k >>= 1) z += __shfl_xor(z, k, VX_WAVE);
     }
-    const bool wbad = __any(bad);
-    if (lane == 0) { s_m[wave] = m; s_i[wave] = best; s_bad[wave] = wbad; }
-    __syncthreads();
-    m = s_m[0]; best = s_i[0]; bad = s_bad[0];
-    for (int w = 1; w < 4; ++w) {
-        if (s_m[w] > m || (s_m[w] == m && s_i[w] < best)) { m = s_m[w]; best = s_i[w]; }
-        bad |= s_bad[w];
+    if (vx_lane() == 0) {
+        const int w = threadIdx.x >> 6;
+        s_m[w] = bad ? __builtin_nanf("") : m;
+        s_z[w] = m == -INFINITY ? 0.f : z;
+        s_i[w] = best;
     }
-    const int status = bad ? VX_STATUS_NAN : (m == -INFINITY ? VX_STATUS_EMPTY_ROW : 0);
-    double z = 0.0;
-    if (!status && T > 0.f) {
-        const double inv_t = 1.0 / (double)T;
-        for (int i = threadIdx.x; i < a.V; i += 256) z += vx_weight((float)row[i], m, inv_t);
-    }
-    for (int k = 32; k >= 1; k >>= 1) z += __shfl_xor(z, k, VX_WAVE);
-    if (lane == 0) s_z[wave] = z;
     __syncthreads();
     if (threadIdx.x == 0) {
-        vx_row_stat r;
-        r.z = (s_z[0] + s_z[1]) + (s_z[2] + s_z[3]);
-        r.m = m; r.best = best; r.status = status; r.pad = 0;
-        stats[blockIdx.x] = r;
+        float M = s_m[0];
+        for (int w = 1; w < 4; ++w) M = M != M || s_m[w] != s_m[w] ? __builtin_nanf("") : fmaxf(M, s_m[w]);
+        float out;
+        if (greedy) {
+            int i = 0x7fffffff;
+            for (int w = 0; w < 4; ++w)
+                if (s_m[w] == M) i = min(i, s_i[w]);
+            out = __int_as_float(i);
+        } else {
+            const double c = vx_verify_c(T);
+            double Z = 0.0;
+            for (int w = 0; w < 4; ++w)
+                if (s_z[w] > 0.f) Z += (double)s_z[w] * vx_weight(s_m[w], M, c);
+            out = (float)Z;
+        }
+        a.stats[((long long)b * (2 * a.K + 1) + j) * a.chunks + chunk] = float2{M, out};
     }
 }
 
-struct vx_choice {                                // what is left to do for a sequence
-    int row;                                      // number of accepted drafts = the row that is drawn from
-    int residual;                                 // 1: from max(0, p - q)
-    int token;                                    // >= 0: known already (greedy); -1: draw; -2: none (invalid row)
-};
+// sum over the workgroup's 256 threads, in one order; every thread gets it
+__device__ __forceinline__ double vx_verify_sum(double v, double *s_sum) {
+#pragma unroll
+    for (int k = 32; k >= 1; k >>= 1) v += __shfl_xor(v, k, VX_WAVE);
+    __syncthreads();
+    if (vx_lane() == 0) s_sum[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+}
 
-// One thread per sequence.
+// this thread's part of a chunk's sum of weights
 template <int DT>
-__global__ __launch_bounds__(64) void vx_k_verify_accept(vx_verify_args a, const vx_row_stat *__restrict__ stats,
-                                                         vx_choice *__restrict__ choice, long long *__restrict__ out,
-                                                         int *__restrict__ counts, float *__restrict__ accept,
-                                                         int *__restrict__ status) {
-    typedef typename vx_elem<DT>::type E;
-    const int b = blockIdx.x * 64 + threadIdx.x;
-    if (b >= a.B) return;
-    const int n = vx_verify_len(a, b), K = a.K;
+__device__ __forceinline__ double vx_verify_chunk_sum(const typename vx_elem<DT>::type *row, int chunk, int V, float m, double c) {
+    constexpr int PER = VX_VERIFY_U * 16 / sizeof(typename vx_elem<DT>::type);
+    float x[PER];
+    vx_verify_load<DT>(row, chunk * vx_verify_chunk<DT>(), V, x);
+    double z = 0.0;
+#pragma unroll 4
+    for (int k = 0; k < PER; ++k) z += vx_weight(x[k], m, c);
+    return z;
+}
+
+// One workgroup per (sequence, chunk).  Each takes the decision of its sequence by itself (a few KB of statistics); the first
+// one of a sequence also writes it down.
+template <int DT>
+__global__ __launch_bounds__(256) void vx_k_verify_choose(vx_verify_args a) {
+    __shared__ double s_z[2 * VX_MAX_DRAFTS + 1], s_sum[4];
+    __shared__ float s_m[2 * VX_MAX_DRAFTS + 1];
+    __shared__ int s_best[VX_MAX_DRAFTS + 1];
+    __shared__ u64 s_ok, s_unsure;
+    const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks, K = a.K, n = vx_verify_len(a, b);
+    const int lane = vx_lane(), w = threadIdx.x >> 6;
     const float T = a.temperature[b];
-    const bool greedy = !(T > 0.f);
-    const double inv_t = 1.0 / (double)T;
-    const vx_row_stat *ts = stats + (long long)b * (2 * K + 1), *ds = ts + K + 1;
-    int st = 0, acc = 0;
-    bool going = true;
-    for (int j = 0; j < n; ++j) {
-        const long long x = a.tokens[(long long)b * K + j];
-        const bool in = x >= 0 && x < a.V;
-        double ratio = 0.0;
-        bool ok = false;
-        st |= ts[j].status | (in ? 0 : VX_STATUS_BAD_TOKEN);
-        if (greedy) {
-            ok = !ts[j].status && x == ts[j].best;
-            ratio = ok ? 1.0 : 0.0;
-        } else {
-            const int dst = a.draft ? ds[j].status : 0;
-            st |= dst;
-            if (in && !ts[j].status && !dst) {
-                const double p = vx_weight((float)((const E *)a.target)[b * a.t_seq + j * a.t_row + x], ts[j].m, inv_t) / ts[j].z;
-                const double q = a.draft ? vx_weight((float)((const E *)a.draft)[b * a.d_seq + j * a.d_row + x], ds[j].m, inv_t) / ds[j].z : 1.0;
-                ok = (double)a.uniforms[(long long)b * (K + 1) + j] * q < p;
-                ratio = p >= q ? (p > 0.0 ? 1.0 : 0.0) : p / q;
+    const bool greedy = !(T > 0.f), has_q = a.draft && !greedy;
+    const double c = vx_verify_c(T);
+    // largest logit and sum of each row: one wave a row, its lanes over the chunks
+    for (int i = w; i < (has_q ? 2 * n + 1 : n + 1); i += 4) {
+        const int j = i <= n ? i : K + 1 + (i - n - 1);           // row of the statistics
+        const float2 *st = a.stats + ((long long)b * (2 * K + 1) + j) * a.chunks;
+        float m = -INFINITY;
+        bool bad = false;
+        for (int k = lane; k < a.chunks; k += 64) {
+            const float v = st[k].x;
+            bad |= v != v;
+            m = fmaxf(m, v);
+        }
+#pragma unroll
+        for (int k = 32; k >= 1; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, VX_WAVE));
+        bad = __any(bad);
+        double z = 0.0;
+        int best = 0x7fffffff;
+        if (!bad && m != -INFINITY)
+            for (int k = lane; k < a.chunks; k += 64) {
+                const float2 v = st[k];
+                if (greedy) best = v.x == m ? min(best, __float_as_int(v.y)) : best;
+                else if (v.y > 0.f) z += (double)v.y * vx_weight(v.x, m, c);
+            }
+#pragma unroll
+        for (int k = 32; k >= 1; k >>= 1) {
+            z += __shfl_xor(z, k, VX_WAVE);
+            best = min(best, __shfl_xor(best, k, VX_WAVE));
+        }
+        if (lane == 0) {
+            const int at = i <= n ? i : VX_MAX_DRAFTS + 1 + (i - n - 1);
+            s_m[at] = bad ? __builtin_nanf("") : m;
+            s_z[at] = z;
+            if (i <= n) s_best[i] = best;
+        }
+    }
+    __syncthreads();
+    auto invalid = [](float m) { return m != m ? VX_STATUS_NAN : (m == -INFINITY ? VX_STATUS_EMPTY_ROW : 0); };
+    // lane j of the first wave decides on draft j
+    long long x = 0;
+    double ratio = 0.0, p = 0.0, uq = 0.0;
+    int st = 0;
+    if (w == 0) {
+        bool ok = false, unsure = false;
+        if (lane < n) {
+            x = a.tokens[(long long)b * K + lane];
+            const bool in = x >= 0 && x < a.V;
+            const int t_bad = invalid(s_m[lane]), q_bad = has_q ? invalid(s_m[VX_MAX_DRAFTS + 1 + lane]) : 0;
+            st = t_bad | q_bad | (in ? 0 : VX_STATUS_BAD_TOKEN);
+            if (in && !t_bad && !q_bad) {
+                if (greedy) {
+                    ok = s_best[lane] == x;
+                    ratio = ok ? 1.0 : 0.0;
+                } else {
+                    p = vx_weight((float)vx_verify_target<DT>(a, b, lane)[x], s_m[lane], c) / s_z[lane];
+                    const double q = has_q ? vx_weight((float)vx_verify_draft<DT>(a, b, lane)[x], s_m[VX_MAX_DRAFTS + 1 + lane], c) / s_z[VX_MAX_DRAFTS + 1 + lane] : 1.0;
+                    uq = (double)a.uniforms[(long long)b * (K + 1) + lane] * q;
+                    ok = uq < p;
+                    unsure = p > 0.0 && fabs(uq - p) <= p * (1.0 / 32768.0);
+                    ratio = p >= q ? (p > 0.0 ? 1.0 : 0.0) : p / q;
+                }
             }
         }
-        accept[(long long)b * K + j] = (float)ratio;
-        going = going && ok;
-        if (going) ++acc;
+        const u64 oks = __ballot(ok), un = __ballot(unsure), sure_no = __ballot(lane < n && !ok && !unsure);
+        if (lane == 0) {
+            s_ok = oks;
+            s_unsure = un & (sure_no ? (sure_no & (0 - sure_no)) - 1 : ~0ull);     // those in front of the first certain rejection
+        }
     }
-    st |= ts[n].status;
-    for (int j = n; j < K; ++j) accept[(long long)b * K + j] = 0.f;
-    vx_choice c;
-    c.row = acc;
-    c.residual = acc < n;
-    c.token = -1;
-    if (ts[acc].status || (!greedy && acc < n && a.draft && ds[acc].status)) c.token = -2;
-    else if (greedy) c.token = ts[acc].best;
-    choice[b] = c;
-    for (int j = 0; j <= K; ++j) out[(long long)b * (K + 1) + j] = j < acc ? a.tokens[(long long)b * K + j] : -1;
-    if (c.token >= 0) out[(long long)b * (K + 1) + acc] = c.token;
-    counts[b] = acc + 1;
-    status[b] = st;
+    __syncthreads();
+    for (u64 left = s_unsure; left; left &= left - 1) {
+        const int j = __builtin_ctzll(left);
+        double zp = 0.0, zq = 0.0;
+        for (int k = 0; k < a.chunks; ++k) zp += vx_verify_chunk_sum<DT>(vx_verify_target<DT>(a, b, j), k, a.V, s_m[j], c);
+        if (has_q)
+            for (int k = 0; k < a.chunks; ++k) zq += vx_verify_chunk_sum<DT>(vx_verify_draft<DT>(a, b, j), k, a.V, s_m[VX_MAX_DRAFTS + 1 + j], c);
+        zp = vx_verify_sum(zp, s_sum);
+        zq = vx_verify_sum(zq, s_sum);
+        if (threadIdx.x == j) {                                   // p and u q from the exact sums
+            p = p * s_z[j] / zp;
+            if (has_q) uq = uq * s_z[VX_MAX_DRAFTS + 1 + j] / zq;
+            s_ok = uq < p ? s_ok | (1ull << j) : s_ok & ~(1ull << j);
+        }
+        __syncthreads();
+    }
+    const u64 no = ~s_ok;
+    const int acc = min(n, no ? (int)__builtin_ctzll(no) : 64);
+    const int row_bad = invalid(s_m[acc]), q_bad = has_q && acc < n ? invalid(s_m[VX_MAX_DRAFTS + 1 + acc]) : 0;
+    const int mode = row_bad || q_bad || greedy ? 0 : (acc == n ? 1 : (a.draft ? 3 : 2));
+    const int known = greedy && !row_bad ? s_best[acc] : -1;      // the drawn token comes with the next launch
+    if (chunk == 0 && w == 0) {
+        if (lane < K) {
+            a.accept[(long long)b * K + lane] = lane < n ? (float)ratio : 0.f;
+            a.out[(long long)b * (K + 1) + lane] = lane < acc ? x : (lane == acc ? known : -1);
+        }
+#pragma unroll
+        for (int k = 32; k >= 1; k >>= 1) st |= __shfl_xor(st, k, VX_WAVE);
+        if (lane == 0) {
+            vx_choice ch;
+            ch.row = acc; ch.mode = mode; ch.mp = s_m[acc];
+            ch.mq = mode == 3 ? s_m[VX_MAX_DRAFTS + 1 + acc] : 0.f;
+            ch.drop = mode == 2 ? a.tokens[(long long)b * K + acc] : -1;
+            a.choice[b] = ch;
+            a.counts[b] = acc + 1;
+            a.status[b] = st | invalid(s_m[n]);
+            a.out[(long long)b * (K + 1) + K] = acc == K ? known : -1;
+        }
+    }
+    if (mode == 0) return;
+    const double zp = vx_verify_sum(vx_verify_chunk_sum<DT>(vx_verify_target<DT>(a, b, acc), chunk, a.V, s_m[acc], c), s_sum);
+    const double zq = mode == 3 ? vx_verify_sum(vx_verify_chunk_sum<DT>(vx_verify_draft<DT>(a, b, acc), chunk, a.V, s_m[VX_MAX_DRAFTS + 1 + acc], c), s_sum) : 0.0;
+    if (threadIdx.x == 0) a.z[(long long)b * a.chunks + chunk] = double2{zp, zq};
 }
 
-// One workgroup per sequence that still draws: the sum of the weights, then the place where the cumulative sum passes.
-template <int DT>
-__global__ __launch_bounds__(256) void vx_k_verify_draw(vx_verify_args a, const vx_row_stat *__restrict__ stats,
-                                                        const vx_choice *__restrict__ choice, long long *__restrict__ out) {
-    typedef typename vx_elem<DT>::type E;
-    __shared__ double s_sum[257];
-    __shared__ int s_last[256];
-    const int b = blockIdx.x, K = a.K, tid = threadIdx.x;
-    const vx_choice c = choice[b];
-    if (c.token != -1) return;
-    const int j = c.row;
-    const vx_row_stat tr = stats[(long long)b * (2 * K + 1) + j];
-    const E *row = (const E *)a.target + b * a.t_seq + j * a.t_row;
-    const bool minus = c.residual && a.draft;
-    const vx_row_stat dr = minus ? stats[(long long)b * (2 * K + 1) + K + 1 + j] : tr;
-    const E *drow = minus ? (const E *)a.draft + b * a.d_seq + j * a.d_row : row;
-    const long long drop = c.residual && !a.draft ? a.tokens[(long long)b * K + j] : -1;
-    const double inv_t = 1.0 / (double)a.temperature[b];
-    // each thread owns one contiguous piece of the row
-    const int per = (a.V + 255) / 256, lo = min(a.V, tid * per), hi = min(a.V, lo + per);
-    for (int only_p = 0; only_p < 2; ++only_p) {
-        auto weight = [&](int i) -> double {
-            if (i == drop && !only_p) return 0.0;
-            const double p = vx_weight((float)row[i], tr.m, inv_t) / tr.z;
-            if (!minus || only_p) return p;
-            const double r = p - vx_weight((float)drow[i], dr.m, inv_t) / dr.z;
-            return r > 0.0 ? r : 0.0;
-        };
+// The first i whose cumulative weight passes goal = u * total; `sums(k)` the weight of chunk k, `weight(i)` of one token.
+// One workgroup: first the chunk, then the place in it; where rounding leaves none, the last token with a weight.  -1 where
+// no token has a weight.
+template <int CHUNK, class S, class W>
+__device__ __forceinline__ int vx_verify_pick(int chunks, int V, float u, S sums, W weight, double *s_run, int *s_int) {
+    const int tid = threadIdx.x;
+    // thread t takes chunks (then tokens) t * per ..: the running sums stay in order
+    int first = 0, last = -1;
+    double base = 0.0, goal = 0.0;
+    for (int level = 0; level < 2; ++level) {
+        const int n = level == 0 ? chunks : min(CHUNK, V - first), per = (n + 255) / 256;
+        const int lo = min(n, tid * per), hi = min(n, lo + per);
         double sum = 0.0;
-        int last = -1;
+        int mine_last = -1;
         for (int i = lo; i < hi; ++i) {
-            const double r = weight(i);
-            sum += r;
-            if (r > 0.0) last = i;
+            const double v = level == 0 ? sums(i) : weight(first + i);
+            sum += v;
+            if (v > 0.0) mine_last = i;
         }
-        s_sum[tid] = sum;
-        s_last[tid] = last;
+        __syncthreads();
+        s_run[tid] = sum;
+        s_int[tid] = mine_last;
         __syncthreads();
         if (tid == 0) {
-            double run = 0.0;
+            double run = base;
             int l = -1;
             for (int t = 0; t < 256; ++t) {
-                const double v = s_sum[t];
-                s_sum[t] = run;
+                const double v = s_run[t];
+                s_run[t] = run;
                 run += v;
-                l = max(l, s_last[t]);
+                l = max(l, s_int[t]);
             }
-            s_sum[256] = run;
-            s_last[0] = l;
+            s_run[256] = run;
+            s_int[256] = l;
+            s_int[257] = -1;
         }
         __syncthreads();
-        const double total = s_sum[256];
-        if (!(total > 0.0)) { __syncthreads(); continue; }   // p and q alike to the last bit: draw from p
-        const double goal = (double)a.uniforms[(long long)b * (K + 1) + K] * total;
-        const bool none = !(goal < total);                    // a uniform of 1, or rounding: the last token with weight
-        if (none) {
-            if (tid == 0) out[(long long)b * (K + 1) + j] = s_last[0];
-        } else if (hi > lo && s_sum[tid] <= goal && goal < s_sum[tid + 1]) {
-            double run = s_sum[tid];
-            int pick = -1;
-            for (int i = lo; i < hi && pick < 0; ++i) {
-                run += weight(i);
-                if (run > goal) pick = i;
+        if (level == 0) goal = (double)u * s_run[256];
+        last = s_int[256];
+        if (lo < hi && s_run[tid] <= goal && goal < s_run[tid + 1]) {
+            double run = s_run[tid];
+            int at = mine_last;
+            for (int i = lo; i < hi; ++i) {
+                const double next = run + (level == 0 ? sums(i) : weight(first + i));
+                if (next > goal) { at = i; break; }
+                run = next;
             }
-            out[(long long)b * (K + 1) + j] = pick < 0 ? last : pick;
+            s_int[257] = at;
+            s_run[257] = run;                                     // the weight in front of it
         }
+        __syncthreads();
+        const bool found = s_int[257] >= 0;
+        const int at = found ? s_int[257] : last;
+        if (level == 0) {
+            if (at < 0) return -1;                                // no weight at all
+            base = found ? s_run[257] : 0.0;
+            if (!found) goal = INFINITY;                          // a uniform of 1, or rounding: the last token with a weight
+            first = at * CHUNK;
+        } else {
+            return first + at;
+        }
+    }
+    return -1;
+}
+
+// One workgroup per (sequence, chunk).
+template <int DT>
+__global__ __launch_bounds__(256) void vx_k_verify_draw(vx_verify_args a) {
+    constexpr int CHUNK = vx_verify_chunk<DT>(), PER = VX_VERIFY_U * 16 / sizeof(typename vx_elem<DT>::type);
+    __shared__ double s_run[258], s_sum[4];
+    __shared__ int s_int[258];
+    __shared__ int s_go;
+    const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks;
+    const vx_choice ch = a.choice[b];
+    if (ch.mode == 0 || (ch.mode != 3 && chunk != 0)) return;
+    const typename vx_elem<DT>::type *trow = vx_verify_target<DT>(a, b, ch.row);
+    const double c = vx_verify_c(a.temperature[b]);
+    const double2 *z = a.z + (long long)b * a.chunks;
+    const float u = a.uniforms[(long long)b * (a.K + 1) + a.K];
+    long long *out = a.out + (long long)b * (a.K + 1) + ch.row;
+    auto from_p = [&](long long drop) {
+        const double dropped = drop >= 0 && drop < a.V ? vx_weight((float)trow[drop], ch.mp, c) : 0.0;
+        const int drop_chunk = dropped > 0.0 ? (int)(drop / CHUNK) : -1;
+        auto one = [&](int i) { return i == drop ? 0.0 : vx_weight((float)trow[i], ch.mp, c); };
+        // a chunk that loses a token is summed again: its sum less the token's weight could be all rounding
+        double again = 0.0;
+        if (drop_chunk >= 0) {
+            for (int k = threadIdx.x; k < CHUNK; k += 256)
+                if (drop_chunk * CHUNK + k < a.V) again += one(drop_chunk * CHUNK + k);
+            again = vx_verify_sum(again, s_sum);
+        }
+        return vx_verify_pick<CHUNK>(a.chunks, a.V, u, [&](int k) { return k == drop_chunk ? again : z[k].x; }, one, s_run, s_int);
+    };
+    if (ch.mode != 3) {
+        int i = from_p(ch.drop);
+        if (i < 0) i = from_p(-1);                                // nothing but the rejected token had a weight
+        if (threadIdx.x == 0) *out = i;
         return;
     }
+    const typename vx_elem<DT>::type *drow = vx_verify_draft<DT>(a, b, ch.row);
+    double zp = 0.0, zq = 0.0;
+    for (int k = 0; k < a.chunks; ++k) {                          // the same order in every workgroup
+        const double2 v = z[k];
+        zp += v.x;
+        zq += v.y;
+    }
+    const double ip = 1.0 / zp, iq = 1.0 / zq;
+    auto rest = [&](float x, float y) {
+        const double r = vx_weight(x, ch.mp, c) * ip - vx_weight(y, ch.mq, c) * iq;
+        return r > 0.0 ? r : 0.0;
+    };
+    {
+        float x[PER], y[PER];
+        vx_verify_load<DT>(trow, chunk * CHUNK, a.V, x);
+        vx_verify_load<DT>(drow, chunk * CHUNK, a.V, y);
+        double sum = 0.0;
+#pragma unroll 4
+        for (int k = 0; k < PER; ++k) sum += rest(x[k], y[k]);
+        sum = vx_verify_sum(sum, s_sum);
+        if (threadIdx.x == 0) {
+            a.r[(long long)b * a.chunks + chunk] = sum;
+            __threadfence();
+            s_go = atomicAdd(&a.ticket[b], 1) == a.chunks - 1;
+            __threadfence();
+        }
+    }
+    __syncthreads();
+    if (!s_go) return;
+    // the last workgroup of the sequence: every chunk's sum is there
+    const double *r = a.r + (long long)b * a.chunks;
+    auto sums = [&](int k) { return __hip_atomic_load(&r[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    double total = 0.0;
+    for (int k = threadIdx.x; k < a.chunks; k += 256) total += sums(k);
+    total = vx_verify_sum(total, s_sum);
+    // p and q alike to the last bit: from p
+    const int i = total > 0.0 ? vx_verify_pick<CHUNK>(a.chunks, a.V, u, sums, [&](int k) { return rest((float)trow[k], (float)drow[k]); }, s_run, s_int)
+                              : from_p(-1);
+    if (threadIdx.x == 0) *out = i;
+}
+
+struct vx_verify_plan {
+    int chunks;
+    size_t stats, z, r, choice, ticket, total;
+};
+
+static vx_verify_plan vx_verify_make_plan(int B, int K, int V, int chunk) {
+    vx_verify_plan p;
+    p.chunks = (V + chunk - 1) / chunk;
+    size_t at = 0;
+    auto take = [&](size_t n) { const size_t o = at; at += (n + 255) & ~(size_t)255; return o; };
+    p.stats = take((size_t)B * (2 * K + 1) * p.chunks * sizeof(float2));
+    p.z = take((size_t)B * p.chunks * sizeof(double2));
+    p.r = take((size_t)B * p.chunks * sizeof(double));
+    p.choice = take((size_t)B * sizeof(vx_choice));
+    p.ticket = take((size_t)B * sizeof(int));
+    p.total = at;
+    return p;
 }
 
 extern "C" size_t vx_verify_drafts_workspace_bytes(int B, int K, int V) {
     if (B <= 0 || K < 0 || V <= 0 || B > VX_MAX_VERIFY_BATCH || K > VX_MAX_DRAFTS || V > VX_MAX_VOCAB) return 0;
-    return (((size_t)B * (2 * K + 1) * sizeof(vx_row_stat) + 255) & ~(size_t)255) + (((size_t)B * sizeof(vx_choice) + 255) & ~(size_t)255);
+    return vx_verify_make_plan(B, K, V, vx_verify_chunk<VX_DTYPE_F32>()).total;      // the smallest chunk
 }
 
 extern "C" int vx_verify_drafts(const void *d_target, int64_t target_seq_stride, int64_t target_row_stride, const void *d_draft,
@@ -238,17 +511,21 @@ extern "C" int vx_verify_drafts(const void *d_target, int64_t target_seq_stride,
         ((uintptr_t)d_workspace & 255))
         return VX_ERR_ALIGNMENT;
     if (workspace_bytes < vx_verify_drafts_workspace_bytes(B, K, V)) return VX_ERR_WORKSPACE;
-    vx_verify_args a = {d_target, d_draft, target_seq_stride, target_row_stride, draft_seq_stride, draft_row_stride,
-                        (const long long *)d_draft_tokens, d_draft_lens, d_uniforms, d_temperature, B, K, V};
-    vx_row_stat *stats = (vx_row_stat *)d_workspace;
-    vx_choice *choice = (vx_choice *)((char *)d_workspace + (((size_t)B * (2 * K + 1) * sizeof(vx_row_stat) + 255) & ~(size_t)255));
+    if (K == 0) d_draft = nullptr;
+    const vx_verify_plan p = vx_verify_make_plan(B, K, V, es == 4 ? vx_verify_chunk<VX_DTYPE_F32>() : vx_verify_chunk<VX_DTYPE_F16>());
+    const int64_t blocks = (int64_t)B * (d_draft ? 2 * K + 1 : K + 1) * p.chunks;
+    if (blocks > 2147483647LL) return VX_ERR_UNSUPPORTED;
+    char *ws = (char *)d_workspace;
+    const vx_verify_args a = {d_target, d_draft, target_seq_stride, target_row_stride, draft_seq_stride, draft_row_stride,
+                              (const long long *)d_draft_tokens, d_draft_lens, d_uniforms, d_temperature, B, K, V, p.chunks,
+                              (float2 *)(ws + p.stats), (double2 *)(ws + p.z), (double *)(ws + p.r), (vx_choice *)(ws + p.choice),
+                              (int *)(ws + p.ticket), (long long *)d_tokens, d_counts, d_status, d_accept};
     hipStream_t st = (hipStream_t)stream;
     vx_prof_begin(VX_PROF_VERIFY, st);
     VX_DISPATCH_DTYPE(dtype, {
-        hipLaunchKernelGGL((vx_k_verify_stats<DT>), dim3((unsigned)(B * (2 * K + 1))), dim3(256), 0, st, a, stats);
-        hipLaunchKernelGGL((vx_k_verify_accept<DT>), dim3((unsigned)((B + 63) / 64)), dim3(64), 0, st, a, stats, choice,
-                           (long long *)d_tokens, d_counts, d_accept, d_status);
-        hipLaunchKernelGGL((vx_k_verify_draw<DT>), dim3((unsigned)B), dim3(256), 0, st, a, stats, choice, (long long *)d_tokens);
+        hipLaunchKernelGGL((vx_k_verify_stats<DT>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((vx_k_verify_choose<DT>), dim3((unsigned)(B * p.chunks)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((vx_k_verify_draw<DT>), dim3((unsigned)(B * p.chunks)), dim3(256), 0, st, a);
     });
     vx_prof_end(VX_PROF_VERIFY, st);
     return hipGetLastError() == hipSuccess ? VX_OK : VX_ERR_LAUNCH;
