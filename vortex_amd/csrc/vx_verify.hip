@@ -64,25 +64,25 @@ __device__ __forceinline__ const typename vx_elem<DT>::type *vx_verify_draft(con
 }
 
 // 2^t for t <= 0: t = n + f, |f| <= 1/2, and the series of e^(f ln 2) up to its 12th term (the 13th is below 2e-16).
-// Below -1000, and for the NaN of -inf * 0 (a masked logit at an infinite temperature), 0.
+// From -1100 down, and for the NaN of -inf * 0 (a masked logit at an infinite temperature), the result underflows to 0.
 __device__ __forceinline__ double vx_exp2_64(double t) {
-    t = fmax(t, -1000.0);
-    const double n = rint(t), f = (t - n) * 0.69314718055994530942;
-    double p = 1.0 / 479001600.0;
-    p = __builtin_fma(p, f, 1.0 / 39916800.0);
-    p = __builtin_fma(p, f, 1.0 / 3628800.0);
-    p = __builtin_fma(p, f, 1.0 / 362880.0);
-    p = __builtin_fma(p, f, 1.0 / 40320.0);
-    p = __builtin_fma(p, f, 1.0 / 5040.0);
-    p = __builtin_fma(p, f, 1.0 / 720.0);
-    p = __builtin_fma(p, f, 1.0 / 120.0);
-    p = __builtin_fma(p, f, 1.0 / 24.0);
-    p = __builtin_fma(p, f, 1.0 / 6.0);
-    p = __builtin_fma(p, f, 0.5);
+    constexpr double L = 0.69314718055994530942;
+    t = fmax(t, -1100.0);
+    const double n = rint(t), f = t - n;
+    double p = L * L * L * L * L * L * L * L * L * L * L * L / 479001600.0;
+    p = __builtin_fma(p, f, L * L * L * L * L * L * L * L * L * L * L / 39916800.0);
+    p = __builtin_fma(p, f, L * L * L * L * L * L * L * L * L * L / 3628800.0);
+    p = __builtin_fma(p, f, L * L * L * L * L * L * L * L * L / 362880.0);
+    p = __builtin_fma(p, f, L * L * L * L * L * L * L * L / 40320.0);
+    p = __builtin_fma(p, f, L * L * L * L * L * L * L / 5040.0);
+    p = __builtin_fma(p, f, L * L * L * L * L * L / 720.0);
+    p = __builtin_fma(p, f, L * L * L * L * L / 120.0);
+    p = __builtin_fma(p, f, L * L * L * L / 24.0);
+    p = __builtin_fma(p, f, L * L * L / 6.0);
+    p = __builtin_fma(p, f, L * L * 0.5);
+    p = __builtin_fma(p, f, L);
     p = __builtin_fma(p, f, 1.0);
-    p = __builtin_fma(p, f, 1.0);
-    p = ldexp(p, (int)n);
-    return t <= -1000.0 ? 0.0 : p;
+    return ldexp(p, (int)n);
 }
 // weight of a logit against the row's largest one; c = log2(e) / T
 __device__ __forceinline__ double vx_weight(float x, float m, double c) {
@@ -132,36 +132,37 @@ __global__ __launch_bounds__(256) void vx_k_verify_stats(vx_verify_args a) {
     const int c0 = chunk * vx_verify_chunk<DT>();
     vx_verify_load<DT>(is_draft ? vx_verify_draft<DT>(a, b, j - a.K - 1) : vx_verify_target<DT>(a, b, j), c0, a.V, x);
     float m = -INFINITY;
-    bool bad = false;
 #pragma unroll
-    for (int k = 0; k < PER; ++k) {
-        bad |= !(x[k] < INFINITY);
-        m = fmaxf(m, x[k]);
-    }
+    for (int k = 0; k < PER; ++k) m = fmaxf(m, x[k]);
 #pragma unroll
     for (int k = 32; k >= 1; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, VX_WAVE));
-    bad = __any(bad);
+    bool bad = false;
     float z = 0.f;
     int best = 0x7fffffff;
     if (greedy) {
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
             const int i = c0 + ((k / VEC) * 256 + threadIdx.x) * VEC + k % VEC;
+            bad |= !(x[k] < INFINITY);
             if (x[k] == m) best = min(best, i);
         }
+        bad = __any(bad);
 #pragma unroll
         for (int k = 32; k >= 1; k >>= 1) best = min(best, __shfl_xor(best, k, VX_WAVE));
     } else {
-        const float c = fminf((float)vx_verify_c(T), 3e38f);
+        // A NaN or +inf makes the sum NaN by itself, and nothing else does: the subtrahend is finite, and so is the factor, which
+        // is not 0 either (a masked logit weighs 0 at an infinite temperature too).
+        const float c = fminf(fmaxf((float)vx_verify_c(T), 1e-45f), 3e38f), top = m == -INFINITY ? 0.f : m;
 #pragma unroll
-        for (int k = 0; k < PER; ++k) z += __builtin_amdgcn_exp2f(fmaxf((x[k] - m) * c, -200.f));   // -inf - -inf, 0 * inf: NaN, weighs 0
+        for (int k = 0; k < PER; ++k) z += __builtin_amdgcn_exp2f((x[k] - top) * c);
 #pragma unroll
         for (int k = 32; k >= 1; k >>= 1) z += __shfl_xor(z, k, VX_WAVE);
+        bad = z != z;
     }
     if (vx_lane() == 0) {
         const int w = threadIdx.x >> 6;
         s_m[w] = bad ? __builtin_nanf("") : m;
-        s_z[w] = m == -INFINITY ? 0.f : z;
+        s_z[w] = z;
         s_i[w] = best;
     }
     __syncthreads();
@@ -332,77 +333,86 @@ __global__ __launch_bounds__(256) void vx_k_verify_choose(vx_verify_args a) {
     if (threadIdx.x == 0) a.z[(long long)b * a.chunks + chunk] = double2{zp, zq};
 }
 
-// The first i whose cumulative weight passes goal = u * total; `sums(k)` the weight of chunk k, `weight(i)` of one token.
-// One workgroup: first the chunk, then the place in it; where rounding leaves none, the last token with a weight.  -1 where
-// no token has a weight.
-template <int CHUNK, class S, class W>
-__device__ __forceinline__ int vx_verify_pick(int chunks, int V, float u, S sums, W weight, double *s_run, int *s_int) {
-    const int tid = threadIdx.x;
-    // thread t takes chunks (then tokens) t * per ..: the running sums stay in order
-    int first = 0, last = -1;
-    double base = 0.0, goal = 0.0;
-    for (int level = 0; level < 2; ++level) {
-        const int n = level == 0 ? chunks : min(CHUNK, V - first), per = (n + 255) / 256;
-        const int lo = min(n, tid * per), hi = min(n, lo + per);
-        double sum = 0.0;
-        int mine_last = -1;
-        for (int i = lo; i < hi; ++i) {
-            const double v = level == 0 ? sums(i) : weight(first + i);
-            sum += v;
-            if (v > 0.0) mine_last = i;
-        }
-        __syncthreads();
-        s_run[tid] = sum;
-        s_int[tid] = mine_last;
-        __syncthreads();
-        if (tid == 0) {
-            double run = base;
-            int l = -1;
-            for (int t = 0; t < 256; ++t) {
-                const double v = s_run[t];
-                s_run[t] = run;
-                run += v;
-                l = max(l, s_int[t]);
-            }
-            s_run[256] = run;
-            s_int[256] = l;
-            s_int[257] = -1;
-        }
-        __syncthreads();
-        if (level == 0) goal = (double)u * s_run[256];
-        last = s_int[256];
-        if (lo < hi && s_run[tid] <= goal && goal < s_run[tid + 1]) {
-            double run = s_run[tid];
-            int at = mine_last;
-            for (int i = lo; i < hi; ++i) {
-                const double next = run + (level == 0 ? sums(i) : weight(first + i));
-                if (next > goal) { at = i; break; }
-                run = next;
-            }
-            s_int[257] = at;
-            s_run[257] = run;                                     // the weight in front of it
-        }
-        __syncthreads();
-        const bool found = s_int[257] >= 0;
-        const int at = found ? s_int[257] : last;
-        if (level == 0) {
-            if (at < 0) return -1;                                // no weight at all
-            base = found ? s_run[257] : 0.0;
-            if (!found) goal = INFINITY;                          // a uniform of 1, or rounding: the last token with a weight
-            first = at * CHUNK;
-        } else {
-            return first + at;
-        }
+struct vx_pick_smem {
+    double run[4], before;
+    int first, last;
+};
+
+// Thread t holds the weight `sum` of the t-th of up to 256 parts: the first part at which the running weight, from `base`
+// on, passes `goal`, and the weight in front of it; -1 where none does.  `last`: the last part with a weight (-1: none).
+__device__ __forceinline__ int vx_pick_part(double sum, double base, double goal, vx_pick_smem &S, double &before, int &last) {
+    const int lane = vx_lane(), w = threadIdx.x >> 6;
+    double run = sum;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const double o = __shfl_up(run, d, VX_WAVE);
+        if (lane >= d) run += o;
     }
-    return -1;
+    __syncthreads();
+    if (lane == 63) S.run[w] = run;
+    if (threadIdx.x == 0) { S.first = 256; S.last = -1; }
+    __syncthreads();
+    double front = base;
+    for (int i = 0; i < w; ++i) front += S.run[i];
+    run += front;
+    const double prev = __shfl_up(run, 1, VX_WAVE);
+    const u64 passed = __ballot(run > goal), any = __ballot(sum > 0.0);
+    if (lane == 0) {
+        if (passed) atomicMin(&S.first, w * 64 + __builtin_ctzll(passed));
+        if (any) atomicMax(&S.last, w * 64 + 63 - __builtin_clzll(any));
+    }
+    __syncthreads();
+    const int first = S.first;
+    last = S.last;
+    if ((int)threadIdx.x == first) S.before = lane ? prev : front;
+    __syncthreads();
+    before = S.before;
+    return first < 256 ? first : -1;
+}
+
+// The first i whose cumulative weight passes u * total; `sums(k)` the weight of chunk k, `weight(i)` of one token.  One
+// workgroup: first the chunk, then the 1/256 of it, then the token; where rounding leaves none, the last one with a weight.
+// -1 where no token has a weight.
+template <int CHUNK, class S, class W>
+__device__ __forceinline__ int vx_verify_pick(int chunks, int V, float u, S sums, W weight, vx_pick_smem &sm, double *s_sum) {
+    constexpr int PART = CHUNK / 256;
+    const int tid = threadIdx.x, per = (chunks + 255) / 256;      // chunks of one thread
+    double mine = 0.0, before;
+    int last;
+    for (int k = tid * per; k < min(chunks, (tid + 1) * per); ++k) mine += sums(k);
+    double goal = (double)u * vx_verify_sum(mine, s_sum);
+    int part = vx_pick_part(mine, 0.0, goal, sm, before, last);
+    if (last < 0) return -1;
+    if (part < 0) { part = last; goal = INFINITY; before = 0.0; } // a uniform of 1, or rounding
+    int chunk = part * per;
+    if (per > 1) {                                                // more than 256 chunks: on through this thread's
+        int c = -1;
+        for (int k = part * per; k < min(chunks, (part + 1) * per); ++k) {
+            const double v = sums(k);
+            if (v > 0.0) c = k;
+            if (before + v > goal) break;
+            before += v;
+        }
+        chunk = c < 0 ? chunk : c;
+    }
+    const int at = chunk * CHUNK + tid * PART;
+    mine = 0.0;
+#pragma unroll 4
+    for (int k = 0; k < PART; ++k)
+        if (at + k < V) mine += weight(at + k);
+    part = vx_pick_part(mine, before, goal, sm, before, last);
+    if (part < 0) { part = max(last, 0); goal = INFINITY; }
+    const int i = chunk * CHUNK + part * PART + tid;
+    part = vx_pick_part(tid < PART && i < V ? weight(i) : 0.0, before, goal, sm, before, last);
+    return i - tid + (part < 0 ? max(last, 0) : part);
 }
 
 // One workgroup per (sequence, chunk).
 template <int DT>
 __global__ __launch_bounds__(256) void vx_k_verify_draw(vx_verify_args a) {
     constexpr int CHUNK = vx_verify_chunk<DT>(), PER = VX_VERIFY_U * 16 / sizeof(typename vx_elem<DT>::type);
-    __shared__ double s_run[258], s_sum[4];
-    __shared__ int s_int[258];
+    __shared__ double s_sum[4];
+    __shared__ vx_pick_smem sm;
     __shared__ int s_go;
     const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks;
     const vx_choice ch = a.choice[b];
@@ -423,7 +433,7 @@ __global__ __launch_bounds__(256) void vx_k_verify_draw(vx_verify_args a) {
                 if (drop_chunk * CHUNK + k < a.V) again += one(drop_chunk * CHUNK + k);
             again = vx_verify_sum(again, s_sum);
         }
-        return vx_verify_pick<CHUNK>(a.chunks, a.V, u, [&](int k) { return k == drop_chunk ? again : z[k].x; }, one, s_run, s_int);
+        return vx_verify_pick<CHUNK>(a.chunks, a.V, u, [&](int k) { return k == drop_chunk ? again : z[k].x; }, one, sm, s_sum);
     };
     if (ch.mode != 3) {
         int i = from_p(ch.drop);
@@ -467,7 +477,7 @@ __global__ __launch_bounds__(256) void vx_k_verify_draw(vx_verify_args a) {
     for (int k = threadIdx.x; k < a.chunks; k += 256) total += sums(k);
     total = vx_verify_sum(total, s_sum);
     // p and q alike to the last bit: from p
-    const int i = total > 0.0 ? vx_verify_pick<CHUNK>(a.chunks, a.V, u, sums, [&](int k) { return rest((float)trow[k], (float)drow[k]); }, s_run, s_int)
+    const int i = total > 0.0 ? vx_verify_pick<CHUNK>(a.chunks, a.V, u, sums, [&](int k) { return rest((float)trow[k], (float)drow[k]); }, sm, s_sum)
                               : from_p(-1);
     if (threadIdx.x == 0) *out = i;
 }
