@@ -6,11 +6,12 @@
 //       r = max(0, p_n - q_n) when a draft was rejected, r = p_n behind the last draft
 // T_b not above 0: greedy (x_j is accepted iff it is the first arg-max of its row; the token behind is the arg-max).
 //
-// Three launches over chunks of the vocabulary:
+// Launches over chunks of the vocabulary:
 //   stats   every used row: largest logit and fp32 sum of exponentials of each chunk (bound by the one read of the logits;
 //           fp64 exponentials here would take twice the time of the read)
 //   choose  the accepted drafts and the row to draw from; that row's (and the draft row's) chunk sums again in fp64
-//   draw    chunk sums of max(0, p - q) in fp64, the last workgroup of a sequence finds the token
+//   rest    (with draft logits) that row's chunk sums of max(0, p - q), fp64
+//   draw    the token, one workgroup a sequence
 // The token that is drawn is a whole number, decided by where a cumulative sum passes a border, and one step of a flat
 // distribution is 1/V: everything it depends on is fp64.  The sums of the first launch are within 2^-17 of the true ones:
 //   an exponential is off by 2^-23 (the instruction) + ln2 |t| 3 * 2^-24 (difference, factor, product), t its exponent to
@@ -33,7 +34,6 @@ struct vx_verify_args {
     double2 *z;                                   // [B][chunks]: sums of the row that is drawn from, target and draft
     double *r;                                    // [B][chunks]: sums of max(0, p - q)
     struct vx_choice *choice;                     // [B]
-    int *ticket;                                  // [B]
     // outputs
     long long *out;                               // [B, K + 1]
     int *counts, *status;
@@ -126,7 +126,6 @@ __global__ __launch_bounds__(256) void vx_k_verify_stats(vx_verify_args a) {
     const bool is_draft = j > a.K;
     const float T = a.temperature[b];
     const bool greedy = !(T > 0.f);
-    if (j == 0 && chunk == 0 && threadIdx.x == 0) a.ticket[b] = 0;
     if (is_draft ? (j - a.K - 1 >= n || greedy) : j > n) return;
     float x[PER];
     const int c0 = chunk * vx_verify_chunk<DT>();
@@ -407,21 +406,57 @@ __device__ __forceinline__ int vx_verify_pick(int chunks, int V, float u, S sums
     return i - tid + (part < 0 ? max(last, 0) : part);
 }
 
-// One workgroup per (sequence, chunk).
+// r of one token from its two logits; ip, iq: the inverse sums of the rows
+__device__ __forceinline__ double vx_verify_rest(float x, float y, const vx_choice &ch, double c, double ip, double iq) {
+    const double r = vx_weight(x, ch.mp, c) * ip - vx_weight(y, ch.mq, c) * iq;
+    return r > 0.0 ? r : 0.0;
+}
+// sums of the two rows over all chunks, in the same order wherever they are needed
+__device__ __forceinline__ double2 vx_verify_totals(const vx_verify_args &a, int b, double *s_sum) {
+    double zp = 0.0, zq = 0.0;
+    for (int k = threadIdx.x; k < a.chunks; k += 256) {
+        const double2 v = a.z[(long long)b * a.chunks + k];
+        zp += v.x;
+        zq += v.y;
+    }
+    zp = vx_verify_sum(zp, s_sum);
+    return double2{zp, vx_verify_sum(zq, s_sum)};
+}
+
+// Chunk sums of max(0, p - q): one workgroup per (sequence, chunk).
 template <int DT>
-__global__ __launch_bounds__(256) void vx_k_verify_draw(vx_verify_args a) {
+__global__ __launch_bounds__(256) void vx_k_verify_rest(vx_verify_args a) {
     constexpr int CHUNK = vx_verify_chunk<DT>(), PER = VX_VERIFY_U * 16 / sizeof(typename vx_elem<DT>::type);
     __shared__ double s_sum[4];
-    __shared__ vx_pick_smem sm;
-    __shared__ int s_go;
     const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks;
     const vx_choice ch = a.choice[b];
-    if (ch.mode == 0 || (ch.mode != 3 && chunk != 0)) return;
+    if (ch.mode != 3) return;
+    float x[PER], y[PER];
+    vx_verify_load<DT>(vx_verify_target<DT>(a, b, ch.row), chunk * CHUNK, a.V, x);
+    vx_verify_load<DT>(vx_verify_draft<DT>(a, b, ch.row), chunk * CHUNK, a.V, y);
+    const double c = vx_verify_c(a.temperature[b]);
+    const double2 z = vx_verify_totals(a, b, s_sum);
+    const double ip = 1.0 / z.x, iq = 1.0 / z.y;
+    double sum = 0.0;
+#pragma unroll 4
+    for (int k = 0; k < PER; ++k) sum += vx_verify_rest(x[k], y[k], ch, c, ip, iq);
+    sum = vx_verify_sum(sum, s_sum);
+    if (threadIdx.x == 0) a.r[(long long)b * a.chunks + chunk] = sum;
+}
+
+// The drawn token: one workgroup per sequence.
+template <int DT>
+__global__ __launch_bounds__(256) void vx_k_verify_draw(vx_verify_args a) {
+    constexpr int CHUNK = vx_verify_chunk<DT>();
+    __shared__ double s_sum[4];
+    __shared__ vx_pick_smem sm;
+    const int b = blockIdx.x;
+    const vx_choice ch = a.choice[b];
+    if (ch.mode == 0) return;
     const typename vx_elem<DT>::type *trow = vx_verify_target<DT>(a, b, ch.row);
     const double c = vx_verify_c(a.temperature[b]);
     const double2 *z = a.z + (long long)b * a.chunks;
     const float u = a.uniforms[(long long)b * (a.K + 1) + a.K];
-    long long *out = a.out + (long long)b * (a.K + 1) + ch.row;
     auto from_p = [&](long long drop) {
         const double dropped = drop >= 0 && drop < a.V ? vx_weight((float)trow[drop], ch.mp, c) : 0.0;
         const int drop_chunk = dropped > 0.0 ? (int)(drop / CHUNK) : -1;
@@ -435,56 +470,23 @@ __global__ __launch_bounds__(256) void vx_k_verify_draw(vx_verify_args a) {
         }
         return vx_verify_pick<CHUNK>(a.chunks, a.V, u, [&](int k) { return k == drop_chunk ? again : z[k].x; }, one, sm, s_sum);
     };
-    if (ch.mode != 3) {
-        int i = from_p(ch.drop);
-        if (i < 0) i = from_p(-1);                                // nothing but the rejected token had a weight
-        if (threadIdx.x == 0) *out = i;
-        return;
+    int i;
+    if (ch.mode == 3) {
+        const typename vx_elem<DT>::type *drow = vx_verify_draft<DT>(a, b, ch.row);
+        const double2 t = vx_verify_totals(a, b, s_sum);
+        const double ip = 1.0 / t.x, iq = 1.0 / t.y, *r = a.r + (long long)b * a.chunks;
+        i = vx_verify_pick<CHUNK>(a.chunks, a.V, u, [&](int k) { return r[k]; },
+                                  [&](int k) { return vx_verify_rest((float)trow[k], (float)drow[k], ch, c, ip, iq); }, sm, s_sum);
+    } else {
+        i = from_p(ch.drop);
     }
-    const typename vx_elem<DT>::type *drow = vx_verify_draft<DT>(a, b, ch.row);
-    double zp = 0.0, zq = 0.0;
-    for (int k = 0; k < a.chunks; ++k) {                          // the same order in every workgroup
-        const double2 v = z[k];
-        zp += v.x;
-        zq += v.y;
-    }
-    const double ip = 1.0 / zp, iq = 1.0 / zq;
-    auto rest = [&](float x, float y) {
-        const double r = vx_weight(x, ch.mp, c) * ip - vx_weight(y, ch.mq, c) * iq;
-        return r > 0.0 ? r : 0.0;
-    };
-    {
-        float x[PER], y[PER];
-        vx_verify_load<DT>(trow, chunk * CHUNK, a.V, x);
-        vx_verify_load<DT>(drow, chunk * CHUNK, a.V, y);
-        double sum = 0.0;
-#pragma unroll 4
-        for (int k = 0; k < PER; ++k) sum += rest(x[k], y[k]);
-        sum = vx_verify_sum(sum, s_sum);
-        if (threadIdx.x == 0) {
-            a.r[(long long)b * a.chunks + chunk] = sum;
-            __threadfence();
-            s_go = atomicAdd(&a.ticket[b], 1) == a.chunks - 1;
-            __threadfence();
-        }
-    }
-    __syncthreads();
-    if (!s_go) return;
-    // the last workgroup of the sequence: every chunk's sum is there
-    const double *r = a.r + (long long)b * a.chunks;
-    auto sums = [&](int k) { return __hip_atomic_load(&r[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-    double total = 0.0;
-    for (int k = threadIdx.x; k < a.chunks; k += 256) total += sums(k);
-    total = vx_verify_sum(total, s_sum);
-    // p and q alike to the last bit: from p
-    const int i = total > 0.0 ? vx_verify_pick<CHUNK>(a.chunks, a.V, u, sums, [&](int k) { return rest((float)trow[k], (float)drow[k]); }, sm, s_sum)
-                              : from_p(-1);
-    if (threadIdx.x == 0) *out = i;
+    if (i < 0) i = from_p(-1);                                    // p and q alike to the last bit; nothing but the rejected token
+    if (threadIdx.x == 0) a.out[(long long)b * (a.K + 1) + ch.row] = i;
 }
 
 struct vx_verify_plan {
     int chunks;
-    size_t stats, z, r, choice, ticket, total;
+    size_t stats, z, r, choice, total;
 };
 
 static vx_verify_plan vx_verify_make_plan(int B, int K, int V, int chunk) {
@@ -496,7 +498,6 @@ static vx_verify_plan vx_verify_make_plan(int B, int K, int V, int chunk) {
     p.z = take((size_t)B * p.chunks * sizeof(double2));
     p.r = take((size_t)B * p.chunks * sizeof(double));
     p.choice = take((size_t)B * sizeof(vx_choice));
-    p.ticket = take((size_t)B * sizeof(int));
     p.total = at;
     return p;
 }
@@ -529,13 +530,14 @@ extern "C" int vx_verify_drafts(const void *d_target, int64_t target_seq_stride,
     const vx_verify_args a = {d_target, d_draft, target_seq_stride, target_row_stride, draft_seq_stride, draft_row_stride,
                               (const long long *)d_draft_tokens, d_draft_lens, d_uniforms, d_temperature, B, K, V, p.chunks,
                               (float2 *)(ws + p.stats), (double2 *)(ws + p.z), (double *)(ws + p.r), (vx_choice *)(ws + p.choice),
-                              (int *)(ws + p.ticket), (long long *)d_tokens, d_counts, d_status, d_accept};
+                              (long long *)d_tokens, d_counts, d_status, d_accept};
     hipStream_t st = (hipStream_t)stream;
     vx_prof_begin(VX_PROF_VERIFY, st);
     VX_DISPATCH_DTYPE(dtype, {
         hipLaunchKernelGGL((vx_k_verify_stats<DT>), dim3((unsigned)blocks), dim3(256), 0, st, a);
         hipLaunchKernelGGL((vx_k_verify_choose<DT>), dim3((unsigned)(B * p.chunks)), dim3(256), 0, st, a);
-        hipLaunchKernelGGL((vx_k_verify_draw<DT>), dim3((unsigned)(B * p.chunks)), dim3(256), 0, st, a);
+        if (d_draft) hipLaunchKernelGGL((vx_k_verify_rest<DT>), dim3((unsigned)(B * p.chunks)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((vx_k_verify_draw<DT>), dim3((unsigned)B), dim3(256), 0, st, a);
     });
     vx_prof_end(VX_PROF_VERIFY, st);
     return hipGetLastError() == hipSuccess ? VX_OK : VX_ERR_LAUNCH;
