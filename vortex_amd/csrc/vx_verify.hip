@@ -64,11 +64,13 @@ __device__ __forceinline__ const typename vx_elem<DT>::type *vx_verify_draft(con
 }
 
 // 2^t for t <= 0: t = n + f, |f| <= 1/2, and the series of e^(f ln 2) up to its 12th term (the 13th is below 2e-16).
-// From -1100 down, and for the NaN of -inf * 0 (a masked logit at an infinite temperature), the result underflows to 0.
+// 0 from t = -1023 down, and for the NaN of -inf * 0 (a masked logit at an infinite temperature).
 __device__ __forceinline__ double vx_exp2_64(double t) {
     constexpr double L = 0.69314718055994530942;
-    t = fmax(t, -1100.0);
-    const double n = rint(t), f = t - n;
+    // 1.5 * 2^52 moves t's integer part into the low bits of the sum (the conversions and ldexp run at a quarter of the rate)
+    constexpr double SHIFT = 6755399441055744.0;
+    const double moved = fmax(t, -1100.0) + SHIFT, f = fmax(t, -1100.0) - (moved - SHIFT);
+    const int n = __double2loint(moved);
     double p = L * L * L * L * L * L * L * L * L * L * L * L / 479001600.0;
     p = __builtin_fma(p, f, L * L * L * L * L * L * L * L * L * L * L / 39916800.0);
     p = __builtin_fma(p, f, L * L * L * L * L * L * L * L * L * L / 3628800.0);
@@ -82,7 +84,7 @@ __device__ __forceinline__ double vx_exp2_64(double t) {
     p = __builtin_fma(p, f, L * L * 0.5);
     p = __builtin_fma(p, f, L);
     p = __builtin_fma(p, f, 1.0);
-    return ldexp(p, (int)n);
+    return p * __hiloint2double(max(n + 1023, 0) << 20, 0);        // 2^n, and 0 from n = -1023 down
 }
 // weight of a logit against the row's largest one; c = log2(e) / T
 __device__ __forceinline__ double vx_weight(float x, float m, double c) {
@@ -90,15 +92,17 @@ __device__ __forceinline__ double vx_weight(float x, float m, double c) {
 }
 __device__ __forceinline__ double vx_verify_c(float T) { return 1.44269504088896340736 / (double)T; }
 
-// the thread's values of a chunk, -inf where the row has ended
-template <int DT>
+// the thread's values of a chunk, -inf where the row has ended: pieces of 16 bytes, 256 apart (the threads side by side) or
+// (IN_ORDER) next to each other
+template <int DT, bool IN_ORDER = false>
 __device__ __forceinline__ void vx_verify_load(const typename vx_elem<DT>::type *row, int c0, int V,
                                                float x[VX_VERIFY_U * 16 / sizeof(typename vx_elem<DT>::type)]) {
     constexpr int VEC = 16 / sizeof(typename vx_elem<DT>::type);
     vx_vec<DT> v[VX_VERIFY_U];
+    auto piece = [](int u) { return IN_ORDER ? threadIdx.x * VX_VERIFY_U + u : u * 256 + threadIdx.x; };
     if (c0 + vx_verify_chunk<DT>() <= V) {
 #pragma unroll
-        for (int u = 0; u < VX_VERIFY_U; ++u) v[u].raw = vx_load16<DT>(row + c0 + (u * 256 + threadIdx.x) * VEC);
+        for (int u = 0; u < VX_VERIFY_U; ++u) v[u].raw = vx_load16<DT>(row + c0 + piece(u) * VEC);
 #pragma unroll
         for (int u = 0; u < VX_VERIFY_U; ++u)
 #pragma unroll
@@ -106,7 +110,7 @@ __device__ __forceinline__ void vx_verify_load(const typename vx_elem<DT>::type 
     } else {
 #pragma unroll
         for (int u = 0; u < VX_VERIFY_U; ++u) {
-            const int at = c0 + (u * 256 + threadIdx.x) * VEC;
+            const int at = c0 + piece(u) * VEC;
             v[u] = vx_load_vec<DT>(row + at, V - at);
 #pragma unroll
             for (int k = 0; k < VEC; ++k) x[u * VEC + k] = at + k < V ? (float)v[u].e[k] : -INFINITY;
@@ -220,34 +224,48 @@ __global__ __launch_bounds__(256) void vx_k_verify_choose(vx_verify_args a) {
     const float T = a.temperature[b];
     const bool greedy = !(T > 0.f), has_q = a.draft && !greedy;
     const double c = vx_verify_c(T);
-    // largest logit and sum of each row: one wave a row, its lanes over the chunks
-    for (int i = w; i < (has_q ? 2 * n + 1 : n + 1); i += 4) {
+    // lane j of the first wave decides on draft j; what it needs is on its way while the rows are summed
+    long long x = 0;
+    float tx = 0.f, dx = 0.f, un = 0.f;
+    bool in = false;
+    if (w == 0 && lane < n) {
+        x = a.tokens[(long long)b * K + lane];
+        un = a.uniforms[(long long)b * (K + 1) + lane];
+        in = x >= 0 && x < a.V;
+        if (in) tx = (float)vx_verify_target<DT>(a, b, lane)[x];
+        if (in && has_q) dx = (float)vx_verify_draft<DT>(a, b, lane)[x];
+    }
+    // largest logit and sum of each row: 16 lanes a row, over its chunks
+    for (int i0 = 0; i0 < (has_q ? 2 * n + 1 : n + 1); i0 += 16) {
+        const int i = i0 + (threadIdx.x >> 4), sub = lane & 15;
+        const bool row = i < (has_q ? 2 * n + 1 : n + 1);
         const int j = i <= n ? i : K + 1 + (i - n - 1);           // row of the statistics
         const float2 *st = a.stats + ((long long)b * (2 * K + 1) + j) * a.chunks;
         float m = -INFINITY;
         bool bad = false;
-        for (int k = lane; k < a.chunks; k += 64) {
-            const float v = st[k].x;
-            bad |= v != v;
-            m = fmaxf(m, v);
-        }
+        if (row)
+            for (int k = sub; k < a.chunks; k += 16) {
+                const float v = st[k].x;
+                bad |= v != v;
+                m = fmaxf(m, v);
+            }
 #pragma unroll
-        for (int k = 32; k >= 1; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, VX_WAVE));
-        bad = __any(bad);
+        for (int k = 8; k >= 1; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, VX_WAVE));
+        bad = (__ballot(bad) >> (lane & 48)) & 0xffff;
         double z = 0.0;
         int best = 0x7fffffff;
-        if (!bad && m != -INFINITY)
-            for (int k = lane; k < a.chunks; k += 64) {
+        if (row && !bad && m != -INFINITY)
+            for (int k = sub; k < a.chunks; k += 16) {
                 const float2 v = st[k];
                 if (greedy) best = v.x == m ? min(best, __float_as_int(v.y)) : best;
                 else if (v.y > 0.f) z += (double)v.y * vx_weight(v.x, m, c);
             }
 #pragma unroll
-        for (int k = 32; k >= 1; k >>= 1) {
+        for (int k = 8; k >= 1; k >>= 1) {
             z += __shfl_xor(z, k, VX_WAVE);
             best = min(best, __shfl_xor(best, k, VX_WAVE));
         }
-        if (lane == 0) {
+        if (row && sub == 0) {
             const int at = i <= n ? i : VX_MAX_DRAFTS + 1 + (i - n - 1);
             s_m[at] = bad ? __builtin_nanf("") : m;
             s_z[at] = z;
@@ -256,15 +274,11 @@ __global__ __launch_bounds__(256) void vx_k_verify_choose(vx_verify_args a) {
     }
     __syncthreads();
     auto invalid = [](float m) { return m != m ? VX_STATUS_NAN : (m == -INFINITY ? VX_STATUS_EMPTY_ROW : 0); };
-    // lane j of the first wave decides on draft j
-    long long x = 0;
     double ratio = 0.0, p = 0.0, uq = 0.0;
     int st = 0;
     if (w == 0) {
         bool ok = false, unsure = false;
         if (lane < n) {
-            x = a.tokens[(long long)b * K + lane];
-            const bool in = x >= 0 && x < a.V;
             const int t_bad = invalid(s_m[lane]), q_bad = has_q ? invalid(s_m[VX_MAX_DRAFTS + 1 + lane]) : 0;
             st = t_bad | q_bad | (in ? 0 : VX_STATUS_BAD_TOKEN);
             if (in && !t_bad && !q_bad) {
@@ -272,19 +286,19 @@ __global__ __launch_bounds__(256) void vx_k_verify_choose(vx_verify_args a) {
                     ok = s_best[lane] == x;
                     ratio = ok ? 1.0 : 0.0;
                 } else {
-                    p = vx_weight((float)vx_verify_target<DT>(a, b, lane)[x], s_m[lane], c) / s_z[lane];
-                    const double q = has_q ? vx_weight((float)vx_verify_draft<DT>(a, b, lane)[x], s_m[VX_MAX_DRAFTS + 1 + lane], c) / s_z[VX_MAX_DRAFTS + 1 + lane] : 1.0;
-                    uq = (double)a.uniforms[(long long)b * (K + 1) + lane] * q;
+                    p = vx_weight(tx, s_m[lane], c) / s_z[lane];
+                    const double q = has_q ? vx_weight(dx, s_m[VX_MAX_DRAFTS + 1 + lane], c) / s_z[VX_MAX_DRAFTS + 1 + lane] : 1.0;
+                    uq = (double)un * q;
                     ok = uq < p;
                     unsure = p > 0.0 && fabs(uq - p) <= p * (1.0 / 32768.0);
                     ratio = p >= q ? (p > 0.0 ? 1.0 : 0.0) : p / q;
                 }
             }
         }
-        const u64 oks = __ballot(ok), un = __ballot(unsure), sure_no = __ballot(lane < n && !ok && !unsure);
+        const u64 oks = __ballot(ok), maybe = __ballot(unsure), sure_no = __ballot(lane < n && !ok && !unsure);
         if (lane == 0) {
             s_ok = oks;
-            s_unsure = un & (sure_no ? (sure_no & (0 - sure_no)) - 1 : ~0ull);     // those in front of the first certain rejection
+            s_unsure = maybe & (sure_no ? (sure_no & (0 - sure_no)) - 1 : ~0ull);     // those in front of the first certain rejection
         }
     }
     __syncthreads();
@@ -369,11 +383,11 @@ __device__ __forceinline__ int vx_pick_part(double sum, double base, double goal
     return first < 256 ? first : -1;
 }
 
-// The first i whose cumulative weight passes u * total; `sums(k)` the weight of chunk k, `weight(i)` of one token.  One
-// workgroup: first the chunk, then the 1/256 of it, then the token; where rounding leaves none, the last one with a weight.
-// -1 where no token has a weight.
-template <int CHUNK, class S, class W>
-__device__ __forceinline__ int vx_verify_pick(int chunks, int V, float u, S sums, W weight, vx_pick_smem &sm, double *s_sum) {
+// The first i whose cumulative weight passes u * total; `sums(k)` the weight of chunk k, `weight(i)` of one token, `part(i)` of
+// the CHUNK / 256 tokens from i on.  One workgroup: first the chunk, then the 1/256 of it, then the token; where rounding
+// leaves none, the last one with a weight.  -1 where no token has a weight.
+template <int CHUNK, class S, class P, class W>
+__device__ __forceinline__ int vx_verify_pick(int chunks, int V, float u, S sums, P part_weight, W weight, vx_pick_smem &sm, double *s_sum) {
     constexpr int PART = CHUNK / 256;
     const int tid = threadIdx.x, per = (chunks + 255) / 256;      // chunks of one thread
     double mine = 0.0, before;
@@ -394,11 +408,7 @@ __device__ __forceinline__ int vx_verify_pick(int chunks, int V, float u, S sums
         }
         chunk = c < 0 ? chunk : c;
     }
-    const int at = chunk * CHUNK + tid * PART;
-    mine = 0.0;
-#pragma unroll 4
-    for (int k = 0; k < PART; ++k)
-        if (at + k < V) mine += weight(at + k);
+    mine = part_weight(chunk * CHUNK + tid * PART);
     part = vx_pick_part(mine, before, goal, sm, before, last);
     if (part < 0) { part = max(last, 0); goal = INFINITY; }
     const int i = chunk * CHUNK + part * PART + tid;
@@ -447,36 +457,47 @@ __global__ __launch_bounds__(256) void vx_k_verify_rest(vx_verify_args a) {
 // The drawn token: one workgroup per sequence.
 template <int DT>
 __global__ __launch_bounds__(256) void vx_k_verify_draw(vx_verify_args a) {
-    constexpr int CHUNK = vx_verify_chunk<DT>();
+    constexpr int CHUNK = vx_verify_chunk<DT>(), PER = CHUNK / 256;
     __shared__ double s_sum[4];
     __shared__ vx_pick_smem sm;
     const int b = blockIdx.x;
     const vx_choice ch = a.choice[b];
+    const float u = a.uniforms[(long long)b * (a.K + 1) + a.K];
+    const double c = vx_verify_c(a.temperature[b]);
     if (ch.mode == 0) return;
     const typename vx_elem<DT>::type *trow = vx_verify_target<DT>(a, b, ch.row);
-    const double c = vx_verify_c(a.temperature[b]);
     const double2 *z = a.z + (long long)b * a.chunks;
-    const float u = a.uniforms[(long long)b * (a.K + 1) + a.K];
     auto from_p = [&](long long drop) {
-        const double dropped = drop >= 0 && drop < a.V ? vx_weight((float)trow[drop], ch.mp, c) : 0.0;
-        const int drop_chunk = dropped > 0.0 ? (int)(drop / CHUNK) : -1;
         auto one = [&](int i) { return i == drop ? 0.0 : vx_weight((float)trow[i], ch.mp, c); };
+        auto part = [&](int i) {                                  // i = the chunk's first token + threadIdx.x * PER
+            float x[PER];
+            vx_verify_load<DT, true>(trow, i - threadIdx.x * PER, a.V, x);
+            double sum = 0.0;
+#pragma unroll 4
+            for (int k = 0; k < PER; ++k) sum += i + k == drop ? 0.0 : vx_weight(x[k], ch.mp, c);
+            return sum;
+        };
         // a chunk that loses a token is summed again: its sum less the token's weight could be all rounding
-        double again = 0.0;
-        if (drop_chunk >= 0) {
-            for (int k = threadIdx.x; k < CHUNK; k += 256)
-                if (drop_chunk * CHUNK + k < a.V) again += one(drop_chunk * CHUNK + k);
-            again = vx_verify_sum(again, s_sum);
-        }
-        return vx_verify_pick<CHUNK>(a.chunks, a.V, u, [&](int k) { return k == drop_chunk ? again : z[k].x; }, one, sm, s_sum);
+        const int drop_chunk = drop >= 0 && drop < a.V ? (int)(drop / CHUNK) : -1;
+        const double again = drop_chunk >= 0 ? vx_verify_sum(part(drop_chunk * CHUNK + threadIdx.x * PER), s_sum) : 0.0;
+        return vx_verify_pick<CHUNK>(a.chunks, a.V, u, [&](int k) { return k == drop_chunk ? again : z[k].x; }, part, one, sm, s_sum);
     };
     int i;
     if (ch.mode == 3) {
         const typename vx_elem<DT>::type *drow = vx_verify_draft<DT>(a, b, ch.row);
         const double2 t = vx_verify_totals(a, b, s_sum);
         const double ip = 1.0 / t.x, iq = 1.0 / t.y, *r = a.r + (long long)b * a.chunks;
-        i = vx_verify_pick<CHUNK>(a.chunks, a.V, u, [&](int k) { return r[k]; },
-                                  [&](int k) { return vx_verify_rest((float)trow[k], (float)drow[k], ch, c, ip, iq); }, sm, s_sum);
+        auto one = [&](int k) { return vx_verify_rest((float)trow[k], (float)drow[k], ch, c, ip, iq); };
+        auto part = [&](int i) {
+            float x[PER], y[PER];
+            vx_verify_load<DT, true>(trow, i - threadIdx.x * PER, a.V, x);
+            vx_verify_load<DT, true>(drow, i - threadIdx.x * PER, a.V, y);
+            double sum = 0.0;
+#pragma unroll 4
+            for (int k = 0; k < PER; ++k) sum += vx_verify_rest(x[k], y[k], ch, c, ip, iq);
+            return sum;
+        };
+        i = vx_verify_pick<CHUNK>(a.chunks, a.V, u, [&](int k) { return r[k]; }, part, one, sm, s_sum);
     } else {
         i = from_p(ch.drop);
     }
