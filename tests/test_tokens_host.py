@@ -81,19 +81,19 @@ def test_verify_refusals():
     nb = lib.vx_verify_drafts_workspace_bytes(2, 3, 100)
     assert nb > 0 and lib.vx_verify_drafts_workspace_bytes(2, 65, 100) == 0 and lib.vx_verify_drafts_workspace_bytes(0, 3, 100) == 0
     assert lib.vx_verify_drafts_workspace_bytes(65536, 3, 100) == 0 and lib.vx_verify_drafts_workspace_bytes(2, 0, 100) > 0
-    ok = [P, 400, 100, P, 300, 100, 2, P, None, P, P, 2, 3, 100, P, P, P, P, P, nb, None]
+    ok = [P, 400, 100, P, 300, 100, 2, P, None, P, P, 1.0, 2, 3, 100, P, P, P, P, P, nb, None]
 
     def rc(**kw):
         a = list(ok)
         for i, v in kw.items():
             a[int(i[1:])] = v
         return lib.vx_verify_drafts(*a)
-    for i in (0, 7, 9, 10, 14, 15, 16, 17, 18):
+    for i in (0, 7, 9, 15, 16, 17, 18, 19):
         assert rc(**{"a%d" % i: None}) == -1
-    assert rc(a6=4) == -1 and rc(a11=0) == -1 and rc(a12=-1) == -1 and rc(a13=0) == -1 and rc(a2=-1) == -1 and rc(a5=-1) == -1
-    assert rc(a11=65536, a19=BIG) == -2 and rc(a12=65, a19=BIG) == -2 and rc(a13=1 << 30, a19=BIG) == -2
-    assert rc(a19=nb - 1) == -3
-    assert rc(a0=P + 1) == -5 and rc(a3=P + 1) == -5 and rc(a7=P + 4) == -5 and rc(a14=P + 4) == -5 and rc(a8=P + 2) == -5 and rc(a18=P + 64) == -5
+    assert rc(a6=4) == -1 and rc(a12=0) == -1 and rc(a13=-1) == -1 and rc(a14=0) == -1 and rc(a2=-1) == -1 and rc(a5=-1) == -1
+    assert rc(a12=65536, a20=BIG) == -2 and rc(a13=65, a20=BIG) == -2 and rc(a14=1 << 30, a20=BIG) == -2
+    assert rc(a20=nb - 1) == -3
+    assert rc(a0=P + 1) == -5 and rc(a3=P + 1) == -5 and rc(a7=P + 4) == -5 and rc(a15=P + 4) == -5 and rc(a8=P + 2) == -5 and rc(a19=P + 64) == -5
 
 
 def test_functional_layer_refuses_cpu_tensors():

@@ -27,7 +27,8 @@ struct vx_verify_args {
     const long long *tokens;                      // [B, K]
     const int *lens;                              // [B] or nullptr
     const float *uniforms;                        // [B, K + 1]
-    const float *temperature;                     // [B]
+    const float *temperature;                     // [B] or nullptr: one_temperature
+    float one_temperature;
     int B, K, V, chunks;
     // workspace
     float2 *stats;                                // [B][2 K + 1][chunks]: largest logit (NaN: an invalid one), sum (greedy: index)
@@ -54,6 +55,7 @@ template <int DT> __host__ __device__ constexpr int vx_verify_chunk() { return 2
 __device__ __forceinline__ int vx_verify_len(const vx_verify_args &a, int b) {
     return a.lens ? vx_clamp_count(a.lens[b], a.K) : a.K;
 }
+__device__ __forceinline__ float vx_verify_t(const vx_verify_args &a, int b) { return a.temperature ? a.temperature[b] : a.one_temperature; }
 template <int DT>
 __device__ __forceinline__ const typename vx_elem<DT>::type *vx_verify_target(const vx_verify_args &a, int b, int j) {
     return (const typename vx_elem<DT>::type *)a.target + b * a.t_seq + j * a.t_row;
@@ -128,7 +130,7 @@ __global__ __launch_bounds__(256) void vx_k_verify_stats(vx_verify_args a) {
     const int item = blockIdx.x / a.chunks, chunk = blockIdx.x - item * a.chunks;
     const int b = item / rows, j = item - b * rows, n = vx_verify_len(a, b);
     const bool is_draft = j > a.K;
-    const float T = a.temperature[b];
+    const float T = vx_verify_t(a, b);
     const bool greedy = !(T > 0.f);
     if (is_draft ? (j - a.K - 1 >= n || greedy) : j > n) return;
     float x[PER];
@@ -221,7 +223,7 @@ __global__ __launch_bounds__(256) void vx_k_verify_choose(vx_verify_args a) {
     __shared__ u64 s_ok, s_unsure;
     const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks, K = a.K, n = vx_verify_len(a, b);
     const int lane = vx_lane(), w = threadIdx.x >> 6;
-    const float T = a.temperature[b];
+    const float T = vx_verify_t(a, b);
     const bool greedy = !(T > 0.f), has_q = a.draft && !greedy;
     const double c = vx_verify_c(T);
     // lane j of the first wave decides on draft j; what it needs is on its way while the rows are summed
@@ -444,7 +446,7 @@ __global__ __launch_bounds__(256) void vx_k_verify_rest(vx_verify_args a) {
     float x[PER], y[PER];
     vx_verify_load<DT>(vx_verify_target<DT>(a, b, ch.row), chunk * CHUNK, a.V, x);
     vx_verify_load<DT>(vx_verify_draft<DT>(a, b, ch.row), chunk * CHUNK, a.V, y);
-    const double c = vx_verify_c(a.temperature[b]);
+    const double c = vx_verify_c(vx_verify_t(a, b));
     const double2 z = vx_verify_totals(a, b, s_sum);
     const double ip = 1.0 / z.x, iq = 1.0 / z.y;
     double sum = 0.0;
@@ -463,7 +465,7 @@ __global__ __launch_bounds__(256) void vx_k_verify_draw(vx_verify_args a) {
     const int b = blockIdx.x;
     const vx_choice ch = a.choice[b];
     const float u = a.uniforms[(long long)b * (a.K + 1) + a.K];
-    const double c = vx_verify_c(a.temperature[b]);
+    const double c = vx_verify_c(vx_verify_t(a, b));
     if (ch.mode == 0) return;
     const typename vx_elem<DT>::type *trow = vx_verify_target<DT>(a, b, ch.row);
     const double2 *z = a.z + (long long)b * a.chunks;
@@ -530,10 +532,10 @@ extern "C" size_t vx_verify_drafts_workspace_bytes(int B, int K, int V) {
 
 extern "C" int vx_verify_drafts(const void *d_target, int64_t target_seq_stride, int64_t target_row_stride, const void *d_draft,
                                 int64_t draft_seq_stride, int64_t draft_row_stride, int dtype, const int64_t *d_draft_tokens,
-                                const int32_t *d_draft_lens, const float *d_uniforms, const float *d_temperature, int B, int K,
-                                int V, int64_t *d_tokens, int32_t *d_counts, float *d_accept, int32_t *d_status,
+                                const int32_t *d_draft_lens, const float *d_uniforms, const float *d_temperature, float temperature,
+                                int B, int K, int V, int64_t *d_tokens, int32_t *d_counts, float *d_accept, int32_t *d_status,
                                 void *d_workspace, size_t workspace_bytes, void *stream) {
-    if (!d_target || !d_uniforms || !d_temperature || !d_tokens || !d_counts || !d_status || !d_workspace || B <= 0 || K < 0 || V <= 0) return VX_ERR_INVALID_ARG;
+    if (!d_target || !d_uniforms || !d_tokens || !d_counts || !d_status || !d_workspace || B <= 0 || K < 0 || V <= 0) return VX_ERR_INVALID_ARG;
     if ((K > 0 && (!d_draft_tokens || !d_accept)) || !vx_dtype_ok(dtype)) return VX_ERR_INVALID_ARG;
     if (target_row_stride < 0 || target_seq_stride < 0 || draft_row_stride < 0 || draft_seq_stride < 0) return VX_ERR_INVALID_ARG;
     if (B > VX_MAX_VERIFY_BATCH || K > VX_MAX_DRAFTS || V > VX_MAX_VOCAB) return VX_ERR_UNSUPPORTED;
@@ -549,7 +551,7 @@ extern "C" int vx_verify_drafts(const void *d_target, int64_t target_seq_stride,
     if (blocks > 2147483647LL) return VX_ERR_UNSUPPORTED;
     char *ws = (char *)d_workspace;
     const vx_verify_args a = {d_target, d_draft, target_seq_stride, target_row_stride, draft_seq_stride, draft_row_stride,
-                              (const long long *)d_draft_tokens, d_draft_lens, d_uniforms, d_temperature, B, K, V, p.chunks,
+                              (const long long *)d_draft_tokens, d_draft_lens, d_uniforms, d_temperature, temperature, B, K, V, p.chunks,
                               (float2 *)(ws + p.stats), (double2 *)(ws + p.z), (double *)(ws + p.r), (vx_choice *)(ws + p.choice),
                               (long long *)d_tokens, d_counts, d_status, d_accept};
     hipStream_t st = (hipStream_t)stream;

@@ -405,29 +405,44 @@ def softmax_max(logits: torch.Tensor) -> torch.Tensor:
 _DTYPES = {torch.float32: L.VX_DTYPE_F32, torch.float16: L.VX_DTYPE_F16, torch.bfloat16: L.VX_DTYPE_BF16}
 
 
-def _need(ok: bool, what: str):
-    if not ok:
-        raise L.VortexHipError(what)
+_IDS = (torch.int64, torch.int32)
+
+
+def _bad(what: str, *args):
+    raise L.VortexHipError(what % args)
 
 
 def _tensor(t, name: str, device, dtypes, ndim: Optional[int] = None):
     """Argument check of the token-model operators: a GPU tensor on `device` (None: any GPU) of one of `dtypes`."""
-    _need(torch.is_tensor(t), "%s must be a tensor, got %s" % (name, type(t).__name__))
+    if (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes and (device is None or t.device == device)
+            and (ndim is None or t.dim() == ndim)):
+        return
+    if not isinstance(t, torch.Tensor):
+        _bad("%s must be a tensor, got %s", name, type(t).__name__)
     L.require_cuda(t, name)
-    _need(device is None or t.device == device, "%s lives on %s, the other arguments on %s" % (name, t.device, device))
-    _need(t.dtype in dtypes, "%s has dtype %s, expected one of %s" % (name, t.dtype, [str(d) for d in dtypes]))
-    _need(ndim is None or t.dim() == ndim, "%s must have %s dimensions, got shape %s" % (name, ndim, tuple(t.shape)))
+    if t.dtype not in dtypes:
+        _bad("%s has dtype %s, expected one of %s", name, t.dtype, [str(d) for d in dtypes])
+    if device is not None and t.device != device:
+        _bad("%s lives on %s, the other arguments on %s", name, t.device, device)
+    _bad("%s must have %s dimensions, got shape %s", name, ndim, tuple(t.shape))
 
 
-def _rows(x: torch.Tensor, name: str) -> torch.Tensor:
+def _rows(x: torch.Tensor) -> torch.Tensor:
     """[M, K] with unit stride along K and rows that do not overlap (copied when it is anything else)."""
-    if x.stride(1) != 1 and x.size(1) > 1 or (x.size(0) > 1 and x.stride(0) < x.size(1)):
-        x = x.contiguous()
-    return x
+    if x.is_contiguous() or (x.stride(1) == 1 and x.stride(0) >= x.size(1)):
+        return x
+    return x.contiguous()
 
 
 def _row_stride(x: torch.Tensor) -> int:
     return max(x.stride(0), x.size(1)) if x.size(0) > 1 else x.size(1)
+
+
+def _status_word(status, device) -> int:
+    _tensor(status, "status", device, (torch.int32,))
+    if status.numel() < 1:
+        _bad("status is empty")
+    return status.data_ptr()
 
 
 @_on_device
@@ -436,20 +451,19 @@ def embed_tokens(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
     """i32/i64[...] ids, table [V,D] (f32, f16 or bf16) -> [..., D] = scale * table[ids]; an id below 0 is padding (zeros),
     an id >= V gives zeros and sets VX_STATUS_BAD_TOKEN in `status` (i32[1], zeroed by the caller) when one is given.
     No autograd: TokenEmbedding has it.  See vx_embed_tokens."""
-    _tensor(ids, "ids", None, (torch.int64, torch.int32))
+    _tensor(ids, "ids", None, _IDS)
     dev = ids.device
     _tensor(table, "table", dev, _DTYPES, 2)
     V, D = table.shape
-    _need(V > 0 and D > 0, "table is empty: %s" % (tuple(table.shape),))
-    if status is not None:
-        _tensor(status, "status", dev, (torch.int32,))
-        _need(status.numel() >= 1, "status is empty")
-    ids, table = ids.contiguous(), _rows(table, "table")
+    if not (V and D):
+        _bad("table is empty: %s", tuple(table.shape))
+    st = None if status is None else _status_word(status, dev)
+    ids, table = ids.contiguous(), _rows(table)
     out = torch.empty(ids.shape + (D,), dtype=table.dtype, device=dev)
-    if ids.numel():
-        rc = L.lib().vx_embed_tokens(ids.data_ptr(), ids.element_size(), ids.numel(), table.data_ptr(), V, D,
-                                     _row_stride(table), _DTYPES[table.dtype], float(scale), out.data_ptr(),
-                                     status.data_ptr() if status is not None else None, L.stream_ptr(dev))
+    T = ids.numel()
+    if T:
+        rc = L.lib().vx_embed_tokens(ids.data_ptr(), ids.element_size(), T, table.data_ptr(), V, D, _row_stride(table),
+                                     _DTYPES[table.dtype], scale, out.data_ptr(), st, L.stream_ptr(dev))
         L.check(rc, "vx_embed_tokens")
     return out
 
@@ -460,21 +474,20 @@ def embed_tokens_grad(ids: torch.Tensor, grad_out: torch.Tensor, n_rows: int, sc
     """Gradient of embed_tokens with respect to the table: [n_rows, D] in grad_out's type, or, with `out` ([n_rows, D]
     contiguous, grad_out's type or f32), added to the rows of `out` that some id points to.  fp32 sums in a fixed
     order.  See vx_embed_tokens_grad."""
-    _tensor(ids, "ids", None, (torch.int64, torch.int32))
+    _tensor(ids, "ids", None, _IDS)
     dev = ids.device
     _tensor(grad_out, "grad_out", dev, _DTYPES, ids.dim() + 1)
-    _need(tuple(grad_out.shape[:-1]) == tuple(ids.shape),
-          "grad_out %s does not fit ids %s" % (tuple(grad_out.shape), tuple(ids.shape)))
+    if grad_out.shape[:-1] != ids.shape:
+        _bad("grad_out %s does not fit ids %s", tuple(grad_out.shape), tuple(ids.shape))
     n_rows, D = int(n_rows), grad_out.size(-1)
-    _need(n_rows > 0 and D > 0, "the gradient of an empty table was asked for: [%d, %d]" % (n_rows, D))
-    if status is not None:
-        _tensor(status, "status", dev, (torch.int32,))
-        _need(status.numel() >= 1, "status is empty")
+    if n_rows <= 0 or D == 0:
+        _bad("the gradient of an empty table was asked for: [%d, %d]", n_rows, D)
+    st = None if status is None else _status_word(status, dev)
     accumulate = out is not None
     if accumulate:
         _tensor(out, "out", dev, (grad_out.dtype, torch.float32), 2)
-        _need(tuple(out.shape) == (n_rows, D) and out.is_contiguous(),
-              "out must be a contiguous [%d, %d] tensor, got %s with strides %s" % (n_rows, D, tuple(out.shape), out.stride()))
+        if tuple(out.shape) != (n_rows, D) or not out.is_contiguous():
+            _bad("out must be a contiguous [%d, %d] tensor, got %s with strides %s", n_rows, D, tuple(out.shape), out.stride())
     T = ids.numel()
     if T == 0:
         return out if accumulate else torch.zeros((n_rows, D), dtype=grad_out.dtype, device=dev)
@@ -485,10 +498,16 @@ def embed_tokens_grad(ids: torch.Tensor, grad_out: torch.Tensor, n_rows: int, sc
     nb = lib.vx_embed_tokens_grad_workspace_bytes(T, n_rows, D)
     ws = _ws(nb, dev)
     rc = lib.vx_embed_tokens_grad(ids.data_ptr(), ids.element_size(), T, grad_out.data_ptr(), _DTYPES[grad_out.dtype], n_rows, D,
-                                  float(scale), out.data_ptr(), _DTYPES[out.dtype], int(accumulate),
-                                  status.data_ptr() if status is not None else None, ws.data_ptr(), nb, L.stream_ptr(dev))
+                                  scale, out.data_ptr(), _DTYPES[out.dtype], int(accumulate), st, ws.data_ptr(), nb,
+                                  L.stream_ptr(dev))
     L.check(rc, "vx_embed_tokens_grad")
     return out
+
+
+def _last_dim(x, name: str) -> int:
+    if x.dim() < 1 or x.size(-1) == 0:
+        _bad("%s needs a last dimension of at least 1, got %s", name, tuple(x.shape))
+    return x.size(-1)
 
 
 @_on_device
@@ -496,15 +515,14 @@ def quantize_rows_i8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """[..., K] (f32, f16, bf16) -> (i8[..., K], f32[...]): each row scaled by its largest magnitude to +-127.
     See vx_quantize_rows_i8."""
     _tensor(x, "input", None, _DTYPES)
-    _need(x.dim() >= 1 and x.size(-1) > 0, "input needs a last dimension of at least 1, got %s" % (tuple(x.shape),))
-    K, lead = x.size(-1), x.shape[:-1]
+    K, lead, dev = _last_dim(x, "input"), x.shape[:-1], x.device
     M = x.numel() // K
-    q = torch.empty(lead + (K,), dtype=torch.int8, device=x.device)
-    s = torch.empty(lead, dtype=torch.float32, device=x.device)
+    q = torch.empty(x.shape, dtype=torch.int8, device=dev)
+    s = torch.empty(lead, dtype=torch.float32, device=dev)
     if M:
-        x2 = _rows(x.reshape(M, K), "input")
-        rc = L.lib().vx_quantize_rows_i8(x2.data_ptr(), _DTYPES[x.dtype], M, K, _row_stride(x2), q.data_ptr(), K, s.data_ptr(),
-                                         L.stream_ptr(x.device))
+        x = _rows(x if x.dim() == 2 else x.reshape(M, K))
+        rc = L.lib().vx_quantize_rows_i8(x.data_ptr(), _DTYPES[x.dtype], M, K, _row_stride(x), q.data_ptr(), K, s.data_ptr(),
+                                         L.stream_ptr(dev))
         L.check(rc, "vx_quantize_rows_i8")
     return q, s
 
@@ -512,15 +530,19 @@ def quantize_rows_i8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 def _linear_weights(qw, w_scale, bias, K: int, dev):
     _tensor(qw, "qw", dev, (torch.int8,), 2)
     N = qw.size(0)
-    _need(qw.size(1) == K, "qw %s does not fit rows of %d values" % (tuple(qw.shape), K))
-    _need(N > 0, "qw has no rows")
+    if qw.size(1) != K:
+        _bad("qw %s does not fit rows of %d values", tuple(qw.shape), K)
+    if N == 0:
+        _bad("qw has no rows")
     _tensor(w_scale, "w_scale", dev, (torch.float32,), 1)
-    _need(w_scale.numel() == N, "w_scale has %d values for %d channels" % (w_scale.numel(), N))
+    if w_scale.numel() != N:
+        _bad("w_scale has %d values for %d channels", w_scale.numel(), N)
     if bias is not None:
         _tensor(bias, "bias", dev, (torch.float32,), 1)
-        _need(bias.numel() == N, "bias has %d values for %d channels" % (bias.numel(), N))
+        if bias.numel() != N:
+            _bad("bias has %d values for %d channels", bias.numel(), N)
         bias = bias.contiguous()
-    qw = _rows(qw, "qw")
+    qw = _rows(qw)
     if K % 16 == 0 and (qw.data_ptr() % 16 or qw.stride(0) % 16):
         qw = qw.contiguous()                     # a slice of wider rows: the tile kernel takes 16-byte aligned ones
     return qw, w_scale.contiguous(), bias, N
@@ -533,20 +555,21 @@ def linear_i8(q: torch.Tensor, scale: torch.Tensor, qw: torch.Tensor, w_scale: t
     scale * w_scale * (exact integer sum) + bias.  See vx_linear_i8."""
     _tensor(q, "q", None, (torch.int8,))
     dev = q.device
-    _need(q.dim() >= 1 and q.size(-1) > 0, "q needs a last dimension of at least 1, got %s" % (tuple(q.shape),))
-    K, lead = q.size(-1), q.shape[:-1]
+    K, lead = _last_dim(q, "q"), q.shape[:-1]
     _tensor(scale, "scale", dev, (torch.float32,))
-    _need(tuple(scale.shape) == tuple(lead), "scale %s does not fit q %s" % (tuple(scale.shape), tuple(q.shape)))
-    _need(out_dtype in _DTYPES, "out_dtype %s: expected one of %s" % (out_dtype, [str(d) for d in _DTYPES]))
+    if scale.shape != lead:
+        _bad("scale %s does not fit q %s", tuple(scale.shape), tuple(q.shape))
+    if out_dtype not in _DTYPES:
+        _bad("out_dtype %s: expected one of %s", out_dtype, [str(d) for d in _DTYPES])
     qw, w_scale, bias, N = _linear_weights(qw, w_scale, bias, K, dev)
     M = q.numel() // K
     out = torch.empty(lead + (N,), dtype=out_dtype, device=dev)
     if M:
         lib = L.lib()
-        q2, scale = _rows(q.reshape(M, K), "q"), scale.contiguous()
+        q, scale = _rows(q if q.dim() == 2 else q.reshape(M, K)), scale.contiguous()
         nb = lib.vx_linear_i8_workspace_bytes(M, N, K)
         ws = _ws(nb, dev)
-        rc = lib.vx_linear_i8(q2.data_ptr(), _row_stride(q2), scale.data_ptr(), M, qw.data_ptr(), _row_stride(qw),
+        rc = lib.vx_linear_i8(q.data_ptr(), _row_stride(q), scale.data_ptr(), M, qw.data_ptr(), _row_stride(qw),
                               w_scale.data_ptr(), N, K, bias.data_ptr() if bias is not None else None, out.data_ptr(),
                               _DTYPES[out_dtype], N, ws.data_ptr(), nb, L.stream_ptr(dev))
         L.check(rc, "vx_linear_i8")
@@ -560,19 +583,20 @@ def linear_w8a8(x: torch.Tensor, qw: torch.Tensor, w_scale: torch.Tensor, bias: 
     call, the same bits.  See vx_linear_w8a8."""
     _tensor(x, "input", None, _DTYPES)
     dev = x.device
-    _need(x.dim() >= 1 and x.size(-1) > 0, "input needs a last dimension of at least 1, got %s" % (tuple(x.shape),))
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    _need(out_dtype in _DTYPES, "out_dtype %s: expected one of %s" % (out_dtype, [str(d) for d in _DTYPES]))
-    K, lead = x.size(-1), x.shape[:-1]
+    if out_dtype is None:
+        out_dtype = x.dtype
+    elif out_dtype not in _DTYPES:
+        _bad("out_dtype %s: expected one of %s", out_dtype, [str(d) for d in _DTYPES])
+    K, lead = _last_dim(x, "input"), x.shape[:-1]
     qw, w_scale, bias, N = _linear_weights(qw, w_scale, bias, K, dev)
     M = x.numel() // K
     out = torch.empty(lead + (N,), dtype=out_dtype, device=dev)
     if M:
         lib = L.lib()
-        x2 = _rows(x.reshape(M, K), "input")
+        x = _rows(x if x.dim() == 2 else x.reshape(M, K))
         nb = lib.vx_linear_w8a8_workspace_bytes(M, N, K)
         ws = _ws(nb, dev)
-        rc = lib.vx_linear_w8a8(x2.data_ptr(), _DTYPES[x.dtype], _row_stride(x2), M, qw.data_ptr(), _row_stride(qw),
+        rc = lib.vx_linear_w8a8(x.data_ptr(), _DTYPES[x.dtype], _row_stride(x), M, qw.data_ptr(), _row_stride(qw),
                                 w_scale.data_ptr(), N, K, bias.data_ptr() if bias is not None else None, out.data_ptr(),
                                 _DTYPES[out_dtype], N, ws.data_ptr(), nb, L.stream_ptr(dev))
         L.check(rc, "vx_linear_w8a8")
@@ -588,46 +612,57 @@ def verify_drafts(target_logits: torch.Tensor, draft_tokens: torch.Tensor, unifo
     -> (tokens i64[B,K+1], counts i32[B], accept f32[B,K], status i32[B]); see vx_verify_drafts."""
     _tensor(target_logits, "target_logits", None, _DTYPES, 3)
     dev = target_logits.device
-    B, K, V = target_logits.size(0), target_logits.size(1) - 1, target_logits.size(2)
-    _need(K >= 0 and V > 0, "target_logits must be [batch, drafts + 1, vocabulary], got %s" % (tuple(target_logits.shape),))
+    B, K1, V = target_logits.shape
+    K = K1 - 1
+    if K < 0 or V == 0:
+        _bad("target_logits must be [batch, drafts + 1, vocabulary], got %s", tuple(target_logits.shape))
     _tensor(draft_tokens, "draft_tokens", dev, (torch.int64,), 2)
-    _need(tuple(draft_tokens.shape) == (B, K), "draft_tokens %s: expected %s" % (tuple(draft_tokens.shape), (B, K)))
+    if draft_tokens.shape != (B, K):
+        _bad("draft_tokens %s: expected %s", tuple(draft_tokens.shape), (B, K))
     _tensor(uniforms, "uniforms", dev, (torch.float32,), 2)
-    _need(tuple(uniforms.shape) == (B, K + 1), "uniforms %s: expected %s" % (tuple(uniforms.shape), (B, K + 1)))
-    if draft_logits is not None:
-        _tensor(draft_logits, "draft_logits", dev, (target_logits.dtype,), 3)
-        _need(tuple(draft_logits.shape) == (B, K, V), "draft_logits %s: expected %s" % (tuple(draft_logits.shape), (B, K, V)))
-        if draft_logits.stride(2) != 1 and V > 1:
-            draft_logits = draft_logits.contiguous()
+    if uniforms.shape != (B, K1):
+        _bad("uniforms %s: expected %s", tuple(uniforms.shape), (B, K1))
+    if V > 1 and target_logits.stride(2) != 1:
+        target_logits = target_logits.contiguous()
+    d = draft_logits
+    if d is not None:
+        _tensor(d, "draft_logits", dev, (target_logits.dtype,), 3)
+        if d.shape != (B, K, V):
+            _bad("draft_logits %s: expected %s", tuple(d.shape), (B, K, V))
+        if V > 1 and d.stride(2) != 1:
+            d = d.contiguous()
+        d = d if K else None
     if draft_lens is not None:
         _tensor(draft_lens, "draft_lens", dev, (torch.int32,), 1)
-        _need(draft_lens.numel() == B, "draft_lens has %d values for %d sequences" % (draft_lens.numel(), B))
+        if draft_lens.numel() != B:
+            _bad("draft_lens has %d values for %d sequences", draft_lens.numel(), B)
         draft_lens = draft_lens.contiguous()
-    if torch.is_tensor(temperature) and temperature.dim() > 0:
+    t_each, t_all = None, 0.0
+    if isinstance(temperature, torch.Tensor) and temperature.dim() > 0:
         _tensor(temperature, "temperature", dev, (torch.float32,), 1)
-        _need(temperature.numel() == B, "temperature has %d values for %d sequences" % (temperature.numel(), B))
-        temperature = temperature.contiguous()
+        if temperature.numel() != B:
+            _bad("temperature has %d values for %d sequences", temperature.numel(), B)
+        t_each = temperature.contiguous()
     else:
-        temperature = float(temperature)
-        _need(temperature >= 0.0, "temperature must not be negative, got %s" % temperature)
-        temperature = torch.full((B,), temperature, dtype=torch.float32, device=dev)
-    if target_logits.stride(2) != 1 and V > 1:
-        target_logits = target_logits.contiguous()
+        t_all = float(temperature)
+        if not t_all >= 0.0:
+            _bad("temperature must not be negative, got %s", t_all)
     draft_tokens, uniforms = draft_tokens.contiguous(), uniforms.contiguous()
-    tokens = torch.empty((B, K + 1), dtype=torch.int64, device=dev)
+    tokens = torch.empty((B, K1), dtype=torch.int64, device=dev)
     accept = torch.empty((B, K), dtype=torch.float32, device=dev)
-    counts, status = torch.empty((2, B), dtype=torch.int32, device=dev).unbind(0)
+    counts = torch.empty((B,), dtype=torch.int32, device=dev)
+    status = torch.empty((B,), dtype=torch.int32, device=dev)
     if B:
         lib = L.lib()
         nb = lib.vx_verify_drafts_workspace_bytes(B, K, V)
         ws = _ws(nb, dev)
-        d = draft_logits
         rc = lib.vx_verify_drafts(target_logits.data_ptr(), target_logits.stride(0), target_logits.stride(1),
-                                  d.data_ptr() if d is not None and K else None, d.stride(0) if d is not None else 0,
+                                  d.data_ptr() if d is not None else None, d.stride(0) if d is not None else 0,
                                   d.stride(1) if d is not None else 0, _DTYPES[target_logits.dtype],
                                   draft_tokens.data_ptr() if K else None, draft_lens.data_ptr() if draft_lens is not None else None,
-                                  uniforms.data_ptr(), temperature.data_ptr(), B, K, V, tokens.data_ptr(), counts.data_ptr(),
-                                  accept.data_ptr() if K else None, status.data_ptr(), ws.data_ptr(), nb, L.stream_ptr(dev))
+                                  uniforms.data_ptr(), t_each.data_ptr() if t_each is not None else None, t_all, B, K, V,
+                                  tokens.data_ptr(), counts.data_ptr(), accept.data_ptr() if K else None, status.data_ptr(),
+                                  ws.data_ptr(), nb, L.stream_ptr(dev))
         L.check(rc, "vx_verify_drafts")
     return tokens, counts, accept, status
 
