@@ -115,7 +115,7 @@ def check_grad(got, ref, err):
 
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("T,Vr,D", [(1, 1, 1), (2, 5, 8), (63, 40, 7), (64, 1000, 64), (1000, 3, 65), (1025, 5000, 100), (4097, 700, 1000),
-                                    (5000, 50021, 33), (20000, 300, 16), (3000, 1, 40), (9000, 70001, 24), (2048, 200, 520), (2049, 200, 520), (8191, 511, 8), (16384, 512, 8),
+                                    (5000, 50021, 33), (20000, 300, 16), (3000, 1, 40), (9000, 70001, 24), (64, 3, 520), (65, 3, 520), (255, 1, 24), (2049, 200, 520), (8192, 5, 8), (8191, 511, 8), (16384, 512, 8),
                                     (16385, 512, 8), (20001, 511, 9),
                                     (70000, 2, 12), (200000, 600000, 4)])
 def test_embed_grad(dt, T, Vr, D):

@@ -74,17 +74,19 @@ extern "C" int vx_embed_tokens(const void *d_ids, int id_bytes, int64_t n_tokens
 // ------------------------------------------------------------------------------------------------ gradient
 // 1. The tokens are sorted by id, stably, so the tokens of a table row lie next to each other in their own order: the sums
 //    have one order whatever the launch does.  Up to 16384 tokens by counting, for each token, the tokens in front of it
-//    (T^2 / 64 compares of a wave: 14 us of the chip's issue at 16384, 3.5 at 8192), beyond by a radix sort.
-// 2. Beyond 2048 tokens every full chunk of 32 sorted tokens of one id is summed once, and (from 8192 tokens) every full
-//    chunk of 32 such chunks: a frequent token's row costs at most 62 rows of grad_out, 62 chunks and one row for each
-//    further 1024 tokens, instead of all its tokens on one wave.
+//    (T^2 / 64 compares of a wave: 14 us of the chip's issue at 16384, 3.5 at 8192; measured 8.5 us at 2048, 13 at 5001),
+//    beyond by a radix sort (38 us at 65536).
+// 2. Beyond 64 tokens every full chunk of 16 sorted tokens of one id is summed once, and (from 8192 tokens) every full chunk
+//    of 16 such chunks: a frequent token's row costs at most 30 rows of grad_out, 30 chunks and one row for each further
+//    256 tokens, instead of all its tokens on one wave (chunks of 32 / 16 / 8: 49 / 42 / 41 us at 2048 x 1024 fp32, whose end is
+//    the longest such chain, 380 / 383 / 394 at 65536 x 4096 bf16).
 // 3. Each table row is written once, from its chunks and the tokens at their ends.
 #define VX_EG_COUNT_MAX 16384     // tokens sorted by counting
 #define VX_EG_SUB 2048            // tokens one workgroup of the radix sort ranks at a time: 256 threads x 8
 #define VX_EG_TILES 256           // workgroups of a sorting pass at most
 #define VX_EG_BINS 512            // 9 bits of the id for each pass at most
-#define VX_EG_CHUNK 32
-#define VX_EG_CHUNK_MIN 2048      // up to here no chunks: a long row is split over the waves of its workgroup
+#define VX_EG_CHUNK 16
+#define VX_EG_CHUNK_MIN 64
 #define VX_EG_CHUNK2_MIN 8192
 #define VX_EG_ROWS 8              // table rows of one workgroup
 
@@ -151,17 +153,24 @@ __global__ __launch_bounds__(1024) void vx_k_eg_count_sort(const void *__restric
     const unsigned k = s_key[t];
     const int per = (groups + 15) / 16, g0 = min(groups, w * per), g1 = min(groups, g0 + per);
     int n = 0;
-    for (int g = g0; g < g1; ++g) {
-        const uint4 q = *(const uint4 *)&s_key[4 * g];
-        if (4 * g + 3 < t0) {
-            n += (q.x <= k) + (q.y <= k) + (q.z <= k) + (q.w <= k);
-        } else if (4 * g >= t0 + 64) {
-            n += (q.x < k) + (q.y < k) + (q.z < k) + (q.w < k);
-        } else {
-            n += (q.x < k || (q.x == k && 4 * g < t)) + (q.y < k || (q.y == k && 4 * g + 1 < t)) +
-                 (q.z < k || (q.z == k && 4 * g + 2 < t)) + (q.w < k || (q.w == k && 4 * g + 3 < t));
+    auto below = [&](int from, int to, unsigned limit) {          // keys below `limit` in groups from .. to
+        int g = from;
+        for (; g + 8 <= to; g += 8) {
+            uint4 q[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q[i] = *(const uint4 *)&s_key[4 * (g + i)];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) n += (q[i].x < limit) + (q[i].y < limit) + (q[i].z < limit) + (q[i].w < limit);
         }
-    }
+        for (; g < to; ++g) {
+            const uint4 q = *(const uint4 *)&s_key[4 * g];
+            n += (q.x < limit) + (q.y < limit) + (q.z < limit) + (q.w < limit);
+        }
+    };
+    const int mid0 = min(max(g0, t0 / 4), g1), mid1 = min(max(g0, t0 / 4 + 16), g1);    // the groups of the 64 tokens themselves
+    below(g0, mid0, k + 1);
+    for (int i = 4 * mid0; i < 4 * mid1; ++i) n += s_key[i] < k || (s_key[i] == k && i < t);
+    below(mid1, g1, k);
     atomicAdd(&s_count[lane], n);
     __syncthreads();
     if (w == 0 && t0 + lane < T) {
@@ -290,31 +299,15 @@ __device__ __forceinline__ void vx_eg_add_n(const typename vx_elem<GT>::type *__
             for (int k = 0; k < VEC; ++k) sum[q * VEC + k] += (float)v[u][q].e[k];
 }
 
-// sum[] += rows of grad_out at pos[a..b), in that order.
-// LONG (chunks, and the rows of a call without chunks): the lanes fetch 64 positions together, eight rows are in flight.
-// Else (the ends of a row whose middle has chunks; most rows have a token or two): scalar positions and few registers --
-// with LONG's registers the rows of 65536 tokens x 4096 columns bf16 took 317 to 355 us instead of 270, and without LONG
-// the rows of 2048 x 1024 fp32 57 instead of 25 us.
-template <int GT, int U, bool TINY, bool LONG>
+// sum[] += rows of grad_out at pos[a..b), in that order.  The positions are scalar loads: as vector loads they wait for the
+// stores of the rows before (355 instead of 268 us for the rows of 65536 tokens x 4096 columns bf16).
+template <int GT, int U, bool TINY>
 __device__ __forceinline__ void vx_eg_add_tokens(const typename vx_elem<GT>::type *__restrict__ grad, const int *__restrict__ pos,
                                                  int a, int b, int D, int c, float *sum) {
-    if (!LONG || b - a < 8) {
-        auto at = [&](int u) { return pos[a + u]; };
-        for (; b - a >= 4; a += 4) vx_eg_add_n<GT, U, TINY, 4>(grad, at, D, c, sum);
-        if ((b - a) & 2) { vx_eg_add_n<GT, U, TINY, 2>(grad, at, D, c, sum); a += 2; }
-        if ((b - a) & 1) vx_eg_add_n<GT, U, TINY, 1>(grad, at, D, c, sum);
-        return;
-    }
-    for (; a < b; a += 64) {
-        const int n = min(64, b - a), lane = vx_lane();
-        const int mine = lane < n ? pos[a + lane] : 0;
-        int i = 0;
-        auto at = [&](int u) { return __builtin_amdgcn_readlane(mine, i + u); };
-        for (; i + 8 <= n; i += 8) vx_eg_add_n<GT, U, TINY, 8>(grad, at, D, c, sum);
-        if (n & 4) { vx_eg_add_n<GT, U, TINY, 4>(grad, at, D, c, sum); i += 4; }
-        if (n & 2) { vx_eg_add_n<GT, U, TINY, 2>(grad, at, D, c, sum); i += 2; }
-        if (n & 1) vx_eg_add_n<GT, U, TINY, 1>(grad, at, D, c, sum);
-    }
+    auto at = [&](int u) { return pos[a + u]; };
+    for (; b - a >= 4; a += 4) vx_eg_add_n<GT, U, TINY, 4>(grad, at, D, c, sum);
+    if ((b - a) & 2) { vx_eg_add_n<GT, U, TINY, 2>(grad, at, D, c, sum); a += 2; }
+    if ((b - a) & 1) vx_eg_add_n<GT, U, TINY, 1>(grad, at, D, c, sum);
 }
 
 // sum[] += rows a..b of fp32 partial sums.  Their rows are padded to VX_EG_SLICE columns (pitch), so no column sticks out: a
@@ -333,7 +326,7 @@ __device__ __forceinline__ void vx_eg_add_partials(const float *__restrict__ par
             }
 }
 
-// One wave per (chunk of 32 sorted tokens, slice of columns); chunks of several ids have no sum of their own.
+// One wave per (chunk of 16 sorted tokens, slice of columns); chunks of several ids have no sum of their own.
 template <int GT, int U, bool TINY>
 __global__ __launch_bounds__(256) void vx_k_eg_chunks(const unsigned *__restrict__ key, const int *__restrict__ pos, int chunks,
                                                       unsigned n_rows, const void *__restrict__ grad, int D, int slices,
@@ -347,7 +340,10 @@ __global__ __launch_bounds__(256) void vx_k_eg_chunks(const unsigned *__restrict
     const unsigned k0 = key[a];
     if (k0 >= n_rows || key[a + VX_EG_CHUNK - 1] != k0) return;
     float sum[U * VEC] = {};
-    vx_eg_add_tokens<GT, U, TINY, true>((const G *)grad, pos, a, a + VX_EG_CHUNK, D, c, sum);
+    const int mine = pos[a + (vx_lane() & (VX_EG_CHUNK - 1))];
+#pragma unroll
+    for (int i = 0; i < VX_EG_CHUNK; i += 4)
+        vx_eg_add_n<GT, U, TINY, 4>((const G *)grad, [&](int u) { return __builtin_amdgcn_readlane(mine, i + u); }, D, c, sum);
 #pragma unroll
     for (int q = 0; q < U; ++q)
 #pragma unroll
@@ -355,7 +351,7 @@ __global__ __launch_bounds__(256) void vx_k_eg_chunks(const unsigned *__restrict
             *(vx_f4 *)(part1 + c1 * pitch + c + q * 64 * VEC + k) = vx_f4{sum[q * VEC + k], sum[q * VEC + k + 1], sum[q * VEC + k + 2], sum[q * VEC + k + 3]};
 }
 
-// The same over 32 chunks; 256 columns for each wave.
+// The same over 16 chunks; 256 columns for each wave.
 __global__ __launch_bounds__(256) void vx_k_eg_chunks2(const unsigned *__restrict__ key, int chunks, unsigned n_rows, int slices,
                                                        long long pitch, const float *__restrict__ part1, float *__restrict__ part2) {
     const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -387,18 +383,18 @@ __device__ __forceinline__ int vx_eg_lower_bound(const unsigned *__restrict__ ke
 }
 
 // Table rows blockIdx + i * gridDim (i < 8): frequent ids lie next to each other, so neighbours go to different workgroups.
-// A wave sums one slice of one row; without chunks rows of more than 32 tokens follow, their tokens split
-// over the four waves and joined through LDS in wave order.
-template <int GT, int TT, int U, bool TINY, bool CHUNKED>
+// A wave sums one slice of one row.  levels: of chunks (0, 1, 2).  Bound by the write of the table: few registers, so that
+// many waves have their loads and stores on the way (a version that split long rows over the waves of a workgroup held 94
+// instead of 62 registers: 292 instead of 265 us for the rows of 65536 tokens x 4096 columns bf16 over 131072).
+template <int GT, int TT, int U, bool TINY>
 __global__ __launch_bounds__(256) void vx_k_eg_rows(const unsigned *__restrict__ key, const int *__restrict__ pos, int T,
                                                     const void *__restrict__ grad, long long n_rows, int D, int slices, float scale,
-                                                    void *__restrict__ out, int accumulate, int chunked2, long long pitch,
+                                                    void *__restrict__ out, int accumulate, int levels, long long pitch,
                                                     const float *__restrict__ part1, const float *__restrict__ part2) {
     typedef typename vx_elem<GT>::type G;
     typedef typename vx_elem<TT>::type E;
     constexpr int VEC = 16 / sizeof(G);
     __shared__ int s_at[2 * VX_EG_ROWS];
-    __shared__ float s_sum[CHUNKED ? 1 : 3][U * VEC][CHUNKED ? 1 : 64];
     const int lane = vx_lane(), w = threadIdx.x >> 6;
     {
         const int q = threadIdx.x >> 4;                           // 16 searches: the beginning and the end of 8 rows
@@ -443,48 +439,24 @@ __global__ __launch_bounds__(256) void vx_k_eg_rows(const unsigned *__restrict__
         const int i = item / slices, c = (item - i * slices) * VX_EG_SLICE + lane * VEC;
         const long long v = blockIdx.x + (long long)i * gridDim.x;
         const int s = __builtin_amdgcn_readfirstlane(s_at[2 * i]), e = __builtin_amdgcn_readfirstlane(s_at[2 * i + 1]);
-        if (v >= n_rows || (accumulate && s == e) || (!CHUNKED && e - s > VX_EG_CHUNK)) continue;
+        if (v >= n_rows || (accumulate && s == e)) continue;
         float sum[U * VEC] = {};
         const int a1 = (s + VX_EG_CHUNK - 1) / VX_EG_CHUNK, b1 = e / VX_EG_CHUNK;
-        if (a1 >= b1 || !CHUNKED) {
-            vx_eg_add_tokens<GT, U, TINY, !CHUNKED>((const G *)grad, pos, s, e, D, c, sum);
+        if (levels == 0 || a1 >= b1) {
+            vx_eg_add_tokens<GT, U, TINY>((const G *)grad, pos, s, e, D, c, sum);
         } else {
-            vx_eg_add_tokens<GT, U, TINY, !CHUNKED>((const G *)grad, pos, s, a1 * VX_EG_CHUNK, D, c, sum);
+            vx_eg_add_tokens<GT, U, TINY>((const G *)grad, pos, s, a1 * VX_EG_CHUNK, D, c, sum);
             const int a2 = (a1 + VX_EG_CHUNK - 1) / VX_EG_CHUNK, b2 = b1 / VX_EG_CHUNK;
-            if (a2 >= b2 || !chunked2) {
+            if (levels == 1 || a2 >= b2) {
                 vx_eg_add_partials<GT, U>(part1, a1, b1, pitch, c, sum);
             } else {
                 vx_eg_add_partials<GT, U>(part1, a1, (long long)a2 * VX_EG_CHUNK, pitch, c, sum);
                 vx_eg_add_partials<GT, U>(part2, a2, b2, pitch, c, sum);
                 vx_eg_add_partials<GT, U>(part1, (long long)b2 * VX_EG_CHUNK, b1, pitch, c, sum);
             }
-            vx_eg_add_tokens<GT, U, TINY, !CHUNKED>((const G *)grad, pos, b1 * VX_EG_CHUNK, e, D, c, sum);
+            vx_eg_add_tokens<GT, U, TINY>((const G *)grad, pos, b1 * VX_EG_CHUNK, e, D, c, sum);
         }
         if (c < D) finish(v, c, sum);
-    }
-    if (CHUNKED) return;
-    for (int i = 0; i < VX_EG_ROWS; ++i) {
-        const long long v = blockIdx.x + (long long)i * gridDim.x;
-        const int s = __builtin_amdgcn_readfirstlane(s_at[2 * i]), e = __builtin_amdgcn_readfirstlane(s_at[2 * i + 1]);
-        if (v >= n_rows || e - s <= VX_EG_CHUNK) continue;        // the same for the whole workgroup
-        const int per = (e - s + 3) / 4, a = min(e, s + w * per), b = min(e, a + per);
-        for (int sl = 0; sl < slices; ++sl) {
-            const int c = sl * VX_EG_SLICE + lane * VEC;
-            float sum[U * VEC] = {};
-            vx_eg_add_tokens<GT, U, TINY, !CHUNKED>((const G *)grad, pos, a, b, D, c, sum);
-            if (w)
-#pragma unroll
-                for (int k = 0; k < U * VEC; ++k) s_sum[w - 1][k][lane] = sum[k];
-            __syncthreads();
-            if (w == 0 && c < D) {
-#pragma unroll
-                for (int q = 0; q < 3; ++q)
-#pragma unroll
-                    for (int k = 0; k < U * VEC; ++k) sum[k] += s_sum[q][k][lane];
-                finish(v, c, sum);
-            }
-            __syncthreads();
-        }
     }
 }
 
@@ -505,13 +477,8 @@ static void vx_eg_sum(const vx_eg_plan &p, const unsigned *key, const int *pos, 
     if (p.chunks2)
         hipLaunchKernelGGL(vx_k_eg_chunks2, dim3((unsigned)(((int64_t)p.chunks2 * slices2 + 3) / 4)), dim3(256), 0, st, key, p.chunks2,
                            (unsigned)n_rows, slices2, p.pitch, part1, part2);
-    const dim3 grid((unsigned)((n_rows + VX_EG_ROWS - 1) / VX_EG_ROWS));
-    if (p.chunks)
-        hipLaunchKernelGGL((vx_k_eg_rows<GT, TT, U, TINY, true>), grid, dim3(256), 0, st, key, pos, T, grad, n_rows, D, slices, scale, out,
-                           accumulate, p.chunks2 > 0, p.pitch, part1, part2);
-    else
-        hipLaunchKernelGGL((vx_k_eg_rows<GT, TT, U, TINY, false>), grid, dim3(256), 0, st, key, pos, T, grad, n_rows, D, slices, scale, out,
-                           accumulate, 0, p.pitch, part1, part2);
+    hipLaunchKernelGGL((vx_k_eg_rows<GT, TT, U, TINY>), dim3((unsigned)((n_rows + VX_EG_ROWS - 1) / VX_EG_ROWS)), dim3(256), 0, st, key,
+                       pos, T, grad, n_rows, D, slices, scale, out, accumulate, p.chunks2 ? 2 : (p.chunks ? 1 : 0), p.pitch, part1, part2);
 }
 
 extern "C" int vx_embed_tokens_grad(const void *d_ids, int id_bytes, int64_t n_tokens, const void *d_grad_out,
