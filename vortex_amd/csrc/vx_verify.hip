@@ -7,16 +7,17 @@
 // T_b not above 0: greedy (x_j is accepted iff it is the first arg-max of its row; the token behind is the arg-max).
 //
 // Launches over chunks of the vocabulary:
-//   stats   every used row: largest logit and fp32 sum of exponentials of each chunk (bound by the one read of the logits;
+//   stats   every used row: largest logit and fp32 sum of exponentials of each quarter of a chunk (bound by the one read of the logits;
 //           fp64 exponentials here would take twice the time of the read)
 //   choose  the accepted drafts and the row to draw from; that row's (and the draft row's) chunk sums again in fp64
 //   rest    (with draft logits) that row's chunk sums of max(0, p - q), fp64
 //   draw    the token, one workgroup a sequence
 // The token that is drawn is a whole number, decided by where a cumulative sum passes a border, and one step of a flat
 // distribution is 1/V: everything it depends on is fp64.  The sums of the first launch are within 2^-17 of the true ones:
-//   an exponential is off by 2^-23 (the instruction) + ln2 |t| 3 * 2^-24 (difference, factor, product), t its exponent to
-//   base 2 below the largest; weighted with the distribution |t| averages at most log2 V <= 30 (it is the entropy less log2
-//   of the sum): 3.9e-6; at most 64 additions follow one another: 3.8e-6.
+//   a weight is the product of two exponentials (of its wave's largest logit against the row's, of its own against the
+//   wave's), each off by 2^-23 (the instruction) + ln2 |t| 3 * 2^-24 (difference, factor, product), t its exponent to base 2;
+//   weighted with the distribution the two |t| together average at most log2 V <= 30 (the entropy less log2 of the sum):
+//   4.0e-6 with the product's rounding; 38 fp32 additions follow one another at most (the rest are fp64): 2.3e-6.
 // So a test u q < p is taken from them unless its sides are within 2^-15 of each other; then both rows are summed in fp64.
 #include "vx_dtype.h"
 #include "vx_profile.h"
@@ -31,7 +32,7 @@ struct vx_verify_args {
     float one_temperature;
     int B, K, V, chunks;
     // workspace
-    float2 *stats;                                // [B][2 K + 1][chunks]: largest logit (NaN: an invalid one), sum (greedy: index)
+    float2 *stats;                                // [B][2 K + 1][4 chunks], for each wave: largest logit (NaN: an invalid one), sum (greedy: its index)
     double2 *z;                                   // [B][chunks]: sums of the row that is drawn from, target and draft
     double *r;                                    // [B][chunks]: sums of max(0, p - q)
     struct vx_choice *choice;                     // [B]
@@ -94,6 +95,9 @@ __device__ __forceinline__ double vx_weight(float x, float m, double c) {
 }
 __device__ __forceinline__ double vx_verify_c(float T) { return 1.44269504088896340736 / (double)T; }
 
+// the same in fp32; finite and not 0, so that the product with a masked logit is -inf at any temperature
+__device__ __forceinline__ float vx_verify_c32(float T) { return fminf(fmaxf((float)vx_verify_c(T), 1e-45f), 3e38f); }
+
 // the thread's values of a chunk, -inf where the row has ended: pieces of 16 bytes, 256 apart (the threads side by side) or
 // (IN_ORDER) next to each other
 template <int DT, bool IN_ORDER = false>
@@ -120,12 +124,11 @@ __device__ __forceinline__ void vx_verify_load(const typename vx_elem<DT>::type 
     }
 }
 
-// One workgroup per (sequence, row, chunk): target rows 0..K, then draft rows 0..K-1.
+// One workgroup per (sequence, row, chunk): target rows 0..K, then draft rows 0..K-1.  Each wave leaves its own statistics: no
+// barrier between a workgroup's loads and its end (185 MB in 29 us at 64 x 11 rows of 131072 bf16).
 template <int DT>
 __global__ __launch_bounds__(256) void vx_k_verify_stats(vx_verify_args a) {
     constexpr int VEC = 16 / sizeof(typename vx_elem<DT>::type), PER = VX_VERIFY_U * VEC;
-    __shared__ float s_m[4], s_z[4];
-    __shared__ int s_i[4];
     const int rows = a.draft ? 2 * a.K + 1 : a.K + 1;
     const int item = blockIdx.x / a.chunks, chunk = blockIdx.x - item * a.chunks;
     const int b = item / rows, j = item - b * rows, n = vx_verify_len(a, b);
@@ -155,40 +158,17 @@ __global__ __launch_bounds__(256) void vx_k_verify_stats(vx_verify_args a) {
 #pragma unroll
         for (int k = 32; k >= 1; k >>= 1) best = min(best, __shfl_xor(best, k, VX_WAVE));
     } else {
-        // A NaN or +inf makes the sum NaN by itself, and nothing else does: the subtrahend is finite, and so is the factor, which
-        // is not 0 either (a masked logit weighs 0 at an infinite temperature too).
-        const float c = fminf(fmaxf((float)vx_verify_c(T), 1e-45f), 3e38f), top = m == -INFINITY ? 0.f : m;
+        // A NaN or +inf makes the sum NaN by itself, and nothing else does: the subtrahend is finite.
+        const float c = vx_verify_c32(T), top = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int k = 0; k < PER; ++k) z += __builtin_amdgcn_exp2f((x[k] - top) * c);
 #pragma unroll
         for (int k = 32; k >= 1; k >>= 1) z += __shfl_xor(z, k, VX_WAVE);
         bad = z != z;
     }
-    if (vx_lane() == 0) {
-        const int w = threadIdx.x >> 6;
-        s_m[w] = bad ? __builtin_nanf("") : m;
-        s_z[w] = z;
-        s_i[w] = best;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        float M = s_m[0];
-        for (int w = 1; w < 4; ++w) M = M != M || s_m[w] != s_m[w] ? __builtin_nanf("") : fmaxf(M, s_m[w]);
-        float out;
-        if (greedy) {
-            int i = 0x7fffffff;
-            for (int w = 0; w < 4; ++w)
-                if (s_m[w] == M) i = min(i, s_i[w]);
-            out = __int_as_float(i);
-        } else {
-            const double c = vx_verify_c(T);
-            double Z = 0.0;
-            for (int w = 0; w < 4; ++w)
-                if (s_z[w] > 0.f) Z += (double)s_z[w] * vx_weight(s_m[w], M, c);
-            out = (float)Z;
-        }
-        a.stats[((long long)b * (2 * a.K + 1) + j) * a.chunks + chunk] = float2{M, out};
-    }
+    if (vx_lane() == 0)
+        a.stats[(((long long)b * (2 * a.K + 1) + j) * a.chunks + chunk) * 4 + (threadIdx.x >> 6)] =
+            float2{bad ? __builtin_nanf("") : m, greedy ? __int_as_float(best) : z};
 }
 
 // sum over the workgroup's 256 threads, in one order; every thread gets it
@@ -208,7 +188,7 @@ __device__ __forceinline__ double vx_verify_chunk_sum(const typename vx_elem<DT>
     float x[PER];
     vx_verify_load<DT>(row, chunk * vx_verify_chunk<DT>(), V, x);
     double z = 0.0;
-#pragma unroll 4
+#pragma unroll
     for (int k = 0; k < PER; ++k) z += vx_weight(x[k], m, c);
     return z;
 }
@@ -242,26 +222,34 @@ __global__ __launch_bounds__(256) void vx_k_verify_choose(vx_verify_args a) {
         const int i = i0 + (threadIdx.x >> 4), sub = lane & 15;
         const bool row = i < (has_q ? 2 * n + 1 : n + 1);
         const int j = i <= n ? i : K + 1 + (i - n - 1);           // row of the statistics
-        const float2 *st = a.stats + ((long long)b * (2 * K + 1) + j) * a.chunks;
+        const float2 *st = a.stats + ((long long)b * (2 * K + 1) + j) * a.chunks * 4;
         float m = -INFINITY;
         bool bad = false;
+        float2 v[4];                                              // the first 64 of the row's statistics
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = row && sub + 16 * k < a.chunks * 4 ? st[sub + 16 * k] : float2{-INFINITY, 0.f};
+        auto look = [&](float x) {
+            bad |= x != x;
+            m = fmaxf(m, x);
+        };
+#pragma unroll
+        for (int k = 0; k < 4; ++k) look(v[k].x);
         if (row)
-            for (int k = sub; k < a.chunks; k += 16) {
-                const float v = st[k].x;
-                bad |= v != v;
-                m = fmaxf(m, v);
-            }
+            for (int k = sub + 64; k < a.chunks * 4; k += 16) look(st[k].x);
 #pragma unroll
         for (int k = 8; k >= 1; k >>= 1) m = fmaxf(m, __shfl_xor(m, k, VX_WAVE));
         bad = (__ballot(bad) >> (lane & 48)) & 0xffff;
         double z = 0.0;
         int best = 0x7fffffff;
-        if (row && !bad && m != -INFINITY)
-            for (int k = sub; k < a.chunks; k += 16) {
-                const float2 v = st[k];
-                if (greedy) best = v.x == m ? min(best, __float_as_int(v.y)) : best;
-                else if (v.y > 0.f) z += (double)v.y * vx_weight(v.x, m, c);
-            }
+        const float c32 = vx_verify_c32(T), top = m == -INFINITY ? 0.f : m;
+        auto join = [&](float2 x) {
+            if (greedy) best = x.x == m ? min(best, __float_as_int(x.y)) : best;
+            else z += (double)(x.y * __builtin_amdgcn_exp2f((x.x - top) * c32));
+        };
+#pragma unroll
+        for (int k = 0; k < 4; ++k) join(v[k]);
+        if (row)
+            for (int k = sub + 64; k < a.chunks * 4; k += 16) join(st[k]);
 #pragma unroll
         for (int k = 8; k >= 1; k >>= 1) {
             z += __shfl_xor(z, k, VX_WAVE);
@@ -450,7 +438,7 @@ __global__ __launch_bounds__(256) void vx_k_verify_rest(vx_verify_args a) {
     const double2 z = vx_verify_totals(a, b, s_sum);
     const double ip = 1.0 / z.x, iq = 1.0 / z.y;
     double sum = 0.0;
-#pragma unroll 4
+#pragma unroll
     for (int k = 0; k < PER; ++k) sum += vx_verify_rest(x[k], y[k], ch, c, ip, iq);
     sum = vx_verify_sum(sum, s_sum);
     if (threadIdx.x == 0) a.r[(long long)b * a.chunks + chunk] = sum;
@@ -475,7 +463,7 @@ __global__ __launch_bounds__(256) void vx_k_verify_draw(vx_verify_args a) {
             float x[PER];
             vx_verify_load<DT, true>(trow, i - threadIdx.x * PER, a.V, x);
             double sum = 0.0;
-#pragma unroll 4
+#pragma unroll
             for (int k = 0; k < PER; ++k) sum += i + k == drop ? 0.0 : vx_weight(x[k], ch.mp, c);
             return sum;
         };
@@ -495,7 +483,7 @@ __global__ __launch_bounds__(256) void vx_k_verify_draw(vx_verify_args a) {
             vx_verify_load<DT, true>(trow, i - threadIdx.x * PER, a.V, x);
             vx_verify_load<DT, true>(drow, i - threadIdx.x * PER, a.V, y);
             double sum = 0.0;
-#pragma unroll 4
+#pragma unroll
             for (int k = 0; k < PER; ++k) sum += vx_verify_rest(x[k], y[k], ch, c, ip, iq);
             return sum;
         };
@@ -517,7 +505,7 @@ static vx_verify_plan vx_verify_make_plan(int B, int K, int V, int chunk) {
     p.chunks = (V + chunk - 1) / chunk;
     size_t at = 0;
     auto take = [&](size_t n) { const size_t o = at; at += (n + 255) & ~(size_t)255; return o; };
-    p.stats = take((size_t)B * (2 * K + 1) * p.chunks * sizeof(float2));
+    p.stats = take((size_t)B * (2 * K + 1) * p.chunks * 4 * sizeof(float2));
     p.z = take((size_t)B * p.chunks * sizeof(double2));
     p.r = take((size_t)B * p.chunks * sizeof(double));
     p.choice = take((size_t)B * sizeof(vx_choice));
