@@ -9,7 +9,7 @@ Tolerances (u = 2^-24, the rounding of one fp32 operation; e = half a step of th
                  rounding: (u + e) |result|
   verification   whole numbers equal.  accept is a quotient of two probabilities whose normalising sums are fp32: an exponential
                  of the sum is off by 2 u (the instruction) + 3 u ln2 |t| (difference, factor and product in its exponent t to base
-                 2), and |t| averages, weighted with the distribution, at most its entropy, log2 V; at most 64 additions follow one
+                 2), and |t| averages, weighted with the distribution, at most its entropy, log2 V; at most 64 operations follow one
                  another, 64 u.  At V = 2^17: (2 + 3 * 0.7 * 17 + 64) u < 102 u for each sum, 2^-16.3 for the quotient: 2^-15 |value|"""
 import numpy as np
 import pytest

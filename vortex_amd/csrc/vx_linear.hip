@@ -185,7 +185,9 @@ __global__ __launch_bounds__(1024) void vx_k_linear_stream(const int8_t *__restr
         b += N_;
     };
     while (b + UN <= end_full) run(std::integral_constant<int, UN>());
-    while (b < end_full) run(std::integral_constant<int, 1>());
+    if (UN > 4 && b + 4 <= end_full) run(std::integral_constant<int, 4>());
+    if (UN > 2 && b + 2 <= end_full) run(std::integral_constant<int, 2>());
+    if (b < end_full) run(std::integral_constant<int, 1>());
     if (b < end) {
         // The last 64 bytes stick out of the rows.  The tokens' bytes from K on are made 0, so the channels' may be anything
         // that lies inside the matrix: only its last rows are read byte by byte.
@@ -436,7 +438,8 @@ __global__ __launch_bounds__(256) void vx_k_pad_rows(const int8_t *__restrict__ 
 //   M <= 8: streaming (32000 x 4096: 30 against 33 by 64 x 64 tiles; at M = 16 36 against 33)
 //   M <= 64: streaming with few channels or an odd K, which the tiles would have to copy (8192 x 8192, M = 32: 27 against 30;
 //            50021 x 1000, M = 37: 23), 64 x 64 tiles from 16384 channels on (32000 x 4096, M = 32: 33 against 43)
-//   more: the largest tile that gives at least 192 workgroups, three for four compute units (8192 x 4096: M = 1536, 192 tiles
+//   more: the largest tile that is at least half full of tokens and gives at least 192 workgroups, three for four compute
+//   units (32000 x 4096, M = 64: 34 by 64 against 37 by 128; M = 96: 44 against 38.  8192 x 4096: M = 1536, 192 tiles
 //   of 256: 54 against 60 by 128; M = 1024, 128 tiles: 48 against 41.  8192 x 8192, M = 128, 64 tiles of 128: 43 against 33 by
 //   64; M = 512, 256 tiles: 47 against 58)
 #define VX_STREAM_MAX 64
@@ -483,8 +486,8 @@ static int vx_linear_launch(const int8_t *q, long long qs, bool q_padded, const 
     if (tiles) {
         auto count = [&](int t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
         VX_DISPATCH_DTYPE(out_dtype, {
-            if (count(256) >= 192) vx_linear_tiles<DT, 256, 2, 4>(q, qs, s, M, w, ws, sw, N, K, bias, out, os, st);
-            else if (count(128) >= 192) vx_linear_tiles<DT, 128, 2, 2>(q, qs, s, M, w, ws, sw, N, K, bias, out, os, st);
+            if (M > 128 && count(256) >= 192) vx_linear_tiles<DT, 256, 2, 4>(q, qs, s, M, w, ws, sw, N, K, bias, out, os, st);
+            else if (M > 64 && count(128) >= 192) vx_linear_tiles<DT, 128, 2, 2>(q, qs, s, M, w, ws, sw, N, K, bias, out, os, st);
             else vx_linear_tiles<DT, 64, 2, 2>(q, qs, s, M, w, ws, sw, N, K, bias, out, os, st);
         });
     } else {

@@ -13,12 +13,13 @@
 //   rest    (with draft logits) that row's chunk sums of max(0, p - q), fp64
 //   draw    the token, one workgroup a sequence
 // The token that is drawn is a whole number, decided by where a cumulative sum passes a border, and one step of a flat
-// distribution is 1/V: everything it depends on is fp64.  The sums of the first launch are within 2^-17 of the true ones:
+// distribution is 1/V: everything it depends on is fp64.  How far the sums of the first launch are off, u = 2^-24:
 //   a weight is the product of two exponentials (of its wave's largest logit against the row's, of its own against the
-//   wave's), each off by 2^-23 (the instruction) + ln2 |t| 3 * 2^-24 (difference, factor, product), t its exponent to base 2;
-//   weighted with the distribution the two |t| together average at most log2 V <= 30 (the entropy less log2 of the sum):
-//   4.0e-6 with the product's rounding; 38 fp32 additions follow one another at most (the rest are fp64): 2.3e-6.
-// So a test u q < p is taken from them unless its sides are within 2^-15 of each other; then both rows are summed in fp64.
+//   wave's), each off by 2 u (the instruction) + ln2 |t| 3 u (difference, factor, product), t its exponent to base 2;
+//   weighted with the distribution the two |t| together average at most log2 V (the entropy less log2 of the sum);
+//   the product 1 u, and 16 fp32 additions that follow one another (the rest are fp64):  (21 + 2.1 log2 V) u
+// So a test u q < p, with two such sums, is taken from them unless its sides are within (42 + 4.2 log2 V) u of each other
+// (6.8e-6 at V = 131072); then both rows are summed in fp64.
 #include "vx_dtype.h"
 #include "vx_profile.h"
 
@@ -160,8 +161,10 @@ __global__ __launch_bounds__(256) void vx_k_verify_stats(vx_verify_args a) {
     } else {
         // A NaN or +inf makes the sum NaN by itself, and nothing else does: the subtrahend is finite.
         const float c = vx_verify_c32(T), top = m == -INFINITY ? 0.f : m;
+        float part[4] = {};
 #pragma unroll
-        for (int k = 0; k < PER; ++k) z += __builtin_amdgcn_exp2f((x[k] - top) * c);
+        for (int k = 0; k < PER; ++k) part[k & 3] += __builtin_amdgcn_exp2f((x[k] - top) * c);
+        z = (part[0] + part[1]) + (part[2] + part[3]);
 #pragma unroll
         for (int k = 32; k >= 1; k >>= 1) z += __shfl_xor(z, k, VX_WAVE);
         bad = z != z;
@@ -280,7 +283,7 @@ __global__ __launch_bounds__(256) void vx_k_verify_choose(vx_verify_args a) {
                     const double q = has_q ? vx_weight(dx, s_m[VX_MAX_DRAFTS + 1 + lane], c) / s_z[VX_MAX_DRAFTS + 1 + lane] : 1.0;
                     uq = (double)un * q;
                     ok = uq < p;
-                    unsure = p > 0.0 && fabs(uq - p) <= p * (1.0 / 32768.0);
+                    unsure = p > 0.0 && fabs(uq - p) <= p * ((42.0 + 4.2 * (32 - __clz(a.V))) * 0x1p-24);
                     ratio = p >= q ? (p > 0.0 ? 1.0 : 0.0) : p / q;
                 }
             }
