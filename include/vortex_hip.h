@@ -365,7 +365,8 @@ int vx_quantize_rows_i8(const void *d_x, int dtype, int64_t M, int K, int64_t x_
                         float *d_scale, void *stream);
 
 /* d_out[m,n] = d_scale[m] * d_w_scale[n] * (sum_k d_q[m,k] d_w[n,k]) (+ d_bias[n]): the sum exact in 32-bit integers, the
- * rest fp32 (the two scales first), rounded once to out_dtype.  d_q [M,K] and d_w [N,K] hold any 8-bit integers.
+ * rest fp32 (the two scales first), rounded once to out_dtype.  d_q [M,K] and d_w [N,K] hold any 8-bit integers (only 131072
+ * products of -128 and -128, 2^31, would not fit).
  * d_bias f32[N] or NULL.  The workspace is 256-byte aligned; K <= VX_MAX_I8_DEPTH. */
 size_t vx_linear_i8_workspace_bytes(int64_t M, int64_t N, int K);
 int vx_linear_i8(const int8_t *d_q, int64_t q_stride, const float *d_scale, int64_t M, const int8_t *d_w, int64_t w_stride,
@@ -389,7 +390,8 @@ int vx_linear_w8a8(const void *d_x, int x_dtype, int64_t x_stride, int64_t M, co
  *   d_tokens[b,0..n) = x_0 .. x_{n-1}, d_tokens[b,n] = that token, -1 behind it; d_counts[b] = n + 1
  * T_b = d_temperature[b], or `temperature` for every sequence where d_temperature is NULL.  Not above 0: greedy -- x_j is accepted iff it is the first arg-max of target row j (d_accept 1 or 0), the
  * token behind is the arg-max of row n; the draft logits and d_uniforms are not used.  d_uniforms [B, K+1] in [0, 1).
- * -inf masks a token (in either distribution).  K = 0 draws one token from each row 0.
+ * -inf masks a token (in either distribution); other logits of a row differ by less than FLT_MAX.  K = 0 draws one token from
+ * each row 0.
  * The drawn token and every accepted / rejected are decided in fp64 from the logits on; d_accept is within 2^-15 relative.
  * d_status[b] (written, not ORed): VX_STATUS_NAN a NaN or +inf in a row that is used,
  * VX_STATUS_EMPTY_ROW all of such a row is -inf, VX_STATUS_BAD_TOKEN a drafted token outside [0, V) (it is rejected).  A

@@ -198,6 +198,40 @@ def test_embedding_module_trains():
     assert not m(ids).requires_grad
 
 
+def test_embedding_gradient_of_an_expanded_and_of_a_strided_grad():
+    m = V.TokenEmbedding(11, 40, scale=0.5, dtype=torch.bfloat16).to(DEV)
+    ids = torch.tensor([3, 3, 10, -1, 3], device=DEV)
+    m(ids).sum().backward()                                        # grad_out: one value, stride 0
+    ref, err = grad_ref(ids.cpu(), torch.ones(5, 40), 11, 0.5)
+    check_grad(m.weight.grad, ref, err)
+    c = torch.randn(40, 5, device=DEV).to(torch.bfloat16).t()
+    (g,) = torch.autograd.grad(m(ids), m.weight, c)
+    check_grad(g, *grad_ref(ids.cpu(), c.cpu(), 11, 0.5))
+
+
+def test_embedding_gradient_in_a_captured_graph():
+    """Forward and torch.autograd.grad captured together, replayed with other ids between eager steps."""
+    m = V.TokenEmbedding(300, 64).to(DEV)
+    ids, c = torch.zeros(90, dtype=torch.int64, device=DEV), torch.randn(90, 64, device=DEV)
+
+    def step():
+        return torch.autograd.grad((m(ids) * c).sum(), m.weight)[0]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for k in range(4):
+        ids.copy_(torch.randint(-1, 300, (90,), generator=gen(k)))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, ops.embed_tokens_grad(ids, c, 300)), "replay %d" % k
+
+
 # ------------------------------------------------------------------------------------------------ 8-bit product
 def quant_ref(x):
     x = x.double()
@@ -246,6 +280,16 @@ def test_quantize_special_rows():
     assert y[[2, 3, 4, 6]].isnan().all() and (y[1] == 2.0).all() and y[[0, 5]].isfinite().all()
 
 
+def test_quantize_subnormal_and_unaligned_rows():
+    for dt in TYPES:
+        tiny = torch.arange(1, 34, dtype=torch.float64) * (2.0 ** -133 if dt != torch.float16 else 2.0 ** -24)
+        base = torch.stack((tiny, -tiny.flip(0), tiny * 3)).to(dt)
+        for cut in (slice(None), slice(1, None), slice(None, None, 2), slice(5, 6)):      # also at odd addresses and strides
+            q, s = ops.quantize_rows_i8(base.to(DEV)[:, cut])
+            qr, sr = quant_ref(base[:, cut])
+            assert torch.equal(q.cpu(), qr) and torch.equal(s.cpu(), sr)
+
+
 def product_ref(q, s, qw, sw, bias, dt):
     """(result, allowed error) in 64 bits from the integers and the scales that the operator uses."""
     y0 = (q.double() @ qw.double().t()) * (s.double()[:, None] * sw.double()[None])
@@ -289,6 +333,34 @@ def test_linear_extreme_integers_are_exact(M):
     got = ops.linear_i8(q.to(DEV), torch.ones(M, device=DEV), qw.to(DEV), torch.ones(N, device=DEV)).cpu().double()
     ref = q.double() @ qw.double().t()
     assert bool(((got - ref).abs() <= U * ref.abs()).all())       # one conversion to fp32
+
+
+def test_linear_offsets_beyond_32_bits():
+    """More than 2^31 weights: the last channels are found by the streaming and by the tile kernel."""
+    N, K = 530000, 4096
+    qw = torch.zeros(N, K, dtype=torch.int8, device=DEV)
+    qw[-2:] = torch.tensor([[3], [-5]], dtype=torch.int8, device=DEV)
+    for M in (1, 130):
+        y = ops.linear_i8(torch.ones(M, K, dtype=torch.int8, device=DEV), torch.ones(M, device=DEV), qw, torch.ones(N, device=DEV), out_dtype=torch.bfloat16)
+        assert y[:, -2].tolist() == [3.0 * K] * M and y[:, -1].tolist() == [-5.0 * K] * M and not y[:, :-2].any()
+
+
+def test_linear_through_the_c_abi_with_unaligned_rows():
+    """What ops copies first, a C caller may pass: weights at an odd address and stride, M beyond the streaming kernel's sizes."""
+    lib, g = L.lib(), gen(6)
+    M, N, K = 150, 70, 64
+    q = torch.randint(-128, 128, (M, K), generator=g, dtype=torch.int8)
+    s, sw = torch.rand(M, generator=g), torch.rand(N, generator=g)
+    wide = torch.randint(-128, 128, (N, 75), generator=g, dtype=torch.int8)
+    out = torch.empty(M, N, device=DEV)
+    nb = lib.vx_linear_i8_workspace_bytes(M, N, K)
+    ws = torch.empty(nb, dtype=torch.uint8, device=DEV)
+    Q, S, W, SW = (t.to(DEV) for t in (q, s, wide, sw))
+    rc = lib.vx_linear_i8(Q.data_ptr(), K, S.data_ptr(), M, W.data_ptr() + 3, 75, SW.data_ptr(), N, K, None, out.data_ptr(), L.VX_DTYPE_F32, N,
+                          ws.data_ptr(), nb, L.stream_ptr(DEV))
+    assert rc == 0
+    ref, tol = product_ref(q, s, wide[:, 3:3 + K], sw, None, torch.float32)
+    assert bool(((out.cpu().double() - ref).abs() <= tol).all())
 
 
 def test_linear_strides_and_leading_shapes():
@@ -578,6 +650,29 @@ def test_verify_strided_logits():
                                                          "draft": draft.to(DEV).transpose(1, 2).contiguous().transpose(1, 2)})
     one = draft[:1].expand(4, 3, 515)
     check_verify(target, tokens, u, one.contiguous(), lens, temp, {"draft": draft[:1].to(DEV).expand(4, 3, 515)})
+
+
+def test_verify_offsets_beyond_32_bits():
+    """Rows more than 2^31 elements apart (a view of 4.4 GB)."""
+    target, tokens, u, draft, _, temp = verify_inputs(2, 1, 777, torch.bfloat16, 91, greedy=0.0)
+    far = torch.empty(2 ** 31 + 4 * 777, dtype=torch.bfloat16, device=DEV)
+    view = far.as_strided((2, 2, 777), (2 ** 31 + 777, 777, 1))
+    view.copy_(target)
+    check_verify(target, tokens, u, draft, None, temp, {"target": view})
+
+
+def test_verify_calls_at_once_on_two_streams():
+    target, tokens, u, draft, lens, temp = (t.to(DEV) for t in verify_inputs(6, 4, 30011, torch.float16, 92))
+    ref = ops.verify_drafts(target, tokens, u, draft, lens, temp)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for k in range(6):
+        with torch.cuda.stream(streams[k % 2]):
+            got.append(ops.verify_drafts(target, tokens, u, draft, lens, temp))
+    torch.cuda.synchronize()
+    for g in got:
+        assert all(torch.equal(a, b) for a, b in zip(g, ref))
 
 
 def test_verify_draws_follow_the_target():

@@ -463,7 +463,7 @@ def embed_tokens(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
     T = ids.numel()
     if T:
         rc = L.lib().vx_embed_tokens(ids.data_ptr(), ids.element_size(), T, table.data_ptr(), V, D, _row_stride(table),
-                                     _DTYPES[table.dtype], scale, out.data_ptr(), st, L.stream_ptr(dev))
+                                     _DTYPES[table.dtype], float(scale), out.data_ptr(), st, L.stream_ptr(dev))
         L.check(rc, "vx_embed_tokens")
     return out
 
@@ -498,7 +498,7 @@ def embed_tokens_grad(ids: torch.Tensor, grad_out: torch.Tensor, n_rows: int, sc
     nb = lib.vx_embed_tokens_grad_workspace_bytes(T, n_rows, D)
     ws = _ws(nb, dev)
     rc = lib.vx_embed_tokens_grad(ids.data_ptr(), ids.element_size(), T, grad_out.data_ptr(), _DTYPES[grad_out.dtype], n_rows, D,
-                                  scale, out.data_ptr(), _DTYPES[out.dtype], int(accumulate), st, ws.data_ptr(), nb,
+                                  float(scale), out.data_ptr(), _DTYPES[out.dtype], int(accumulate), st, ws.data_ptr(), nb,
                                   L.stream_ptr(dev))
     L.check(rc, "vx_embed_tokens_grad")
     return out
@@ -580,7 +580,7 @@ def linear_i8(q: torch.Tensor, scale: torch.Tensor, qw: torch.Tensor, w_scale: t
 def linear_w8a8(x: torch.Tensor, qw: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
                 out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """[..., K] (f32, f16, bf16) -> [..., N] of out_dtype (default: x's type): quantize_rows_i8 and linear_i8 in one
-    call, the same bits.  See vx_linear_w8a8."""
+    call, the same bits.  No autograd.  See vx_linear_w8a8."""
     _tensor(x, "input", None, _DTYPES)
     dev = x.device
     if out_dtype is None:
@@ -608,7 +608,8 @@ def verify_drafts(target_logits: torch.Tensor, draft_tokens: torch.Tensor, unifo
                   draft_logits: Optional[torch.Tensor] = None, draft_lens: Optional[torch.Tensor] = None,
                   temperature=1.0):
     """target_logits [B,K+1,V] (f32, f16, bf16), draft_tokens i64[B,K], uniforms f32[B,K+1], draft_logits [B,K,V] of the
-    same type or None (drafts without a distribution), draft_lens i32[B] or None, temperature a number or f32[B] (0: greedy)
+    same type or None (drafts without a distribution), draft_lens i32[B] or None, temperature a number (a 0-dim tensor is read
+    back) or f32[B], 0: greedy
     -> (tokens i64[B,K+1], counts i32[B], accept f32[B,K], status i32[B]); see vx_verify_drafts."""
     _tensor(target_logits, "target_logits", None, _DTYPES, 3)
     dev = target_logits.device

@@ -78,7 +78,10 @@ class _EmbedTokens(torch.autograd.Function):
 class TokenEmbedding(nn.Module):
     """The pre-process of a token model: integer ids -> the network's input vectors, scale * weight[ids] (what Normalize
     is for images).  An id below 0 is padding: a row of zeros that gets no gradient.  The gradient of `weight` is summed in
-    fp32 over the tokens in a fixed order (vx_embed_tokens_grad), dense, in the type of `weight`."""
+    fp32 over the tokens in a fixed order (vx_embed_tokens_grad), dense, in the type of `weight`.
+
+    In a captured HIP graph, take the gradient with torch.autograd.grad: a captured backward() accumulates into `weight.grad`
+    on the stream of whatever eager graph of `weight` is still alive, which torch answers by ending the process."""
 
     def __init__(self, n_rows: int, dim: int, scale: float = 1.0, dtype=None, device=None):
         super(TokenEmbedding, self).__init__()
