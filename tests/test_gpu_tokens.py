@@ -38,7 +38,7 @@ def zipf(n, V_, g):
 
 # ------------------------------------------------------------------------------------------------ embedding
 @pytest.mark.parametrize("dt", TYPES)
-@pytest.mark.parametrize("T,Vr,D", [(1, 1, 1), (1, 7, 8), (3, 50, 7), (64, 1000, 64), (65, 1000, 1027), (500, 333, 1000), (33, 5000, 4096), (7, 11, 8200)])
+@pytest.mark.parametrize("T,Vr,D", [(1, 1, 1), (1, 7, 8), (3, 50, 7), (64, 1000, 64), (65, 1000, 1027), (500, 333, 1000), (33, 5000, 4096), (7, 11, 8200), (9000, 70, 2048), (9001, 70, 2056)])
 def test_embed_rows(dt, T, Vr, D):
     g = gen(T * 31 + D)
     table = torch.randn(Vr, D, generator=g).to(dt)
@@ -117,7 +117,7 @@ def check_grad(got, ref, err):
 @pytest.mark.parametrize("T,Vr,D", [(1, 1, 1), (2, 5, 8), (63, 40, 7), (64, 1000, 64), (1000, 3, 65), (1025, 5000, 100), (4097, 700, 1000),
                                     (5000, 50021, 33), (20000, 300, 16), (3000, 1, 40), (9000, 70001, 24), (64, 3, 520), (65, 3, 520), (255, 1, 24), (2049, 200, 520), (8192, 5, 8), (8191, 511, 8), (16384, 512, 8),
                                     (16385, 512, 8), (20001, 511, 9),
-                                    (70000, 2, 12), (200000, 600000, 4)])
+                                    (70000, 2, 12), (200000, 600000, 4), (300, 20000, 1024), (301, 20001, 1028)])
 def test_embed_grad(dt, T, Vr, D):
     g = gen(T + Vr)
     ids = zipf(T, Vr, g)

@@ -10,7 +10,7 @@ __device__ __forceinline__ long long vx_id_at(const void *ids, int id_bytes, lon
 
 // ------------------------------------------------------------------------------------------------ lookup
 // One wave per slice of one token's row, U 16-byte pieces for each lane, all loads issued before the first store.
-template <int DT, int U, bool TINY>
+template <int DT, int U, bool TINY, bool NT>
 __global__ __launch_bounds__(256) void vx_k_embed(const void *__restrict__ ids, int id_bytes, long long T,
                                                   const void *__restrict__ table, long long n_rows, int D, int slices,
                                                   long long stride, float scale, void *__restrict__ out,
@@ -35,7 +35,7 @@ __global__ __launch_bounds__(256) void vx_k_embed(const void *__restrict__ ids, 
         float f[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; ++k) f[k] = ok ? (float)v[u].e[k] * scale : 0.f;
-        vx_cols<DT>(c0 + u * 64 * VEC, D).store(dst, f, D);
+        vx_cols<DT>(c0 + u * 64 * VEC, D).template store<NT>(dst, f, D);
     }
 }
 
@@ -56,17 +56,16 @@ extern "C" int vx_embed_tokens(const void *d_ids, int id_bytes, int64_t n_tokens
     const int64_t blocks = (n_tokens * slices + 3) / 4;
     if (blocks > 2147483647LL) return VX_ERR_UNSUPPORTED;
     vx_prof_begin(VX_PROF_EMBED, st);
+#define VX_EMBED_GO(...)                                                                                                       \
+    hipLaunchKernelGGL((vx_k_embed<__VA_ARGS__>), dim3((unsigned)blocks), dim3(256), 0, st, d_ids, id_bytes, (long long)n_tokens, d_table, \
+                       (long long)n_rows, D, slices, (long long)table_stride, scale, d_out, d_status)
     VX_DISPATCH_DTYPE(dtype, {
-        if (D < vec)
-            hipLaunchKernelGGL((vx_k_embed<DT, 1, true>), dim3((unsigned)blocks), dim3(256), 0, st, d_ids, id_bytes, (long long)n_tokens,
-                               d_table, (long long)n_rows, D, slices, (long long)table_stride, scale, d_out, d_status);
-        else if (wide)
-            hipLaunchKernelGGL((vx_k_embed<DT, 4, false>), dim3((unsigned)blocks), dim3(256), 0, st, d_ids, id_bytes, (long long)n_tokens,
-                               d_table, (long long)n_rows, D, slices, (long long)table_stride, scale, d_out, d_status);
-        else
-            hipLaunchKernelGGL((vx_k_embed<DT, 1, false>), dim3((unsigned)blocks), dim3(256), 0, st, d_ids, id_bytes, (long long)n_tokens,
-                               d_table, (long long)n_rows, D, slices, (long long)table_stride, scale, d_out, d_status);
+        if (D < vec) VX_EMBED_GO(DT, 1, true, false);
+        else if (vx_past_caches(d_out, n_tokens, D, dtype)) VX_EMBED_GO(DT, 4, false, true);
+        else if (wide) VX_EMBED_GO(DT, 4, false, false);
+        else VX_EMBED_GO(DT, 1, false, false);
     });
+#undef VX_EMBED_GO
     vx_prof_end(VX_PROF_EMBED, st);
     return hipGetLastError() == hipSuccess ? VX_OK : VX_ERR_LAUNCH;
 }
@@ -386,7 +385,7 @@ __device__ __forceinline__ int vx_eg_lower_bound(const unsigned *__restrict__ ke
 // A wave sums one slice of one row.  levels: of chunks (0, 1, 2).  Bound by the write of the table: few registers, so that
 // many waves have their loads and stores on the way (a version that split long rows over the waves of a workgroup held 94
 // instead of 62 registers: 292 instead of 265 us for the rows of 65536 tokens x 4096 columns bf16 over 131072).
-template <int GT, int TT, int U, bool TINY>
+template <int GT, int TT, int U, bool TINY, bool NT>
 __global__ __launch_bounds__(256) void vx_k_eg_rows(const unsigned *__restrict__ key, const int *__restrict__ pos, int T,
                                                     const void *__restrict__ grad, long long n_rows, int D, int slices, float scale,
                                                     void *__restrict__ out, int accumulate, int levels, long long pitch,
@@ -431,7 +430,7 @@ __global__ __launch_bounds__(256) void vx_k_eg_rows(const unsigned *__restrict__
 #pragma unroll
                     for (int j = 0; j < W; ++j) f[j] = (float)old.e[j] + f[j];
                 }
-                part.store(dst, f, D);
+                part.template store<NT>(dst, f, D);
             }
         }
     };
@@ -477,8 +476,14 @@ static void vx_eg_sum(const vx_eg_plan &p, const unsigned *key, const int *pos, 
     if (p.chunks2)
         hipLaunchKernelGGL(vx_k_eg_chunks2, dim3((unsigned)(((int64_t)p.chunks2 * slices2 + 3) / 4)), dim3(256), 0, st, key, p.chunks2,
                            (unsigned)n_rows, slices2, p.pitch, part1, part2);
-    hipLaunchKernelGGL((vx_k_eg_rows<GT, TT, U, TINY>), dim3((unsigned)((n_rows + VX_EG_ROWS - 1) / VX_EG_ROWS)), dim3(256), 0, st, key,
-                       pos, T, grad, n_rows, D, slices, scale, out, accumulate, p.chunks2 ? 2 : (p.chunks ? 1 : 0), p.pitch, part1, part2);
+    const dim3 grid((unsigned)((n_rows + VX_EG_ROWS - 1) / VX_EG_ROWS));
+    const int levels = p.chunks2 ? 2 : (p.chunks ? 1 : 0);
+    if (!TINY && !accumulate && vx_past_caches(out, n_rows, D, TT))
+        hipLaunchKernelGGL((vx_k_eg_rows<GT, TT, U, TINY, !TINY>), grid, dim3(256), 0, st, key, pos, T, grad, n_rows, D, slices, scale, out,
+                           accumulate, levels, p.pitch, part1, part2);
+    else
+        hipLaunchKernelGGL((vx_k_eg_rows<GT, TT, U, TINY, false>), grid, dim3(256), 0, st, key, pos, T, grad, n_rows, D, slices, scale, out,
+                           accumulate, levels, p.pitch, part1, part2);
 }
 
 extern "C" int vx_embed_tokens_grad(const void *d_ids, int id_bytes, int64_t n_tokens, const void *d_grad_out,
