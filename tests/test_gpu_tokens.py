@@ -261,6 +261,24 @@ def test_quantize_ties_go_to_even_in_every_type():
             assert torch.equal(q.cpu()[0, :-1].float(), k.round())
 
 
+def test_quantize_many_ties_and_short_mantissas():
+    """Rows of 16-bit types whose largest value has few bits: many quotients are ties, others as near to one as the type allows;
+    also at both ends of the range."""
+    g = gen(77)
+    for dt, bits in ((torch.bfloat16, 8), (torch.float16, 11), (torch.float32, 11)):
+        for e in (0, -8, 8) if dt == torch.float16 else (0, -125, -140, 110, -30):
+            rows = []
+            for _ in range(48):
+                ma = int(torch.randint(1, 256, (), generator=g))
+                near = ((torch.randint(0, 127, (256,), generator=g).double() * 2 + 1) * ma / 254).to(dt).double()       # the values next to ties
+                rows.append(torch.cat((near.clamp(max=ma), torch.tensor([float(ma)], dtype=torch.float64), torch.randint(-ma, ma + 1, (256,), generator=g).double())))
+            x = (torch.stack(rows) * 2.0 ** e).to(dt)
+            assert bool(x.isfinite().all())
+            q, s = ops.quantize_rows_i8(x.to(DEV))
+            qr, sr = quant_ref(x)
+            assert torch.equal(q.cpu(), qr) and torch.equal(s.cpu(), sr), (dt, e)
+
+
 def test_quantize_special_rows():
     x = torch.randn(8, 33)
     x[1] = 0
@@ -333,6 +351,53 @@ def test_linear_extreme_integers_are_exact(M):
     got = ops.linear_i8(q.to(DEV), torch.ones(M, device=DEV), qw.to(DEV), torch.ones(N, device=DEV)).cpu().double()
     ref = q.double() @ qw.double().t()
     assert bool(((got - ref).abs() <= U * ref.abs()).all())       # one conversion to fp32
+
+
+@pytest.mark.parametrize("M,N,K", [(65, 255, 16), (66, 256, 240), (80, 1, 256), (97, 17, 272), (4097, 100, 512), (1000, 33, 528), (8200, 255, 1008),
+                                   (12289, 256, 1024), (16385, 255, 256), (300, 256, 1024), (65, 257, 1024), (65, 256, 1040), (70, 200, 1000)])
+def test_linear_of_few_channels(M, N, K):
+    """Up to 256 channels the weights stay on the chip and x passes by: one to many tiles of tokens for each workgroup, every type,
+    and the sizes behind the last that go this way."""
+    g = gen(M + N + K)
+    qw = torch.randint(-128, 128, (N, K), generator=g, dtype=torch.int8)
+    sw, bias = torch.rand(N, generator=g) * 0.01, torch.randn(N, generator=g)
+    for xt in TYPES:
+        x = (torch.randn(M, K, generator=g) * torch.exp(3 * torch.randn(M, 1, generator=g))).to(xt)
+        x[3] = 0
+        x[M - 1, K - 1] = float("nan")
+        q, s = quant_ref(x)
+        for ot, b in zip(TYPES, (bias, None, bias)):
+            d = [t.to(DEV) if t is not None else None for t in (x, qw, sw, b)]
+            got = ops.linear_w8a8(*d, out_dtype=ot)
+            ref, tol = product_ref(q, s, qw, sw, b, ot)
+            y = got.cpu().double()
+            ok = (y - ref).abs() <= tol
+            if ot == torch.float16:                               # from 65520 on, half a step above the largest, fp16 rounds to infinity
+                ok |= (ref.abs() + tol >= 65520) & (y == torch.sign(ref) * float("inf"))
+            finite = x.isfinite().all(1)                          # a few rows of fp16 hold an infinity themselves
+            assert bool(ok[finite].all()) and bool(y[~finite].isnan().all()) and not bool(finite[-1])
+            two = ops.linear_i8(*ops.quantize_rows_i8(d[0]), d[1], d[2], d[3], out_dtype=ot)
+            assert torch.equal(got[finite.to(DEV)], two[finite.to(DEV)])
+
+
+def test_linear_of_few_channels_writes_its_rows_only():
+    """Strides of every operand, none a multiple of 16 bytes, through the C ABI: the columns and rows around the result stay."""
+    lib, g = L.lib(), gen(19)
+    M, N, K = 1003, 77, 144
+    x, w = torch.randn(M, 151, generator=g), torch.randint(-128, 128, (N, 150), generator=g, dtype=torch.int8)
+    sw = torch.rand(N, generator=g)
+    for ot, code in ((torch.float32, L.VX_DTYPE_F32), (torch.bfloat16, L.VX_DTYPE_BF16)):
+        out = torch.full((M + 2, 83), 7.0, dtype=ot, device=DEV)
+        nb = lib.vx_linear_w8a8_workspace_bytes(M, N, K)
+        ws, X, W, SW = torch.empty(nb, dtype=torch.uint8, device=DEV), x.to(DEV), w.to(DEV), sw.to(DEV)
+        rc = lib.vx_linear_w8a8(X.data_ptr() + 4, L.VX_DTYPE_F32, 151, M, W.data_ptr() + 3, 150, SW.data_ptr(), N, K, None,
+                                out.data_ptr() + 83 * out.element_size(), code, 83, ws.data_ptr(), nb, L.stream_ptr(DEV))
+        assert rc == 0
+        q, s = quant_ref(x[:, 1:1 + K])
+        ref, tol = product_ref(q, s, w[:, 3:3 + K], sw, None, ot)
+        got = out.cpu().double()
+        assert bool(((got[1:-1, :N] - ref).abs() <= tol).all())
+        assert bool((got[0] == 7).all()) and bool((got[-1] == 7).all()) and bool((got[:, N:] == 7).all())
 
 
 def test_linear_offsets_beyond_32_bits():

@@ -5,22 +5,92 @@
 #include "vx_profile.h"
 #include <type_traits>
 
-// rint(127 x / amax), exactly (ties to even), for x and amax of the input type, by division:
-//  16-bit types: 127 x is exact in fp32 (11 + 7 bits) and the quotient of an (11+7)-bit by an 11-bit number, at most 127,
-//  is either a tie itself or further than 2^-12 from one: the rounded fp32 quotient falls on the same side.
-//  fp32: the same argument holds for fp64 (24 + 7 bits over 24 bits: at least 2^-25 from a tie, rounding 2^-47).
+// rint(127 x / top), exactly, ties to even: with n = floor of the quotient (one below or above it by rounding does no harm) it is
+// n or n + 1 by 127 |x| against (n + 1/2) top.  Each product is taken as its rounded value and what the rounding left (a fma);
+// where the two are close, their difference and that of the rests are exact.  Rows near the ends of the range are scaled first.
+__device__ __forceinline__ unsigned vx_quant_exact(float x, float top) {
+    const float up = top < 1e-30f ? 0x1p64f : (top > 1e30f ? 0x1p-64f : 1.f), xs = fabsf(x) * up, ts = top * up;
+    const float n = floorf(xs * (127.0f / ts)), a = xs * 127.0f, b = (n + 0.5f) * ts;
+    const float d = (a - b) + (__builtin_fmaf(xs, 127.0f, -a) - __builtin_fmaf(n + 0.5f, ts, -b));
+    const int i = (int)n, v = i + (d > 0.f || (d == 0.f && (i & 1)) ? 1 : 0);
+    return (unsigned)(x < 0.f ? -v : v);
+}
+
+// What a row's largest |x| says: q = rint(x r), s = scale.  |x| is compared by its bits: they order as the values do, with
+// infinity and NaN above all.  A row that holds one gets the scale NaN (and q = 0): its products are all NaN.
+struct vx_quant_row {
+    float top, r;                                                 // 127 / top
+    bool bad, zero, tiny;
+    __device__ __forceinline__ explicit vx_quant_row(unsigned bits) {
+        bad = bits >= 0x7f800000u;
+        zero = bad || bits == 0;
+        top = __uint_as_float(bits);
+        r = zero ? 0.f : 127.0f / top;
+        tiny = !zero && !(r <= 3.4028234663852886e38f);
+    }
+    __device__ __forceinline__ float scale() const { return bad ? __builtin_nanf("") : top / 127.0f; }
+};
 template <int DT>
-__device__ __forceinline__ float vx_quant_exact(float x, float amax) {
-    if (DT == VX_DTYPE_F32) return (float)rint(((double)x * 127.0) / (double)amax);
-    return rintf((x * 127.0f) / amax);
+__device__ __forceinline__ unsigned vx_quant_look(const vx_vec<DT> &a, unsigned top) {
+#pragma unroll
+    for (int k = 0; k < 16 / (int)sizeof(typename vx_elem<DT>::type); ++k) top = max(top, __float_as_uint((float)a.e[k]) & 0x7fffffffu);
+    return top;
+}
+// largest value of the wave, in a scalar register: by rows of 16 lanes (1, 2, 4, 8 lanes up), then row to row and half to half
+__device__ __forceinline__ unsigned vx_wave_max(unsigned v) {
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false));
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false));
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false));
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false));
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));
+    return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
+}
+template <int DT>
+struct vx_quant_out {
+    unsigned w[4 / sizeof(typename vx_elem<DT>::type)];           // four integers each
+};
+// The quotient is a product with r; added to 1.5 * 2^23 it is rounded to an integer, in the sum's low byte.
+//  fp32: r is off by at most half a step, the product (in the fma) by 127 * 2^-24 < 7.6e-6; where that could change the integer
+//  (closer than 1e-5 to a tie) the exact way is taken.
+//  16-bit types: ties are frequent (rows whose largest value has a short mantissa), but other quotients are at least 2^-19 of
+//  their size away from one: |254 x - odd top| is a whole number over 254 |x| < 2^19, in units of x's last bit.  The product is
+//  within two steps of fp32 of the quotient; rounded to a multiple of 8 of them (2^-20) it is the tie if there is one, and
+//  otherwise stays on its side.
+// r overflows for a largest value below 127 / FLT_MAX: such rows go the exact way throughout.
+template <int DT>
+__device__ __forceinline__ vx_quant_out<DT> vx_quant_piece(const vx_vec<DT> &a, const vx_quant_row &row) {
+    constexpr int VEC = 16 / sizeof(typename vx_elem<DT>::type);
+    constexpr float SHIFT = 12582912.f;
+    vx_quant_out<DT> o;
+    unsigned t[VEC];
+    bool exact = row.tiny;
+    if (DT == VX_DTYPE_F32) {
+        float off = 0.f;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+            const float x = (float)a.e[k], sum = __builtin_fmaf(x, row.r, SHIFT);
+            off = fmaxf(off, fabsf(__builtin_fmaf(x, row.r, SHIFT - sum)));
+            t[k] = __float_as_uint(sum);
+        }
+        exact |= off > 0.49999f;
+    } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+            t[k] = __float_as_uint(__uint_as_float((__float_as_uint((float)a.e[k] * row.r) + 4u) & ~7u) + SHIFT);
+    }
+    if (exact) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) t[k] = vx_quant_exact((float)a.e[k], row.top);
+    }
+#pragma unroll
+    for (int k = 0; k < VEC / 4; ++k)
+        o.w[k] = row.zero ? 0u : __builtin_amdgcn_perm(t[4 * k + 1], t[4 * k], 0x0c0c0400u) | __builtin_amdgcn_perm(t[4 * k + 3], t[4 * k + 2], 0x04000c0cu);
+    return o;
 }
 
 // WAVES waves per row, U 16-byte pieces of it in the registers of each lane between the two passes (maximum, quotients);
-// longer rows are read again.  The quotient is a product with r = 127 / amax, off by at most 3 roundings of a value up to
-// 127 (127 * 3 * 2^-24 < 2.3e-5); where that could change the integer (closer than 1e-4 to a tie) it is divided: 46 -> 24 us
-// for 8192 x 4096 bf16.  r overflows for amax below 127 / FLT_MAX: such rows are divided throughout.
-// |x| is compared by its bits: they order as the values do, with infinity and NaN above all.  A row that holds one gets the
-// scale NaN (and q = 0): its products are all NaN.
+// longer rows are read again.
 template <int DT, int WAVES, int U>
 __global__ __launch_bounds__(256) void vx_k_quant_rows(const void *__restrict__ x, long long M, int K, long long xs,
                                                        int8_t *__restrict__ q, long long qs, float *__restrict__ scale) {
@@ -34,10 +104,7 @@ __global__ __launch_bounds__(256) void vx_k_quant_rows(const void *__restrict__ 
     unsigned top = 0;
     vx_vec<DT> v[U];
     const bool once = K <= THREADS * VEC * U;
-    auto look = [&](const vx_vec<DT> &a) {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) top = max(top, __float_as_uint((float)a.e[k]) & 0x7fffffffu);
-    };
+    auto look = [&](const vx_vec<DT> &a) { top = vx_quant_look<DT>(a, top); };
     if (once) {
 #pragma unroll
         for (int u = 0; u < U; ++u) v[u] = vx_load_vec<DT>(row + (u * THREADS + tid) * VEC, K - (u * THREADS + tid) * VEC);
@@ -46,33 +113,16 @@ __global__ __launch_bounds__(256) void vx_k_quant_rows(const void *__restrict__ 
     } else {
         for (int c = tid * VEC; c < K; c += THREADS * VEC) look(vx_load_vec<DT>(row + c, K - c));
     }
-#pragma unroll
-    for (int i = 32; i >= 1; i >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, i, VX_WAVE));
+    top = vx_wave_max(top);
     if (WAVES > 1) {
         if (vx_lane() == 0) s_max[w] = top;
         __syncthreads();
         top = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
     }
-    const bool bad = top >= 0x7f800000u, zero = bad || top == 0;
-    const float mx = __uint_as_float(top), r = zero ? 0.f : 127.0f / mx;
-    const bool divide = !zero && !(r <= 3.4028234663852886e38f);
+    const vx_quant_row what(top);
     int8_t *dst = q + m * qs;
     auto put = [&](const vx_vec<DT> &a, int c) {
-        union { int8_t b[VEC]; unsigned w[VEC / 4]; } o;
-        float t[VEC];
-        bool near = divide;
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-            const float y = zero ? 0.f : (float)a.e[k] * r;
-            t[k] = rintf(y);
-            near |= fabsf(y - t[k]) > 0.4999f;
-        }
-        if (near) {
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) t[k] = vx_quant_exact<DT>((float)a.e[k], mx);
-        }
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) o.b[k] = (int8_t)(int)t[k];
+        const vx_quant_out<DT> o = vx_quant_piece<DT>(a, what);
         if (c + VEC <= qs) {                                      // columns K .. qs - 1 come out as 0
             typedef unsigned u32_at1 __attribute__((aligned(1)));
 #pragma unroll
@@ -80,7 +130,7 @@ __global__ __launch_bounds__(256) void vx_k_quant_rows(const void *__restrict__ 
         } else {
 #pragma unroll
             for (int k = 0; k < VEC; ++k)
-                if (c + k < qs) dst[c + k] = o.b[k];
+                if (c + k < qs) dst[c + k] = (int8_t)(o.w[k / 4] >> (k % 4 * 8));
         }
     };
     if (once) {
@@ -89,7 +139,7 @@ __global__ __launch_bounds__(256) void vx_k_quant_rows(const void *__restrict__ 
     }
     for (long long c = (once ? THREADS * VEC * U : 0) + tid * VEC; c < qs; c += THREADS * VEC)
         put(vx_load_vec<DT>(row + c, K - (int)c), (int)c);
-    if (tid == 0) scale[m] = bad ? __builtin_nanf("") : mx / 127.0f;
+    if (tid == 0) scale[m] = what.scale();
 }
 
 static int vx_quant_launch(const void *x, int dtype, long long M, int K, long long xs, int8_t *q, long long qs, float *s, hipStream_t st) {
@@ -422,6 +472,154 @@ __global__ __launch_bounds__(WM * WN * 64) void vx_k_linear_tile(const int8_t *_
     }
 }
 
+// ---- many tokens, few channels: the weights stay in registers and x passes by once; no quantised copy of it in memory.
+// A persistent workgroup of 16 waves, each with 16 channels x KC bytes of weights (16x16x64 as in the streaming kernel).  For each
+// tile of 16 tokens a wave quantises one row into LDS from registers that were filled two tiles ahead, multiplies the tile with
+// its channels, and stores one row of the results of the tile before: one barrier a tile, all LDS double.  Rows in LDS are an
+// odd number of 16-byte pieces long: 16 of them lie in all banks.  With KC = 1024 a third of the weights is in LDS instead: 128
+// registers are all that 16 waves have.
+// Bound by the read of x: 43264 x 255 x 1024 (1x1 convolution in front of a YOLO layer) fp32 in 54 us, 221 MB at 4.1 TB/s;
+// quantised to memory and multiplied by tiles 71.  A workgroup for each 64 / 32 / 16 tokens that read the weights from L2 took
+// 70 / 92 / 122.
+// Needs K a multiple of 16 (the pieces of weights beyond K lie inside the row before) and up to 256 channels.
+#define VX_ROWS_MAX_N 256
+template <int OT>
+__device__ __forceinline__ void vx_linear_put_row(const float *y, void *out, long long at, int N) {
+    typedef typename vx_elem<OT>::type O;
+    constexpr int OV = 16 / sizeof(O);
+    const int c = vx_lane() * OV;
+    if (c >= N) return;
+    vx_vec<OT> o;
+#pragma unroll
+    for (int k = 0; k < OV; k += 4) {
+        const vx_v4 v = *(const vx_v4 *)(y + c + k);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o.e[k + j] = vx_store_cast<OT>(v[j]);
+    }
+    O *to = (O *)((char *)out + at * (long long)sizeof(O) + vx_lane() * 16u);
+    if (c + OV <= N) {
+        if (sizeof(O) == 2) *(vx_v4_at2 *)to = o.raw;
+        else *(vx_v4_at4 *)to = o.raw;
+    } else {
+#pragma unroll
+        for (int k = 0; k < OV; ++k)
+            if (c + k < N) to[k] = o.e[k];
+    }
+}
+
+template <int DT, int KC>
+__global__ __launch_bounds__(1024) void vx_k_linear_rows(const void *__restrict__ x, long long xs, long long M,
+                                                         const int8_t *__restrict__ w, long long ws, const float *__restrict__ sw,
+                                                         int N, int K, const float *__restrict__ bias, void *__restrict__ out,
+                                                         int out_dtype, long long os) {
+    typedef typename vx_elem<DT>::type E;
+    constexpr int VEC = 16 / sizeof(E), U = KC > 64 * VEC ? KC / (64 * VEC) : 1, B = KC / 64, PITCH = KC + 16, YP = VX_ROWS_MAX_N + 4;
+    constexpr int BL = KC > 512 ? 5 : 0, BR = B - BL;         // 64-byte blocks of weights in LDS and in registers
+    __shared__ __attribute__((aligned(16))) int8_t s_w[BL ? BL * 16384 : 16];
+    __shared__ __attribute__((aligned(16))) int8_t s_q[2][16 * PITCH];
+    __shared__ __attribute__((aligned(16))) float s_y[2][16 * YP], s_sw[VX_ROWS_MAX_N], s_bias[VX_ROWS_MAX_N];
+    __shared__ float s_scale[2][16];
+    const int lane = vx_lane(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long long tiles = (M + 15) >> 4;
+    auto fetch = [&](vx_vec<DT> (&v)[U], long long tile) {       // without a branch: the loads in flight stay countable
+        const char *row = (const char *)((const E *)x + min(tile * 16 + wave, M - 1) * xs);
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u].raw = vx_load16<DT>((const E *)(row + min((u * 64 + lane) * 16u, (unsigned)(K * sizeof(E) - 16))));
+    };
+    vx_vec<DT> va[U], vb[U];
+    fetch(va, blockIdx.x);
+    fetch(vb, (long long)blockIdx.x + gridDim.x);
+    const int n = wave * 16 + (lane & 15), koff = (lane >> 4) * 16;
+    const int8_t *wrow = w + min(n, N - 1) * ws;
+    // pieces from K on meet zeros of q: what they hold does not matter
+    auto load_w = [&](int b) { return (vx_i4)*(const vx_i4_at1 *)(wrow + min(b * 64 + koff, K - 16)); };
+    vx_i4 weights[BR];
+#pragma unroll
+    for (int b = 0; b < BR; ++b) weights[b] = load_w(b);
+    for (int b = 0; b < BL; ++b) *(vx_i4 *)(s_w + ((b * 16 + wave) * 64 + lane) * 16) = load_w(BR + b);   // read by this lane only
+    if (threadIdx.x < N) {
+        s_sw[threadIdx.x] = sw[threadIdx.x];
+        s_bias[threadIdx.x] = bias ? bias[threadIdx.x] : 0.f;
+    }
+    auto put = [&](int buf, long long tile) {
+        const long long m = tile * 16 + wave;
+        if (m >= M) return;
+        const float *y = &s_y[buf][wave * YP];
+        if (out_dtype == VX_DTYPE_F32) vx_linear_put_row<VX_DTYPE_F32>(y, out, m * os, N);
+        else if (out_dtype == VX_DTYPE_F16) vx_linear_put_row<VX_DTYPE_F16>(y, out, m * os, N);
+        else vx_linear_put_row<VX_DTYPE_BF16>(y, out, m * os, N);
+    };
+    auto step = [&](vx_vec<DT> (&v)[U], int buf, long long tile) {
+        unsigned top = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if ((u * 64 + lane) * VEC >= K) v[u].raw = vx_v4{0.f, 0.f, 0.f, 0.f};
+            top = vx_quant_look<DT>(v[u], top);
+        }
+        top = vx_wave_max(top);
+        const vx_quant_row what(top);
+        if (lane == 0) s_scale[buf][wave] = what.scale();
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int c = (u * 64 + lane) * VEC;
+            const vx_quant_out<DT> o = vx_quant_piece<DT>(v[u], what);
+            if (U * 64 * VEC == KC || c < KC) {
+#pragma unroll
+                for (int k = 0; k < VEC / 4; ++k) *(unsigned *)(&s_q[buf][wave * PITCH + c + 4 * k]) = o.w[k];
+            }
+        }
+        __syncthreads();
+        if (tile != blockIdx.x) put(buf ^ 1, tile - gridDim.x);
+        fetch(v, tile + 2 * (long long)gridDim.x);
+        vx_i4 acc[2] = {};
+        const int8_t *q = &s_q[buf][(lane & 15) * PITCH + koff];
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            const vx_i4 a = b < BR ? weights[b < BR ? b : 0] : *(const vx_i4 *)(s_w + (((b - BR) * 16 + wave) * 64 + lane) * 16);
+            acc[b & 1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, *(const vx_i4 *)(q + b * 64), acc[b & 1], 0, 0, 0);
+            if (b % 4 == 3) __builtin_amdgcn_sched_barrier(0);    // no more operands on their way than registers left
+        }
+        // lane l holds token l % 16, channels 4 (l / 16) .. + 3 of the wave's
+        const int n4 = wave * 16 + (lane >> 4) * 4;
+        const float sm = s_scale[buf][lane & 15];
+        vx_v4 y;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[k] = vx_linear_out(acc[0][k] + acc[1][k], sm, s_sw[n4 + k], bias != nullptr, s_bias[n4 + k]);
+        *(vx_v4 *)&s_y[buf][(lane & 15) * YP + n4] = y;
+    };
+    long long tile = blockIdx.x;                                  // the grid has no more workgroups than tiles
+    while (true) {
+        step(va, 0, tile);
+        if (tile + gridDim.x >= tiles) { __syncthreads(); put(0, tile); return; }
+        tile += gridDim.x;
+        step(vb, 1, tile);
+        if (tile + gridDim.x >= tiles) { __syncthreads(); put(1, tile); return; }
+        tile += gridDim.x;
+    }
+}
+
+// Which products with quantisation go this way (us of the whole call, this / quantise and multiply; N = 255, x fp32):
+// M = 43264: K = 256 26/39, 512 31/44, 1024 54/67; M = 8192: 16/18, 15/17, 20/19; M = 65: 15/17.  At M = 1 it is
+// 11 us of kernel time against 7 (the weights take longer to arrive than to be used).  N = 64 behaves alike.
+#define VX_STREAM_MAX 64
+#define VX_ROWS_MAX_K 1024
+static bool vx_linear_by_rows(int64_t M, int64_t N, int K) {
+    return M > VX_STREAM_MAX && N <= VX_ROWS_MAX_N && K <= VX_ROWS_MAX_K && K % 16 == 0;
+}
+
+static int vx_linear_rows_launch(const void *x, int dtype, long long xs, long long M, const int8_t *w, long long ws, const float *sw, int N,
+                                 int K, const float *bias, void *out, int out_dtype, long long os, hipStream_t st) {
+    vx_prof_begin(VX_PROF_LINEAR, st);
+    const dim3 grid((unsigned)min((M + 15) / 16, 256LL));         // one workgroup a compute unit
+    VX_DISPATCH_DTYPE(dtype, {
+        if (K <= 256) hipLaunchKernelGGL((vx_k_linear_rows<DT, 256>), grid, dim3(1024), 0, st, x, xs, M, w, ws, sw, N, K, bias, out, out_dtype, os);
+        else if (K <= 512) hipLaunchKernelGGL((vx_k_linear_rows<DT, 512>), grid, dim3(1024), 0, st, x, xs, M, w, ws, sw, N, K, bias, out, out_dtype, os);
+        else hipLaunchKernelGGL((vx_k_linear_rows<DT, 1024>), grid, dim3(1024), 0, st, x, xs, M, w, ws, sw, N, K, bias, out, out_dtype, os);
+    });
+    vx_prof_end(VX_PROF_LINEAR, st);
+    return hipGetLastError() == hipSuccess ? VX_OK : VX_ERR_LAUNCH;
+}
+
 // rows of K bytes to rows of `pitch` (a multiple of 128), padded with zeros
 __global__ __launch_bounds__(256) void vx_k_pad_rows(const int8_t *__restrict__ src, long long stride, long long rows, int K,
                                                      int8_t *__restrict__ dst, int pitch) {
@@ -442,7 +640,6 @@ __global__ __launch_bounds__(256) void vx_k_pad_rows(const int8_t *__restrict__ 
 //   units (32000 x 4096, M = 64: 34 by 64 against 37 by 128; M = 96: 44 against 38.  8192 x 4096: M = 1536, 192 tiles
 //   of 256: 54 against 60 by 128; M = 1024, 128 tiles: 48 against 41.  8192 x 8192, M = 128, 64 tiles of 128: 43 against 33 by
 //   64; M = 512, 256 tiles: 47 against 58)
-#define VX_STREAM_MAX 64
 static bool vx_linear_streams(int64_t M, int64_t N, int K) {
     return M <= 8 || (M <= VX_STREAM_MAX && (N < 16384 || K % 16 != 0));
 }
@@ -557,6 +754,8 @@ extern "C" int vx_linear_w8a8(const void *d_x, int x_dtype, int64_t x_stride, in
     if (((uintptr_t)d_x & (vx_elem_size(x_dtype) - 1)) || ((uintptr_t)d_workspace & 255)) return VX_ERR_ALIGNMENT;
     if (workspace_bytes < vx_linear_w8a8_workspace_bytes(M, N, K)) return VX_ERR_WORKSPACE;
     hipStream_t st = (hipStream_t)stream;
+    if (vx_linear_by_rows(M, N, K))
+        return vx_linear_rows_launch(d_x, x_dtype, x_stride, M, d_w, w_stride, d_w_scale, (int)N, K, d_bias, d_out, out_dtype, out_stride, st);
     const long long pitch = vx_k_pitch(K);
     float *s = (float *)d_workspace;
     int8_t *q = (int8_t *)d_workspace + vx_up256((size_t)M * 4), *pad = q + vx_up256((size_t)(M * pitch));
