@@ -380,6 +380,31 @@ def test_linear_of_few_channels(M, N, K):
             assert torch.equal(got[finite.to(DEV)], two[finite.to(DEV)])
 
 
+@pytest.mark.parametrize("N,K", [(1, 1), (17, 63), (255, 64), (4096, 1024), (4097, 512), (5000, 1000), (16385, 2049), (32000, 640), (65536, 70), (65537, 64),
+                                 (5, 32768), (7, 32769), (40001, 513)])
+def test_linear_of_one_token(N, K):
+    """A single token is quantised by every workgroup for itself: one to several tiles of channels each, odd sizes, every type, and
+    the sizes behind the last that go this way."""
+    g = gen(N + K)
+    qw = torch.randint(-128, 128, (N, K), generator=g, dtype=torch.int8)
+    sw, bias = torch.rand(N, generator=g) * 0.01, torch.randn(N, generator=g)
+    W, SW, B = qw.to(DEV), sw.to(DEV), bias.to(DEV)
+    for xt in TYPES:
+        x = torch.randn(1, K, generator=g).to(xt)
+        X = x.to(DEV)
+        q, s = quant_ref(x)
+        for ot, b, bd in zip(TYPES, (None, bias, None), (None, B, None)):
+            got = ops.linear_w8a8(X, W, SW, bd, out_dtype=ot)
+            ref, tol = product_ref(q, s, qw, sw, b, ot)
+            assert bool(((got.cpu().double() - ref).abs() <= tol).all())
+            assert torch.equal(got, ops.linear_i8(*ops.quantize_rows_i8(X), W, SW, bd, out_dtype=ot))
+        for value in (float("nan"), -float("inf")):
+            X[0, K // 2] = value
+            assert bool(ops.linear_w8a8(X, W, SW).isnan().all())
+        X.zero_()
+        assert torch.equal(ops.linear_w8a8(X, W, SW, B, out_dtype=torch.float32), B[None])
+
+
 def test_linear_of_few_channels_writes_its_rows_only():
     """Strides of every operand, none a multiple of 16 bytes, through the C ABI: the columns and rows around the result stay."""
     lib, g = L.lib(), gen(19)

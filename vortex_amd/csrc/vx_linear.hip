@@ -275,6 +275,111 @@ __global__ __launch_bounds__(1024) void vx_k_linear_stream(const int8_t *__restr
     }
 }
 
+// The same for one token that is quantised on the way: every workgroup does it for itself, in LDS, while its first weights are
+// coming, and then takes several tiles of 16 channels.  The loads of a tile's first weights are on their way while the waves
+// join the sums of the tile before.  32000 x 4096: 131 MB in 25 us of the whole call, against 28 in two launches.
+template <int DT>
+__global__ __launch_bounds__(1024) void vx_k_linear_one(const void *__restrict__ x, const int8_t *__restrict__ w, long long ws,
+                                                        const float *__restrict__ sw, long long N, int K, const float *__restrict__ bias,
+                                                        void *__restrict__ out, int out_dtype, int tiles) {
+    typedef typename vx_elem<DT>::type E;
+    constexpr int VEC = 16 / sizeof(E), UN = 8;
+    extern __shared__ __attribute__((aligned(16))) int8_t s_one[];    // q: K rounded up to 64; sums: 2 x [waves][16 channels]
+    __shared__ unsigned s_top[16];
+    const int lane = vx_lane(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int k64 = (K + 63) & ~63, koff = (lane >> 4) * 16;
+    int *s_sum = (int *)(s_one + k64);
+    const int blocks = k64 >> 6, per = (blocks + waves - 1) / waves, full = K >> 6;
+    const int b0 = min(blocks, wave * per), end = min(blocks, b0 + per), end_full = min(end, full);
+    auto row_of = [&](int tile) { return w + min((long long)tile * 16 + (lane & 15), N - 1) * ws + koff; };
+    auto load = [](const int8_t *row, int at) { return (vx_i4)*(const vx_i4_at1 *)(row + at * 64); };
+    const int8_t *wrow = row_of(blockIdx.x);
+    vx_i4 a[UN];
+    const bool ahead = b0 + UN <= end_full;
+    if (ahead) {
+#pragma unroll
+        for (int u = 0; u < UN; ++u) a[u] = load(wrow, b0 + u);
+    }
+    const E *row = (const E *)x;
+    unsigned top = 0;
+    for (int c = threadIdx.x * VEC; c < K; c += blockDim.x * VEC) top = vx_quant_look<DT>(vx_load_vec<DT>(row + c, K - c), top);
+    top = vx_wave_max(top);
+    if (lane == 0) s_top[wave] = top;
+    __syncthreads();
+    for (int i = 0; i < waves; ++i) top = max(top, s_top[i]);
+    const vx_quant_row what(top);
+    for (int c = threadIdx.x * VEC; c < k64; c += blockDim.x * VEC) {
+        const vx_quant_out<DT> o = vx_quant_piece<DT>(vx_load_vec<DT>(row + c, K - c), what);
+#pragma unroll
+        for (int k = 0; k < VEC / 4; ++k) *(unsigned *)(s_one + c + 4 * k) = o.w[k];
+    }
+    __syncthreads();
+    const int8_t *q = s_one + koff;                               // all 16 columns of the matrix instruction are this token
+    for (int tile = blockIdx.x, buf = 0; tile < tiles; tile += gridDim.x, buf ^= 1) {
+        const int8_t *next = row_of(min(tile + (int)gridDim.x, tiles - 1));
+        vx_i4 acc[2] = {};
+        auto multiply = [&](const vx_i4 &weights, int at, int i) {
+            acc[i & 1] = __builtin_amdgcn_mfma_i32_16x16x64_i8(weights, *(const vx_i4 *)(q + at * 64), acc[i & 1], 0, 0, 0);
+        };
+        int b = b0;
+        if (ahead) {
+            for (; b + 2 * UN <= end_full; b += UN) {
+#pragma unroll
+                for (int u = 0; u < UN; ++u) {
+                    multiply(a[u], b + u, u);
+                    a[u] = load(wrow, b + UN + u);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < UN; ++u) {
+                multiply(a[u], b + u, u);
+                if (tile + (int)gridDim.x < tiles) a[u] = load(next, b0 + u);
+            }
+            b += UN;
+        }
+        for (; b < end_full; ++b) multiply(load(wrow, b), b, 0);
+        if (b < end) {                                            // weights from K on meet zeros; those outside the matrix are not read
+            const int k = b * 64;
+            multiply(wrow + k + 16 <= w + (N - 1) * ws + K ? load(wrow, b) : vx_i8_tail(wrow, k, K - koff), b, 0);
+        }
+        int *sums = s_sum + buf * waves * 16;
+        if ((lane & 15) == 0) *(vx_i4 *)&sums[wave * 16 + (lane >> 4) * 4] = acc[0] + acc[1];
+        __syncthreads();
+        const long long n = (long long)tile * 16 + threadIdx.x;
+        if (threadIdx.x < 16 && n < N) {
+            int sum = 0;
+            for (int i = 0; i < waves; ++i) sum += sums[i * 16 + threadIdx.x];
+            const float y = vx_linear_out(sum, what.scale(), sw[n], bias != nullptr, bias ? bias[n] : 0.f);
+            if (out_dtype == VX_DTYPE_F32) ((float *)out)[n] = y;
+            else if (out_dtype == VX_DTYPE_F16) ((_Float16 *)out)[n] = vx_store_cast<VX_DTYPE_F16>(y);
+            else ((__bf16 *)out)[n] = vx_store_cast<VX_DTYPE_BF16>(y);
+        }
+        wrow = next;
+    }
+}
+
+// Which single tokens go this way (us in a graph, this / quantise and stream; bf16): 1000 x 512 4/7, 4096 x 4096 7/10,
+// 8192 x 8192 17/19, 32000 x 1024 10/13, 32000 x 4096 26/28, 65536 x 4096 48/50, but 131072 x 4096 101/94.  Two tokens gain
+// in bf16 (27/28) and lose in fp32 (31/28).
+#define VX_ONE_MAX_N 65536
+#define VX_ONE_MAX_K 32768
+static bool vx_linear_by_one(int64_t M, int64_t N, int K) { return M == 1 && N <= VX_ONE_MAX_N && K <= VX_ONE_MAX_K; }
+
+static int vx_linear_one_launch(const void *x, int dtype, const int8_t *w, long long ws, const float *sw, long long N, int K,
+                                const float *bias, void *out, int out_dtype, hipStream_t st) {
+    vx_prof_begin(VX_PROF_LINEAR, st);
+    const int waves = N <= 4096 ? 16 : 4;                         // few channels: more waves side by side along K
+    // up to four workgroups a compute unit, with equally many tiles (512 / 1280 / 2048 of them: 28 / 26 / 28 instead of 26 us)
+    const int tiles = (int)((N + 15) / 16), each = (tiles + 1023) / 1024;
+    const dim3 grid((unsigned)((tiles + each - 1) / each));
+    const size_t lds = (size_t)((K + 63) & ~63) + (size_t)2 * waves * 64;
+    VX_DISPATCH_DTYPE(dtype, {
+        hipLaunchKernelGGL((vx_k_linear_one<DT>), grid, dim3(waves * 64), lds, st, x, w, ws, sw, N, K, bias, out, out_dtype, tiles);
+    });
+    vx_prof_end(VX_PROF_LINEAR, st);
+    return hipGetLastError() == hipSuccess ? VX_OK : VX_ERR_LAUNCH;
+}
+
 // ---- many tokens: TM x TN outputs for each workgroup, WM x WN waves of 32x32x32 mfma tiles (weights as rows, tokens as
 // columns, so a lane's four accumulators in a row are four neighbouring channels of one token).
 // K goes by stages of 128 bytes, a whole cache line of each row (requests of 64 bytes found the line of the request before
@@ -754,6 +859,8 @@ extern "C" int vx_linear_w8a8(const void *d_x, int x_dtype, int64_t x_stride, in
     if (((uintptr_t)d_x & (vx_elem_size(x_dtype) - 1)) || ((uintptr_t)d_workspace & 255)) return VX_ERR_ALIGNMENT;
     if (workspace_bytes < vx_linear_w8a8_workspace_bytes(M, N, K)) return VX_ERR_WORKSPACE;
     hipStream_t st = (hipStream_t)stream;
+    if (vx_linear_by_one(M, N, K))
+        return vx_linear_one_launch(d_x, x_dtype, d_w, w_stride, d_w_scale, N, K, d_bias, d_out, out_dtype, st);
     if (vx_linear_by_rows(M, N, K))
         return vx_linear_rows_launch(d_x, x_dtype, x_stride, M, d_w, w_stride, d_w_scale, (int)N, K, d_bias, d_out, out_dtype, out_stride, st);
     const long long pitch = vx_k_pitch(K);
