@@ -9,8 +9,8 @@
 // Launches over chunks of the vocabulary:
 //   stats   every used row: largest logit and fp32 sum of exponentials of each quarter of a chunk (bound by the one read of the logits;
 //           fp64 exponentials here would take twice the time of the read)
-//   choose  the accepted drafts and the row to draw from; that row's (and the draft row's) chunk sums again in fp64
-//   rest    (with draft logits) that row's chunk sums of max(0, p - q), fp64
+//   choose  the accepted drafts and the row to draw from; that row's (and the draft row's) sums again in fp64, of each quarter
+//   rest    (with draft logits) that row's sums of max(0, p - q), fp64, of each quarter
 //   draw    the token, one workgroup a sequence
 // The token that is drawn is a whole number, decided by where a cumulative sum passes a border, and one step of a flat
 // distribution is 1/V: everything it depends on is fp64.  How far the sums of the first launch are off, u = 2^-24:
@@ -34,8 +34,8 @@ struct vx_verify_args {
     int B, K, V, chunks;
     // workspace
     float2 *stats;                                // [B][2 K + 1][4 chunks], for each wave: largest logit (NaN: an invalid one), sum (greedy: its index)
-    double2 *z;                                   // [B][chunks]: sums of the row that is drawn from, target and draft
-    double *r;                                    // [B][chunks]: sums of max(0, p - q)
+    double2 *z;                                   // [B][4 chunks]: sums of the row that is drawn from, target and draft, of each quarter of a chunk
+    double *r;                                    // [B][4 chunks]: sums of max(0, p - q)
     struct vx_choice *choice;                     // [B]
     // outputs
     long long *out;                               // [B, K + 1]
@@ -52,6 +52,7 @@ struct vx_choice {                                // what is left to do for a se
 
 // chunk of a row: 256 threads x U pieces of 16 bytes
 #define VX_VERIFY_U 4
+// (256 threads x one piece in the draw: a quarter of it)
 template <int DT> __host__ __device__ constexpr int vx_verify_chunk() { return 256 * VX_VERIFY_U * 16 / (int)sizeof(typename vx_elem<DT>::type); }
 
 __device__ __forceinline__ int vx_verify_len(const vx_verify_args &a, int b) {
@@ -99,17 +100,20 @@ __device__ __forceinline__ double vx_verify_c(float T) { return 1.44269504088896
 // the same in fp32; finite and not 0, so that the product with a masked logit is -inf at any temperature
 __device__ __forceinline__ float vx_verify_c32(float T) { return fminf(fmaxf((float)vx_verify_c(T), 1e-45f), 3e38f); }
 
-// the thread's values of a chunk, -inf where the row has ended: pieces of 16 bytes, 256 apart (the threads side by side) or
-// (IN_ORDER) next to each other
-template <int DT, bool IN_ORDER = false>
+// the thread's values of a chunk, -inf where the row has ended: pieces of 16 bytes, the lanes side by side.  QUARTERS: each wave has
+// its own quarter of the chunk; otherwise the waves' pieces alternate (statistics of 185 MB: 37 against 32 us)
+template <bool QUARTERS>
+__device__ __forceinline__ int vx_verify_piece(int u) {
+    return QUARTERS ? ((int)(threadIdx.x >> 6) * VX_VERIFY_U + u) * 64 + vx_lane() : u * 256 + (int)threadIdx.x;
+}
+template <int DT, bool QUARTERS>
 __device__ __forceinline__ void vx_verify_load(const typename vx_elem<DT>::type *row, int c0, int V,
                                                float x[VX_VERIFY_U * 16 / sizeof(typename vx_elem<DT>::type)]) {
     constexpr int VEC = 16 / sizeof(typename vx_elem<DT>::type);
     vx_vec<DT> v[VX_VERIFY_U];
-    auto piece = [](int u) { return IN_ORDER ? threadIdx.x * VX_VERIFY_U + u : u * 256 + threadIdx.x; };
     if (c0 + vx_verify_chunk<DT>() <= V) {
 #pragma unroll
-        for (int u = 0; u < VX_VERIFY_U; ++u) v[u].raw = vx_load16<DT>(row + c0 + piece(u) * VEC);
+        for (int u = 0; u < VX_VERIFY_U; ++u) v[u].raw = vx_load16<DT>(row + c0 + vx_verify_piece<QUARTERS>(u) * VEC);
 #pragma unroll
         for (int u = 0; u < VX_VERIFY_U; ++u)
 #pragma unroll
@@ -117,7 +121,7 @@ __device__ __forceinline__ void vx_verify_load(const typename vx_elem<DT>::type 
     } else {
 #pragma unroll
         for (int u = 0; u < VX_VERIFY_U; ++u) {
-            const int at = c0 + piece(u) * VEC;
+            const int at = c0 + vx_verify_piece<QUARTERS>(u) * VEC;
             v[u] = vx_load_vec<DT>(row + at, V - at);
 #pragma unroll
             for (int k = 0; k < VEC; ++k) x[u * VEC + k] = at + k < V ? (float)v[u].e[k] : -INFINITY;
@@ -139,7 +143,7 @@ __global__ __launch_bounds__(256) void vx_k_verify_stats(vx_verify_args a) {
     if (is_draft ? (j - a.K - 1 >= n || greedy) : j > n) return;
     float x[PER];
     const int c0 = chunk * vx_verify_chunk<DT>();
-    vx_verify_load<DT>(is_draft ? vx_verify_draft<DT>(a, b, j - a.K - 1) : vx_verify_target<DT>(a, b, j), c0, a.V, x);
+    vx_verify_load<DT, false>(is_draft ? vx_verify_draft<DT>(a, b, j - a.K - 1) : vx_verify_target<DT>(a, b, j), c0, a.V, x);
     float m = -INFINITY;
 #pragma unroll
     for (int k = 0; k < PER; ++k) m = fmaxf(m, x[k]);
@@ -151,7 +155,7 @@ __global__ __launch_bounds__(256) void vx_k_verify_stats(vx_verify_args a) {
     if (greedy) {
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
-            const int i = c0 + ((k / VEC) * 256 + threadIdx.x) * VEC + k % VEC;
+            const int i = c0 + vx_verify_piece<false>(k / VEC) * VEC + k % VEC;
             bad |= !(x[k] < INFINITY);
             if (x[k] == m) best = min(best, i);
         }
@@ -174,10 +178,14 @@ __global__ __launch_bounds__(256) void vx_k_verify_stats(vx_verify_args a) {
             float2{bad ? __builtin_nanf("") : m, greedy ? __int_as_float(best) : z};
 }
 
-// sum over the workgroup's 256 threads, in one order; every thread gets it
-__device__ __forceinline__ double vx_verify_sum(double v, double *s_sum) {
+__device__ __forceinline__ double vx_verify_wave_sum(double v) {
 #pragma unroll
     for (int k = 32; k >= 1; k >>= 1) v += __shfl_xor(v, k, VX_WAVE);
+    return v;
+}
+// sum over the workgroup's 256 threads, in one order; every thread gets it
+__device__ __forceinline__ double vx_verify_sum(double v, double *s_sum) {
+    v = vx_verify_wave_sum(v);
     __syncthreads();
     if (vx_lane() == 0) s_sum[threadIdx.x >> 6] = v;
     __syncthreads();
@@ -189,7 +197,7 @@ template <int DT>
 __device__ __forceinline__ double vx_verify_chunk_sum(const typename vx_elem<DT>::type *row, int chunk, int V, float m, double c) {
     constexpr int PER = VX_VERIFY_U * 16 / sizeof(typename vx_elem<DT>::type);
     float x[PER];
-    vx_verify_load<DT>(row, chunk * vx_verify_chunk<DT>(), V, x);
+    vx_verify_load<DT, true>(row, chunk * vx_verify_chunk<DT>(), V, x);
     double z = 0.0;
 #pragma unroll
     for (int k = 0; k < PER; ++k) z += vx_weight(x[k], m, c);
@@ -334,9 +342,9 @@ __global__ __launch_bounds__(256) void vx_k_verify_choose(vx_verify_args a) {
         }
     }
     if (mode == 0) return;
-    const double zp = vx_verify_sum(vx_verify_chunk_sum<DT>(vx_verify_target<DT>(a, b, acc), chunk, a.V, s_m[acc], c), s_sum);
-    const double zq = mode == 3 ? vx_verify_sum(vx_verify_chunk_sum<DT>(vx_verify_draft<DT>(a, b, acc), chunk, a.V, s_m[VX_MAX_DRAFTS + 1 + acc], c), s_sum) : 0.0;
-    if (threadIdx.x == 0) a.z[(long long)b * a.chunks + chunk] = double2{zp, zq};
+    const double zp = vx_verify_wave_sum(vx_verify_chunk_sum<DT>(vx_verify_target<DT>(a, b, acc), chunk, a.V, s_m[acc], c));
+    const double zq = mode == 3 ? vx_verify_wave_sum(vx_verify_chunk_sum<DT>(vx_verify_draft<DT>(a, b, acc), chunk, a.V, s_m[VX_MAX_DRAFTS + 1 + acc], c)) : 0.0;
+    if (lane == 0) a.z[((long long)b * a.chunks + chunk) * 4 + w] = double2{zp, zq};
 }
 
 struct vx_pick_smem {
@@ -376,35 +384,35 @@ __device__ __forceinline__ int vx_pick_part(double sum, double base, double goal
     return first < 256 ? first : -1;
 }
 
-// The first i whose cumulative weight passes u * total; `sums(k)` the weight of chunk k, `weight(i)` of one token, `part(i)` of
-// the CHUNK / 256 tokens from i on.  One workgroup: first the chunk, then the 1/256 of it, then the token; where rounding
-// leaves none, the last one with a weight.  -1 where no token has a weight.
-template <int CHUNK, class S, class P, class W>
-__device__ __forceinline__ int vx_verify_pick(int chunks, int V, float u, S sums, P part_weight, W weight, vx_pick_smem &sm, double *s_sum) {
-    constexpr int PART = CHUNK / 256;
-    const int tid = threadIdx.x, per = (chunks + 255) / 256;      // chunks of one thread
+// The first i whose cumulative weight passes u * total; `sums(k)` the weight of the k-th run of RUN tokens, `weight(i)` of one
+// token, `part(i)` of the RUN / 256 tokens from i on.  One workgroup: first the run, then the 1/256 of it, then the token; where
+// rounding leaves none, the last one with a weight.  -1 where no token has a weight.
+template <int RUN, class S, class P, class W>
+__device__ __forceinline__ int vx_verify_pick(int runs, int V, float u, S sums, P part_weight, W weight, vx_pick_smem &sm, double *s_sum) {
+    constexpr int PART = RUN / 256;
+    const int tid = threadIdx.x, per = (runs + 255) / 256;        // runs of one thread
     double mine = 0.0, before;
     int last;
-    for (int k = tid * per; k < min(chunks, (tid + 1) * per); ++k) mine += sums(k);
+    for (int k = tid * per; k < min(runs, (tid + 1) * per); ++k) mine += sums(k);
     double goal = (double)u * vx_verify_sum(mine, s_sum);
     int part = vx_pick_part(mine, 0.0, goal, sm, before, last);
     if (last < 0) return -1;
     if (part < 0) { part = last; goal = INFINITY; before = 0.0; } // a uniform of 1, or rounding
-    int chunk = part * per;
-    if (per > 1) {                                                // more than 256 chunks: on through this thread's
+    int run = part * per;
+    if (per > 1) {                                                // more than 256 runs: on through this thread's
         int c = -1;
-        for (int k = part * per; k < min(chunks, (part + 1) * per); ++k) {
+        for (int k = part * per; k < min(runs, (part + 1) * per); ++k) {
             const double v = sums(k);
             if (v > 0.0) c = k;
             if (before + v > goal) break;
             before += v;
         }
-        chunk = c < 0 ? chunk : c;
+        run = c < 0 ? run : c;
     }
-    mine = part_weight(chunk * CHUNK + tid * PART);
+    mine = part_weight(run * RUN + tid * PART);
     part = vx_pick_part(mine, before, goal, sm, before, last);
     if (part < 0) { part = max(last, 0); goal = INFINITY; }
-    const int i = chunk * CHUNK + part * PART + tid;
+    const int i = run * RUN + part * PART + tid;
     part = vx_pick_part(tid < PART && i < V ? weight(i) : 0.0, before, goal, sm, before, last);
     return i - tid + (part < 0 ? max(last, 0) : part);
 }
@@ -417,8 +425,8 @@ __device__ __forceinline__ double vx_verify_rest(float x, float y, const vx_choi
 // sums of the two rows over all chunks, in the same order wherever they are needed
 __device__ __forceinline__ double2 vx_verify_totals(const vx_verify_args &a, int b, double *s_sum) {
     double zp = 0.0, zq = 0.0;
-    for (int k = threadIdx.x; k < a.chunks; k += 256) {
-        const double2 v = a.z[(long long)b * a.chunks + k];
+    for (int k = threadIdx.x; k < a.chunks * 4; k += 256) {
+        const double2 v = a.z[(long long)b * a.chunks * 4 + k];
         zp += v.x;
         zq += v.y;
     }
@@ -426,7 +434,7 @@ __device__ __forceinline__ double2 vx_verify_totals(const vx_verify_args &a, int
     return double2{zp, vx_verify_sum(zq, s_sum)};
 }
 
-// Chunk sums of max(0, p - q): one workgroup per (sequence, chunk).
+// Sums of max(0, p - q): one workgroup per (sequence, chunk).
 template <int DT>
 __global__ __launch_bounds__(256) void vx_k_verify_rest(vx_verify_args a) {
     constexpr int CHUNK = vx_verify_chunk<DT>(), PER = VX_VERIFY_U * 16 / sizeof(typename vx_elem<DT>::type);
@@ -435,62 +443,59 @@ __global__ __launch_bounds__(256) void vx_k_verify_rest(vx_verify_args a) {
     const vx_choice ch = a.choice[b];
     if (ch.mode != 3) return;
     float x[PER], y[PER];
-    vx_verify_load<DT>(vx_verify_target<DT>(a, b, ch.row), chunk * CHUNK, a.V, x);
-    vx_verify_load<DT>(vx_verify_draft<DT>(a, b, ch.row), chunk * CHUNK, a.V, y);
+    vx_verify_load<DT, true>(vx_verify_target<DT>(a, b, ch.row), chunk * CHUNK, a.V, x);
+    vx_verify_load<DT, true>(vx_verify_draft<DT>(a, b, ch.row), chunk * CHUNK, a.V, y);
     const double c = vx_verify_c(vx_verify_t(a, b));
     const double2 z = vx_verify_totals(a, b, s_sum);
     const double ip = 1.0 / z.x, iq = 1.0 / z.y;
     double sum = 0.0;
 #pragma unroll
     for (int k = 0; k < PER; ++k) sum += vx_verify_rest(x[k], y[k], ch, c, ip, iq);
-    sum = vx_verify_sum(sum, s_sum);
-    if (threadIdx.x == 0) a.r[(long long)b * a.chunks + chunk] = sum;
+    sum = vx_verify_wave_sum(sum);
+    if (vx_lane() == 0) a.r[((long long)b * a.chunks + chunk) * 4 + (threadIdx.x >> 6)] = sum;
 }
 
 // The drawn token: one workgroup per sequence.
 template <int DT>
 __global__ __launch_bounds__(256) void vx_k_verify_draw(vx_verify_args a) {
-    constexpr int CHUNK = vx_verify_chunk<DT>(), PER = CHUNK / 256;
+    constexpr int RUN = vx_verify_chunk<DT>() / 4, PER = RUN / 256;
     __shared__ double s_sum[4];
     __shared__ vx_pick_smem sm;
-    const int b = blockIdx.x;
+    const int b = blockIdx.x, runs = a.chunks * 4;
     const vx_choice ch = a.choice[b];
     const float u = a.uniforms[(long long)b * (a.K + 1) + a.K];
     const double c = vx_verify_c(vx_verify_t(a, b));
     if (ch.mode == 0) return;
     const typename vx_elem<DT>::type *trow = vx_verify_target<DT>(a, b, ch.row);
-    const double2 *z = a.z + (long long)b * a.chunks;
+    const double2 *z = a.z + (long long)b * runs;
     auto from_p = [&](long long drop) {
         auto one = [&](int i) { return i == drop ? 0.0 : vx_weight((float)trow[i], ch.mp, c); };
-        auto part = [&](int i) {                                  // i = the chunk's first token + threadIdx.x * PER
-            float x[PER];
-            vx_verify_load<DT, true>(trow, i - threadIdx.x * PER, a.V, x);
+        auto part = [&](int i) {                                  // the PER tokens from i on
+            const vx_vec<DT> x = vx_load_vec<DT>(trow + i, a.V - i);
             double sum = 0.0;
 #pragma unroll
-            for (int k = 0; k < PER; ++k) sum += i + k == drop ? 0.0 : vx_weight(x[k], ch.mp, c);
+            for (int k = 0; k < PER; ++k) sum += i + k >= a.V || i + k == drop ? 0.0 : vx_weight((float)x.e[k], ch.mp, c);
             return sum;
         };
-        // a chunk that loses a token is summed again: its sum less the token's weight could be all rounding
-        const int drop_chunk = drop >= 0 && drop < a.V ? (int)(drop / CHUNK) : -1;
-        const double again = drop_chunk >= 0 ? vx_verify_sum(part(drop_chunk * CHUNK + threadIdx.x * PER), s_sum) : 0.0;
-        return vx_verify_pick<CHUNK>(a.chunks, a.V, u, [&](int k) { return k == drop_chunk ? again : z[k].x; }, part, one, sm, s_sum);
+        // a run that loses a token is summed again: its sum less the token's weight could be all rounding
+        const int drop_run = drop >= 0 && drop < a.V ? (int)(drop / RUN) : -1;
+        const double again = drop_run >= 0 ? vx_verify_sum(part(drop_run * RUN + threadIdx.x * PER), s_sum) : 0.0;
+        return vx_verify_pick<RUN>(runs, a.V, u, [&](int k) { return k == drop_run ? again : z[k].x; }, part, one, sm, s_sum);
     };
     int i;
     if (ch.mode == 3) {
         const typename vx_elem<DT>::type *drow = vx_verify_draft<DT>(a, b, ch.row);
         const double2 t = vx_verify_totals(a, b, s_sum);
-        const double ip = 1.0 / t.x, iq = 1.0 / t.y, *r = a.r + (long long)b * a.chunks;
+        const double ip = 1.0 / t.x, iq = 1.0 / t.y, *r = a.r + (long long)b * runs;
         auto one = [&](int k) { return vx_verify_rest((float)trow[k], (float)drow[k], ch, c, ip, iq); };
         auto part = [&](int i) {
-            float x[PER], y[PER];
-            vx_verify_load<DT, true>(trow, i - threadIdx.x * PER, a.V, x);
-            vx_verify_load<DT, true>(drow, i - threadIdx.x * PER, a.V, y);
+            const vx_vec<DT> x = vx_load_vec<DT>(trow + i, a.V - i), y = vx_load_vec<DT>(drow + i, a.V - i);
             double sum = 0.0;
 #pragma unroll
-            for (int k = 0; k < PER; ++k) sum += vx_verify_rest(x[k], y[k], ch, c, ip, iq);
+            for (int k = 0; k < PER; ++k) sum += i + k >= a.V ? 0.0 : vx_verify_rest((float)x.e[k], (float)y.e[k], ch, c, ip, iq);
             return sum;
         };
-        i = vx_verify_pick<CHUNK>(a.chunks, a.V, u, [&](int k) { return r[k]; }, part, one, sm, s_sum);
+        i = vx_verify_pick<RUN>(runs, a.V, u, [&](int k) { return r[k]; }, part, one, sm, s_sum);
     } else {
         i = from_p(ch.drop);
     }
@@ -509,8 +514,8 @@ static vx_verify_plan vx_verify_make_plan(int B, int K, int V, int chunk) {
     size_t at = 0;
     auto take = [&](size_t n) { const size_t o = at; at += (n + 255) & ~(size_t)255; return o; };
     p.stats = take((size_t)B * (2 * K + 1) * p.chunks * 4 * sizeof(float2));
-    p.z = take((size_t)B * p.chunks * sizeof(double2));
-    p.r = take((size_t)B * p.chunks * sizeof(double));
+    p.z = take((size_t)B * p.chunks * 4 * sizeof(double2));
+    p.r = take((size_t)B * p.chunks * 4 * sizeof(double));
     p.choice = take((size_t)B * sizeof(vx_choice));
     p.total = at;
     return p;
