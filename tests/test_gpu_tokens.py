@@ -405,6 +405,61 @@ def test_linear_of_one_token(N, K):
         assert torch.equal(ops.linear_w8a8(X, W, SW, B, out_dtype=torch.float32), B[None])
 
 
+@pytest.mark.parametrize("M,N,K", [(2, 1, 1), (2, 15, 64), (64, 100, 512), (3, 2049, 1000), (5, 5000, 513), (8, 9000, 4096), (9, 4097, 4097), (17, 20001, 70),
+                                   (33, 33000, 129), (37, 16401, 1000), (48, 66000, 96), (64, 70001, 513), (16, 32769, 2048), (16, 17000, 4096), (4, 131073, 100),
+                                   (64, 33000, 2301), (1, 40001, 4097), (32, 200, 1024), (49, 131075, 65)])
+def test_linear_of_few_tokens(M, N, K):
+    """2 to 64 tokens that a workgroup holds all at once, quantised by itself or before: one to sixteen waves for a tile of channels, one
+    to several tiles for a wave, odd sizes, every type, nearly all of the LDS."""
+    g = gen(M + N + K)
+    qw = torch.randint(-128, 128, (N, K), generator=g, dtype=torch.int8)
+    sw, bias = torch.rand(N, generator=g) * 0.01, torch.randn(N, generator=g)
+    W, SW, B = qw.to(DEV), sw.to(DEV), bias.to(DEV)
+    for xt, ot, b, bd in zip(TYPES, (torch.float16, torch.bfloat16, torch.float32), (None, bias, None), (None, B, None)):
+        x = torch.randn(M, K, generator=g).to(xt)
+        if M > 2:
+            x[1] = 0
+            x[2, K - 1] = float("inf")
+        X = x.to(DEV)
+        q, s = quant_ref(x)
+        ref, tol = product_ref(q, s, qw, sw, b, ot)
+        ok = x.isfinite().all(1)
+        q8, s8 = ops.quantize_rows_i8(X)
+        for got in (ops.linear_w8a8(X, W, SW, bd, out_dtype=ot), ops.linear_i8(q8, s8, W, SW, bd, out_dtype=ot)):
+            y = got.cpu().double()
+            assert bool(((y - ref).abs() <= tol)[ok].all()) and bool(y[~ok].isnan().all())
+
+
+def test_linear_of_few_tokens_writes_its_rows_only():
+    """The same with strides that are no multiple of 16 bytes, through the C ABI: the columns and rows around the result stay, and the
+    last channel's weights end where the allocation ends."""
+    lib, g = L.lib(), gen(23)
+    for M, N, K in ((5, 77, 130), (13, 40000, 99), (1, 300, 75), (37, 17000, 65)):
+        x, w = torch.randn(M, K + 3, generator=g), torch.randint(-128, 128, (N * (K + 5),), generator=g, dtype=torch.int8)
+        sw = torch.rand(N, generator=g)
+        rows = w.as_strided((N, K), (K + 5, 1), 5)
+        q, s = quant_ref(x[:, 1:1 + K])
+        for ot, code in ((torch.float32, L.VX_DTYPE_F32), (torch.float16, L.VX_DTYPE_F16)):
+            ref, tol = product_ref(q, s, rows, sw, None, ot)
+            for quantised in (False, True):
+                out = torch.full((M + 2, N + 3), 7.0, dtype=ot, device=DEV)
+                size = lib.vx_linear_i8_workspace_bytes if quantised else lib.vx_linear_w8a8_workspace_bytes
+                nb = size(M, N, K)
+                ws, X, W, SW = torch.empty(nb, dtype=torch.uint8, device=DEV), x.to(DEV), w.to(DEV), sw.to(DEV)
+                to = out.data_ptr() + (N + 3) * out.element_size()
+                if quantised:
+                    Q, S = q.to(DEV), s.to(DEV)
+                    rc = lib.vx_linear_i8(Q.data_ptr(), K, S.data_ptr(), M, W.data_ptr() + 5, K + 5, SW.data_ptr(), N, K, None, to, code, N + 3,
+                                          ws.data_ptr(), nb, L.stream_ptr(DEV))
+                else:
+                    rc = lib.vx_linear_w8a8(X.data_ptr() + 4, L.VX_DTYPE_F32, K + 3, M, W.data_ptr() + 5, K + 5, SW.data_ptr(), N, K, None, to, code, N + 3,
+                                            ws.data_ptr(), nb, L.stream_ptr(DEV))
+                assert rc == 0
+                got = out.cpu().double()
+                assert bool(((got[1:-1, :N] - ref).abs() <= tol).all())
+                assert bool((got[0] == 7).all()) and bool((got[-1] == 7).all()) and bool((got[:, N:] == 7).all())
+
+
 def test_linear_of_few_channels_writes_its_rows_only():
     """Strides of every operand, none a multiple of 16 bytes, through the C ABI: the columns and rows around the result stay."""
     lib, g = L.lib(), gen(19)

@@ -277,7 +277,8 @@ __global__ __launch_bounds__(1024) void vx_k_linear_stream(const int8_t *__restr
 
 // The same for one token that is quantised on the way: every workgroup does it for itself, in LDS, while its first weights are
 // coming, and then takes several tiles of 16 channels.  The loads of a tile's first weights are on their way while the waves
-// join the sums of the tile before.  32000 x 4096: 131 MB in 25 us of the whole call, against 28 in two launches.
+// join the sums of the tile before.  32000 x 4096: 131 MB, 25 us for the whole call, against 28 in two
+// launches.
 template <int DT>
 __global__ __launch_bounds__(1024) void vx_k_linear_one(const void *__restrict__ x, const int8_t *__restrict__ w, long long ws,
                                                         const float *__restrict__ sw, long long N, int K, const float *__restrict__ bias,
@@ -337,6 +338,13 @@ __global__ __launch_bounds__(1024) void vx_k_linear_one(const void *__restrict__
             }
             b += UN;
         }
+        for (; b + 4 <= end_full; b += 4) {
+            vx_i4 v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = load(wrow, b + u);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) multiply(v[u], b + u, u);
+        }
         for (; b < end_full; ++b) multiply(load(wrow, b), b, 0);
         if (b < end) {                                            // weights from K on meet zeros; those outside the matrix are not read
             const int k = b * 64;
@@ -359,9 +367,9 @@ __global__ __launch_bounds__(1024) void vx_k_linear_one(const void *__restrict__
 }
 
 // Which single tokens go this way (us in a graph, this / quantise and stream; bf16): 1000 x 512 4/7, 4096 x 4096 7/10,
-// 8192 x 8192 17/19, 32000 x 1024 10/13, 32000 x 4096 26/28, 65536 x 4096 48/50, but 131072 x 4096 101/94.  Two tokens gain
-// in bf16 (27/28) and lose in fp32 (31/28).
-#define VX_ONE_MAX_N 65536
+// 8192 x 8192 16/19, 32000 x 1024 9/13, 32000 x 4096 25/28; beyond two tiles a workgroup the next kernel is faster
+// (50021 x 1000 17/13, 4000 49/40; 65536 x 512 10.6/9.6).
+#define VX_ONE_MAX_N 32768
 #define VX_ONE_MAX_K 32768
 static bool vx_linear_by_one(int64_t M, int64_t N, int K) { return M == 1 && N <= VX_ONE_MAX_N && K <= VX_ONE_MAX_K; }
 
@@ -378,6 +386,241 @@ static int vx_linear_one_launch(const void *x, int dtype, const int8_t *w, long 
     });
     vx_prof_end(VX_PROF_LINEAR, st);
     return hipGetLastError() == hipSuccess ? VX_OK : VX_ERR_LAUNCH;
+}
+
+// four results next to each other, `left` of them inside the row
+template <int OT>
+__device__ __forceinline__ void vx_store4(void *out, long long at, const float y[4], long long left) {
+    typedef typename vx_elem<OT>::type O;
+    O *to = (O *)out + at;
+    union { O e[4]; vx_v2 v2; vx_v4 v4; } o;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o.e[k] = vx_store_cast<OT>(y[k]);
+    if (left >= 4) {
+        if (sizeof(O) == 2) *(vx_v2_at2 *)to = o.v2;
+        else *(vx_v4_at4 *)to = o.v4;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+            if (k < left) to[k] = o.e[k];
+    }
+}
+
+// ---- few tokens, in LDS: one persistent workgroup of 16 waves a compute unit holds them all (quantised on the way, or copied) and
+// its waves take tiles of 16 channels, the first weights of each on their way since the tile before.  With fewer than 16 tiles
+// a compute unit 2 to 16 waves share a tile's K and join their sums in LDS.  Rows in LDS are an odd number of 16-byte pieces
+// long: 16 of them lie in all banks.  Bound by the read of the weights and, with more tokens, of LDS:
+// 37 x 50021 x 1000 fp16 to fp32 in 18 us of the whole call (57 MB), where quantising to memory and streaming took 26.
+#define VX_SRC_I8 3                                               // the tokens come quantised, with their scales
+template <int SRC, int MT, int UN>
+__global__ __launch_bounds__(1024) void vx_k_linear_few(const void *__restrict__ x, long long xs, const float *__restrict__ s, int M,
+                                                        const int8_t *__restrict__ w, long long ws, const float *__restrict__ sw,
+                                                        long long N, int K, const float *__restrict__ bias, void *__restrict__ out,
+                                                        int out_dtype, long long os, int tiles, int ks_log2) {
+    extern __shared__ __attribute__((aligned(16))) int8_t s_few[];    // q: [M][K rounded up to 64, + 16]; sums: [16 waves][MT][256] if waves share K
+    __shared__ float s_scale[16 * MT];
+    __shared__ unsigned s_top[16];
+    const int lane = vx_lane(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), KS = 1 << ks_log2, CT = 16 >> ks_log2;
+    const int ct = wave >> ks_log2, ks = wave & (KS - 1), grid = gridDim.x;
+    const int slot = grid == 256 ? (blockIdx.x & 7) * 32 + (blockIdx.x >> 3) : blockIdx.x;
+    const int k64 = (K + 63) & ~63, pitch = k64 + 16, koff = (lane >> 4) * 16;
+    const int blocks = k64 >> 6, per = (blocks + KS - 1) >> ks_log2, full = K >> 6;
+    const int b0 = min(blocks, ks * per), end = min(blocks, b0 + per), end_full = min(end, full);
+    auto row_of = [&](int tile) { return w + min((long long)tile * 16 + (lane & 15), N - 1) * ws + koff; };
+    auto load = [](const int8_t *row, int at) { return (vx_i4)*(const vx_i4_at1 *)(row + at * 64); };
+    // columns c, c + step, .. of token m
+    auto quantise = [&](const auto *row, int m, int c, int step, const vx_quant_row &what) {
+        if constexpr (SRC != VX_SRC_I8) {
+            constexpr int VEC = 16 / sizeof(*row);
+            if (c == lane * VEC && lane == 0) s_scale[m] = what.scale();
+            auto put = [&](const vx_vec<SRC> &v, int c) {
+                const vx_quant_out<SRC> o = vx_quant_piece<SRC>(v, what);
+#pragma unroll
+                for (int k = 0; k < VEC / 4; ++k) *(unsigned *)(s_few + m * pitch + c + 4 * k) = o.w[k];
+            };
+#pragma unroll 4
+            for (; c - lane * VEC + 64 * VEC <= K; c += step) {
+                vx_vec<SRC> v;
+                v.raw = vx_load16<SRC>(row + c);
+                put(v, c);
+            }
+            if (c < k64) put(vx_load_vec<SRC>(row + c, K - c), c);
+        }
+    };
+    int tile = slot + grid * ct;
+    const int8_t *wrow = row_of(min(tile, tiles - 1));
+    vx_i4 a[UN];
+    const bool ahead = b0 + UN <= end_full;
+    if (ahead && tile < tiles) {
+#pragma unroll
+        for (int u = 0; u < UN; ++u) a[u] = load(wrow, b0 + u);
+    }
+    if constexpr (SRC == VX_SRC_I8) {
+        for (int m = wave; m < M; m += 16) {
+            const int8_t *row = (const int8_t *)x + m * xs;
+            for (int c = lane * 16; c < k64; c += 1024)
+                *(vx_i4 *)(s_few + m * pitch + c) = c + 16 <= K ? (vx_i4)*(const vx_i4_at1 *)(row + c) : vx_i8_tail(row, c, K);
+            if (lane == 0) s_scale[m] = s[m];
+        }
+    } else {
+        // 1, 2, 4, 8 or 16 waves a row
+        typedef typename vx_elem<SRC>::type E;
+        constexpr int VEC = 16 / sizeof(E);
+        const int wl = M == 1 ? 4 : (M > 8 ? 0 : 4 - (32 - __builtin_clz(M - 1))), step = 64 * VEC << wl;
+        for (int m = wave >> wl; m < M; m += 16 >> wl) {          // wl > 0: one row each at most
+            const E *row = (const E *)x + m * xs;
+            const int lead = (wave & ((1 << wl) - 1)) * 64 * VEC, c0 = lead + lane * VEC;
+            unsigned top = 0;
+            int c = c0;
+#pragma unroll 4
+            for (; c - lane * VEC + 64 * VEC <= K; c += step) {
+                vx_vec<SRC> v;
+                v.raw = vx_load16<SRC>(row + c);
+                top = vx_quant_look<SRC>(v, top);
+            }
+            if (c < K) top = vx_quant_look<SRC>(vx_load_vec<SRC>(row + c, K - c), top);
+            top = vx_wave_max(top);
+            if (wl) {
+                if (lane == 0) s_top[wave] = top;
+            } else {
+                quantise(row, m, c0, step, vx_quant_row(top));
+            }
+        }
+        if (wl) {
+            __syncthreads();
+            const int m = wave >> wl;
+            if (m < M) {
+                unsigned top = 0;
+                for (int i = 0; i < 1 << wl; ++i) top = max(top, s_top[(m << wl) + i]);
+                quantise((const E *)x + m * xs, m, ((wave & ((1 << wl) - 1)) * 64 + lane) * VEC, step, vx_quant_row(top));
+            }
+        }
+    }
+    __syncthreads();
+    auto put = [&](int m, long long n, int sum) {
+        const float y = vx_linear_out(sum, s_scale[m], sw[n], bias != nullptr, bias ? bias[n] : 0.f);
+        if (out_dtype == VX_DTYPE_F32) ((float *)out)[m * os + n] = y;
+        else if (out_dtype == VX_DTYPE_F16) ((_Float16 *)out)[m * os + n] = vx_store_cast<VX_DTYPE_F16>(y);
+        else ((__bf16 *)out)[m * os + n] = vx_store_cast<VX_DTYPE_BF16>(y);
+    };
+    int *s_sum = (int *)(s_few + M * pitch);
+    const int8_t *q[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) q[t] = s_few + min(t * 16 + (lane & 15), M - 1) * pitch + koff;
+    for (int first = slot; first < tiles; first += grid * CT, tile += grid * CT) {      // first: the tile of the first wave
+        const bool more = tile + grid * CT < tiles;
+        const int8_t *next = row_of(more ? tile + grid * CT : tiles - 1);
+        vx_i4 acc[MT] = {};
+        const long long n0 = (long long)tile * 16 + (lane >> 4) * 4;
+        float scale[4], plus[4];
+        if (KS == 1) {                                            // in front of the next tile's weights
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                scale[k] = sw[min(n0 + k, N - 1)];
+                plus[k] = bias ? bias[min(n0 + k, N - 1)] : 0.f;
+            }
+        }
+        if (tile < tiles) {
+            auto multiply = [&](const vx_i4 &weights, int at) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(weights, *(const vx_i4 *)(q[t] + at * 64), acc[t], 0, 0, 0);
+            };
+            int b = b0;
+            if (ahead) {
+                for (; b + 2 * UN <= end_full; b += UN) {
+#pragma unroll
+                    for (int u = 0; u < UN; ++u) {
+                        multiply(a[u], b + u);
+                        a[u] = load(wrow, b + UN + u);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < UN; ++u) {
+                    multiply(a[u], b + u);
+                    if (more) a[u] = load(next, b0 + u);
+                }
+                b += UN;
+            }
+            for (; b + 4 <= end_full; b += 4) {
+                vx_i4 v[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) v[u] = load(wrow, b + u);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) multiply(v[u], b + u);
+            }
+            for (; b < end_full; ++b) multiply(load(wrow, b), b);
+            if (b < end) {                                        // weights from K on meet zeros; those outside the matrix are not read
+                const int k = b * 64;
+                multiply(wrow + k + 16 <= w + (N - 1) * ws + K ? load(wrow, b) : vx_i8_tail(wrow, k, K - koff), b);
+            }
+        }
+        wrow = next;
+        // lane l holds token l % 16, channels 4 (l / 16) .. + 3
+        if (KS == 1) {
+            if (tile < tiles) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    const int m = t * 16 + (lane & 15);
+                    if (m >= M) continue;
+                    float y[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) y[k] = vx_linear_out(acc[t][k], s_scale[m], scale[k], bias != nullptr, plus[k]);
+                    if (out_dtype == VX_DTYPE_F32) vx_store4<VX_DTYPE_F32>(out, m * os + n0, y, N - n0);
+                    else if (out_dtype == VX_DTYPE_F16) vx_store4<VX_DTYPE_F16>(out, m * os + n0, y, N - n0);
+                    else vx_store4<VX_DTYPE_BF16>(out, m * os + n0, y, N - n0);
+                }
+            }
+        } else {
+            __syncthreads();                                      // the sums of the tiles before are read
+            if (tile < tiles) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t) *(vx_i4 *)&s_sum[(wave * MT + t) * 256 + (lane & 15) * 16 + (lane >> 4) * 4] = acc[t];
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < CT * MT * 256; i += 1024) {
+                const int c = i / (MT * 256), r = i - c * (MT * 256), m = r >> 4, at = first + grid * c;
+                const long long n = (long long)at * 16 + (r & 15);
+                if (m >= M || at >= tiles || n >= N) continue;
+                int sum = 0;
+                for (int k = 0; k < KS; ++k) sum += s_sum[((c << ks_log2) + k) * MT * 256 + r];
+                put(m, n, sum);
+            }
+        }
+    }
+}
+
+static int vx_few_ks(int64_t N) {                                 // log2 of the waves that share K: as many as leave none without a tile
+    const int64_t tiles = (N + 15) / 16;
+    int l = 0;
+    while (l < 4 && (tiles << (l + 1)) <= 256 * 16) ++l;
+    return l;
+}
+static size_t vx_few_lds(int64_t M, int64_t N, int K) {
+    return (size_t)M * (((K + 63) & ~63) + 16) + (vx_few_ks(N) ? (size_t)16 * ((M + 15) / 16) * 1024 : 0);
+}
+#define VX_FEW_MAX 64
+static bool vx_few_fits(int64_t M, int64_t N, int K) { return M <= VX_FEW_MAX && vx_few_lds(M, N, K) <= 160 * 1024 - 512; }
+// Which products with quantisation go this way (us in a graph, this / quantise and multiply; bf16): every workgroup quantises all
+// M x K values, which costs it what the saved launch cost at about 32768 of them (65536 where the tiles would copy an odd K):
+//   32000 x 4096, M = 4: 27/29, 8: 29/33    4096 x 4096, M = 4: 9/10, 8: 10/10, 16: 12/11    8192 x 8192, M = 4: 18/19, 8: 21/20
+//   131072 x 2048, M = 16: 56/59, 32: 63/62    1000 x 512, M = 64: 9/12    16384 x 1024, M = 32: 11/12, 64: 16/12
+//   50021 x 1000, M = 32: 18/29, 64: 25/38
+static bool vx_linear_by_few(int64_t M, int64_t N, int K) { return vx_few_fits(M, N, K) && M * K <= (K % 16 ? 65536 : 32768); }
+// Which products of quantised tokens: many channels, and few tokens or an odd K (this / streaming or tiles):
+//   32000 x 4096, M = 1: 26/26, 4: 25/26, 8: 26/29, 16: 26/31    131072 x 2048, M = 1: 49/45, 8: 50/56, 16: 54/55, 32: 58/57
+//   50021 x 1000, M = 4: 14/16, 16: 15/21, 37: 19/29, 64: 22/36    4096 x 4096, M = 8: 7/6.5    16384 x 1024, M = 16: 7/7
+static bool vx_i8_by_few(int64_t M, int64_t N, int K) { return M > 1 && N > 16384 && (M <= 16 || K % 16) && vx_few_fits(M, N, K); }
+
+template <int SRC>
+static void vx_few_launch(const void *x, long long xs, const float *s, int M, const int8_t *w, long long ws, const float *sw, long long N,
+                          int K, const float *bias, void *out, int out_dtype, long long os, hipStream_t st) {
+    const int tiles = (int)((N + 15) / 16), ks = vx_few_ks(N);
+    const dim3 grid((unsigned)min(tiles, 256));
+    const size_t lds = vx_few_lds(M, N, K);
+    if (M <= 16) hipLaunchKernelGGL((vx_k_linear_few<SRC, 1, 12>), grid, dim3(1024), lds, st, x, xs, s, M, w, ws, sw, N, K, bias, out, out_dtype, os, tiles, ks);
+    else if (M <= 32) hipLaunchKernelGGL((vx_k_linear_few<SRC, 2, 12>), grid, dim3(1024), lds, st, x, xs, s, M, w, ws, sw, N, K, bias, out, out_dtype, os, tiles, ks);
+    else if (M <= 48) hipLaunchKernelGGL((vx_k_linear_few<SRC, 3, 8>), grid, dim3(1024), lds, st, x, xs, s, M, w, ws, sw, N, K, bias, out, out_dtype, os, tiles, ks);
+    else hipLaunchKernelGGL((vx_k_linear_few<SRC, 4, 8>), grid, dim3(1024), lds, st, x, xs, s, M, w, ws, sw, N, K, bias, out, out_dtype, os, tiles, ks);
 }
 
 // ---- many tokens: TM x TN outputs for each workgroup, WM x WN waves of 32x32x32 mfma tiles (weights as rows, tokens as
@@ -746,7 +989,7 @@ __global__ __launch_bounds__(256) void vx_k_pad_rows(const int8_t *__restrict__ 
 //   of 256: 54 against 60 by 128; M = 1024, 128 tiles: 48 against 41.  8192 x 8192, M = 128, 64 tiles of 128: 43 against 33 by
 //   64; M = 512, 256 tiles: 47 against 58)
 static bool vx_linear_streams(int64_t M, int64_t N, int K) {
-    return M <= 8 || (M <= VX_STREAM_MAX && (N < 16384 || K % 16 != 0));
+    return vx_i8_by_few(M, N, K) || M <= 8 || (M <= VX_STREAM_MAX && (N < 16384 || K % 16 != 0));
 }
 
 static size_t vx_up256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -768,6 +1011,11 @@ static int vx_linear_launch(const int8_t *q, long long qs, bool q_padded, const 
     const long long pitch = vx_k_pitch(K);
     bool tiles = !vx_linear_streams(M, N, K);
     vx_prof_begin(VX_PROF_LINEAR, st);
+    if (vx_i8_by_few(M, N, K)) {
+        vx_few_launch<VX_SRC_I8>(q, qs, s, (int)M, w, ws, sw, N, K, bias, out, out_dtype, os, st);
+        vx_prof_end(VX_PROF_LINEAR, st);
+        return hipGetLastError() == hipSuccess ? VX_OK : VX_ERR_LAUNCH;
+    }
     if (tiles) {
         if (K % 128 && !q_padded) {
             const long long n = M * (pitch / 16);
@@ -861,6 +1109,12 @@ extern "C" int vx_linear_w8a8(const void *d_x, int x_dtype, int64_t x_stride, in
     hipStream_t st = (hipStream_t)stream;
     if (vx_linear_by_one(M, N, K))
         return vx_linear_one_launch(d_x, x_dtype, d_w, w_stride, d_w_scale, N, K, d_bias, d_out, out_dtype, st);
+    if (vx_linear_by_few(M, N, K)) {
+        vx_prof_begin(VX_PROF_LINEAR, st);
+        VX_DISPATCH_DTYPE(x_dtype, vx_few_launch<DT>(d_x, x_stride, nullptr, (int)M, d_w, w_stride, d_w_scale, N, K, d_bias, d_out, out_dtype, out_stride, st););
+        vx_prof_end(VX_PROF_LINEAR, st);
+        return hipGetLastError() == hipSuccess ? VX_OK : VX_ERR_LAUNCH;
+    }
     if (vx_linear_by_rows(M, N, K))
         return vx_linear_rows_launch(d_x, x_dtype, x_stride, M, d_w, w_stride, d_w_scale, (int)N, K, d_bias, d_out, out_dtype, out_stride, st);
     const long long pitch = vx_k_pitch(K);
