@@ -162,6 +162,30 @@ def test_embed_grad_accumulates_into_a_given_gradient(dt, ot):
     check_grad(got[~untouched.to(DEV)], ref[~untouched], err[~untouched])
 
 
+@pytest.mark.parametrize("T,Vr,D", [(1, 2, 1), (3, 7, 5), (40, 300, 8), (70, 140, 1027), (500, 1000, 1000), (501, 1001, 64), (16384, 32768, 40), (16384, 32767, 40),
+                                    (300, 40000, 2050), (129, 258, 4097)])
+@pytest.mark.parametrize("dt", TYPES)
+def test_embed_grad_of_few_tokens_clears_the_other_rows(T, Vr, D, dt):
+    """Up to half as many tokens as rows the table is cleared beside the sort: at any address, and nothing around it."""
+    lib, g = L.lib(), gen(T + Vr + D)
+    ids = zipf(T, Vr, g)
+    ids[0], ids[T // 2] = Vr - 1, -1
+    grad = torch.randn(T, D, generator=g).to(dt)
+    I, G = ids.to(DEV), grad.to(DEV)
+    code = {torch.float32: L.VX_DTYPE_F32, torch.float16: L.VX_DTYPE_F16, torch.bfloat16: L.VX_DTYPE_BF16}[dt]
+    nb = lib.vx_embed_tokens_grad_workspace_bytes(T, Vr, D)
+    ws = torch.empty(nb, dtype=torch.uint8, device=DEV)
+    ref, err = grad_ref(ids, grad, Vr, 0.5)
+    for lead in (0, 1, 5):
+        out = torch.full((lead + Vr * D + 9,), 7.0, dtype=dt, device=DEV)
+        rc = lib.vx_embed_tokens_grad(I.data_ptr(), 8, T, G.data_ptr(), code, Vr, D, 0.5, out.data_ptr() + lead * out.element_size(), code, 0, None,
+                                      ws.data_ptr(), nb, L.stream_ptr(DEV))
+        assert rc == 0
+        check_grad(out[lead:lead + Vr * D].view(Vr, D), ref, err)
+        assert bool((out[:lead] == 7).all()) and bool((out[lead + Vr * D:] == 7).all())
+    assert torch.equal(ops.embed_tokens_grad(I, G, Vr, 0.5), out[lead:lead + Vr * D].view(Vr, D))
+
+
 def test_embed_grad_keeps_nan_and_inf_in_their_rows():
     ids = torch.tensor([1, 2, 2, 3], device=DEV)
     grad = torch.ones(4, 9, device=DEV)

@@ -102,7 +102,8 @@ struct vx_cols {
 
 // Whether a result of `rows` rows of D values is written past the caches: more than the 32 MB of the chip's L2, so that none
 // of it would stay there, and rows of whole 128-byte lines.  Measured (ordinary / past the caches): lookup of 32768 x 4096 bf16
-// 73 / 63 us, gradient of 131072 x 4096 bf16 385 / 366, 32000 x 1024 fp32 40.8 / 39.0; rows of 2000 bytes 37 / 44.
+// 73 / 63 us, every row of a gradient of 131072 x 4096 bf16 385 / 366; rows of 2000 bytes 37 / 44.  (A pure fill is faster by
+// ordinary stores.)
 static inline bool vx_past_caches(const void *out, int64_t rows, int D, int dtype) {
     const int64_t row = (int64_t)D * vx_elem_size(dtype);
     return rows * row > (32 << 20) && row % 128 == 0 && ((uintptr_t)out & 127) == 0;

@@ -79,7 +79,8 @@ extern "C" int vx_embed_tokens(const void *d_ids, int id_bytes, int64_t n_tokens
 //    of 16 such chunks: a frequent token's row costs at most 30 rows of grad_out, 30 chunks and one row for each further
 //    256 tokens, instead of all its tokens on one wave (chunks of 32 / 16 / 8: 49 / 42 / 41 us at 2048 x 1024 fp32, whose end is
 //    the longest such chain, 380 / 383 / 394 at 65536 x 4096 bf16).
-// 3. Each table row is written once, from its chunks and the tokens at their ends.
+// 3. Each table row is written once, from its chunks and the tokens at their ends; or, with few tokens, the rows without any are
+//    cleared while the tokens are sorted.
 #define VX_EG_COUNT_MAX 16384     // tokens sorted by counting
 #define VX_EG_SUB 2048            // tokens one workgroup of the radix sort ranks at a time: 256 threads x 8
 #define VX_EG_TILES 256           // workgroups of a sorting pass at most
@@ -93,6 +94,15 @@ extern "C" int vx_embed_tokens(const void *d_ids, int id_bytes, int64_t n_tokens
 // 27 instead of 24 us at 2048 x 1024; 16-bit types with two: 33 instead of 24 us at 5001 x 1000 fp16, no gain at 4096 columns).
 #define VX_EG_SLICE 512
 template <int GT> __host__ __device__ constexpr int vx_eg_u() { return GT == VX_DTYPE_F32 ? 2 : 1; }
+
+// Which tables are cleared beside the sort and then written only where there are tokens (us, this / every row once):
+//   2048 x 32000 x 1024 fp32 34/39, 5001 x 50021 x 1000 fp16 27/37, 64 x 32000 24/30, 16000 x 32000 63/69, 2000 x 4096 23/23;
+//   as many tokens as rows 93/86; beyond the 256 MB of the last cache the zeros are still on their way when the rows come
+//   (16384 x 131072 x 4096 bf16 312/261, 5000 x 223/223, 2048 x 200/211).  Added to a given gradient: 2048 x 32000 20/24,
+//   16000 x 57/59, 65536 x 129/121.
+#define VX_EG_CLEAR_MAX (256LL << 20)
+#define VX_EG_CLEAR_BLOCKS 1024   // 512 / 2048: 35 / 34 instead of 34 us at 2048 x 32000 x 1024 fp32
+#define VX_EG_SPLIT 65536         // up to so many (token, slice) pairs there is a wave for each
 
 struct vx_eg_plan {
     int bits, passes, tiles;
@@ -128,6 +138,24 @@ static vx_eg_plan vx_eg_make_plan(int64_t T, int64_t n_rows, int D) {
     return p;
 }
 
+// Zeros for the table, written by the workgroups behind those that sort: `pieces` of 16 bytes at the aligned address `base`, and a
+// few elements (2 bytes each) in front of and behind them.  A contiguous range for each workgroup, ordinary stores: 131 MB in
+// 17.5 us (all workgroups side by side 21, past the caches 24).
+struct vx_eg_zero {
+    char *base;
+    long long pieces;
+    unsigned short *head, *tail;
+    int heads, tails;
+};
+__device__ __forceinline__ void vx_eg_fill(const vx_eg_zero &z, int block, int blocks) {
+    if (block == 0) {
+        if ((int)threadIdx.x < z.heads) z.head[threadIdx.x] = 0;
+        if ((int)threadIdx.x < z.tails) z.tail[threadIdx.x] = 0;
+    }
+    const long long per = (z.pieces + blocks - 1) / blocks, a = block * per, e = min(z.pieces, a + per);
+    for (long long i = a + threadIdx.x; i < e; i += blockDim.x) ((vx_v4 *)z.base)[i] = vx_v4{0.f, 0.f, 0.f, 0.f};
+}
+
 __device__ __forceinline__ unsigned vx_eg_key(const void *ids, int id_bytes, long long t, long long n_rows, int *status) {
     const long long id = vx_id_at(ids, id_bytes, t);
     if (id >= n_rows && status) atomicOr(status, VX_STATUS_BAD_TOKEN);
@@ -136,12 +164,13 @@ __device__ __forceinline__ unsigned vx_eg_key(const void *ids, int id_bytes, lon
 
 // Stable sort by counting: a workgroup places 64 tokens, one for each lane; its 16 waves share the scan of all keys, four
 // to an LDS read, a compare and an add-with-carry each.  Keys behind a token count when they are smaller, keys in front of
-// it also when they are equal.
+// it also when they are equal.  Workgroups from `own` on clear the table instead.
 __global__ __launch_bounds__(1024) void vx_k_eg_count_sort(const void *__restrict__ ids, int id_bytes, int T, long long n_rows,
                                                            unsigned *__restrict__ key_out, int *__restrict__ pos_out,
-                                                           int *__restrict__ status) {
+                                                           int *__restrict__ status, int own, vx_eg_zero zero) {
     __shared__ __attribute__((aligned(16))) unsigned s_key[VX_EG_COUNT_MAX];
     __shared__ int s_count[64];
+    if ((int)blockIdx.x >= own) { vx_eg_fill(zero, blockIdx.x - own, gridDim.x - own); return; }
     const int lane = vx_lane(), w = threadIdx.x >> 6;
     const int groups = (T + 3) >> 2;                              // of four keys
     for (int i = threadIdx.x; i < groups * 4; i += 1024)
@@ -381,82 +410,117 @@ __device__ __forceinline__ int vx_eg_lower_bound(const unsigned *__restrict__ ke
     return lo;
 }
 
-// Table rows blockIdx + i * gridDim (i < 8): frequent ids lie next to each other, so neighbours go to different workgroups.
-// A wave sums one slice of one row.  levels: of chunks (0, 1, 2).  Bound by the write of the table: few registers, so that
-// many waves have their loads and stores on the way (a version that split long rows over the waves of a workgroup held 94
-// instead of 62 registers: 292 instead of 265 us for the rows of 65536 tokens x 4096 columns bf16 over 131072).
+struct vx_eg_sums {                                               // what a table row is summed from
+    const unsigned *key;
+    const int *pos;
+    const void *grad;
+    long long pitch, n_rows;
+    const float *part1, *part2;
+    int T, D, slices, levels;                                     // levels: of chunks (0, 1, 2)
+    float scale;
+    void *out;
+    int accumulate;
+};
+
+// Columns c .. of row v from the sorted tokens s .. e - 1 and their chunks.
 template <int GT, int TT, int U, bool TINY, bool NT>
-__global__ __launch_bounds__(256) void vx_k_eg_rows(const unsigned *__restrict__ key, const int *__restrict__ pos, int T,
-                                                    const void *__restrict__ grad, long long n_rows, int D, int slices, float scale,
-                                                    void *__restrict__ out, int accumulate, int levels, long long pitch,
-                                                    const float *__restrict__ part1, const float *__restrict__ part2) {
+__device__ __forceinline__ void vx_eg_row(const vx_eg_sums &a, long long v, int s, int e, int c) {
     typedef typename vx_elem<GT>::type G;
     typedef typename vx_elem<TT>::type E;
     constexpr int VEC = 16 / sizeof(G);
+    const int D = a.D;
+    float sum[U * VEC] = {};
+    const int a1 = (s + VX_EG_CHUNK - 1) / VX_EG_CHUNK, b1 = e / VX_EG_CHUNK;
+    if (a.levels == 0 || a1 >= b1) {
+        vx_eg_add_tokens<GT, U, TINY>((const G *)a.grad, a.pos, s, e, D, c, sum);
+    } else {
+        vx_eg_add_tokens<GT, U, TINY>((const G *)a.grad, a.pos, s, a1 * VX_EG_CHUNK, D, c, sum);
+        const int a2 = (a1 + VX_EG_CHUNK - 1) / VX_EG_CHUNK, b2 = b1 / VX_EG_CHUNK;
+        if (a.levels == 1 || a2 >= b2) {
+            vx_eg_add_partials<GT, U>(a.part1, a1, b1, a.pitch, c, sum);
+        } else {
+            vx_eg_add_partials<GT, U>(a.part1, a1, (long long)a2 * VX_EG_CHUNK, a.pitch, c, sum);
+            vx_eg_add_partials<GT, U>(a.part2, a2, b2, a.pitch, c, sum);
+            vx_eg_add_partials<GT, U>(a.part1, (long long)b2 * VX_EG_CHUNK, b1, a.pitch, c, sum);
+        }
+        vx_eg_add_tokens<GT, U, TINY>((const G *)a.grad, a.pos, b1 * VX_EG_CHUNK, e, D, c, sum);
+    }
+    if (c >= D) return;
+    E *dst = (E *)a.out + v * D;
+#pragma unroll
+    for (int k = 0; k < U * VEC; ++k) sum[k] *= a.scale;
+    // columns at .. at + VEC of the sums, from c on to be stored; the table's pieces are VEC wide, or half of it where a
+    // 16-bit gradient is summed into fp32
+    constexpr int W = 16 / sizeof(E);
+#pragma unroll
+    for (int q = 0; q < U; ++q) {
+        const vx_cols<GT> col(c + q * 64 * VEC, D);
+        if (col.c >= D) continue;
+#pragma unroll
+        for (int k = 0; k < VEC; k += W) {
+            vx_cols<TT> part(0, D);
+            part.c = max(col.c, col.at + k);
+            part.at = col.at + k;
+            float *f = sum + q * VEC + k;
+            if (a.accumulate) {
+                vx_vec<TT> old;
+                if (!TINY) {
+                    old.raw = vx_load16<TT>(dst + part.at);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < W; ++j) old.e[j] = part.at + j < D ? dst[part.at + j] : (E)0.0f;
+                }
+#pragma unroll
+                for (int j = 0; j < W; ++j) f[j] = (float)old.e[j] + f[j];
+            }
+            part.template store<NT>(dst, f, D);
+        }
+    }
+}
+
+// Every table row: blockIdx + i * gridDim (i < 8), as frequent ids lie next to each other and go to different workgroups.
+// A wave sums one slice of one row.  Bound by the write of the table: few registers, so that many waves have their loads and
+// stores on the way (a version that split long rows over the waves of a workgroup held 94 instead of 62 registers: 292
+// instead of 265 us for the rows of 65536 tokens x 4096 columns bf16 over 131072).
+template <int GT, int TT, int U, bool TINY, bool NT>
+__global__ __launch_bounds__(256) void vx_k_eg_rows(vx_eg_sums a) {
+    constexpr int VEC = 16 / sizeof(typename vx_elem<GT>::type);
     __shared__ int s_at[2 * VX_EG_ROWS];
     const int lane = vx_lane(), w = threadIdx.x >> 6;
     {
         const int q = threadIdx.x >> 4;                           // 16 searches: the beginning and the end of 8 rows
         const long long v = blockIdx.x + (long long)(q >> 1) * gridDim.x + (q & 1);
-        const int at = vx_eg_lower_bound(key, T, (unsigned)min(v, n_rows));
+        const int at = vx_eg_lower_bound(a.key, a.T, (unsigned)min(v, a.n_rows));
         if ((lane & 15) == 0) s_at[q] = at;
     }
     __syncthreads();
-    auto finish = [&](long long v, int c, float *sum) {
-        E *dst = (E *)out + v * D;
-#pragma unroll
-        for (int k = 0; k < U * VEC; ++k) sum[k] *= scale;
-        // columns at .. at + VEC of the sums, from c on to be stored; the table's pieces are VEC wide, or half of it where a
-        // 16-bit gradient is summed into fp32
-        constexpr int W = 16 / sizeof(E);
-#pragma unroll
-        for (int q = 0; q < U; ++q) {
-            const vx_cols<GT> col(c + q * 64 * VEC, D);
-            if (col.c >= D) continue;
-#pragma unroll
-            for (int k = 0; k < VEC; k += W) {
-                vx_cols<TT> part(0, D);
-                part.c = max(col.c, col.at + k);
-                part.at = col.at + k;
-                float *f = sum + q * VEC + k;
-                if (accumulate) {
-                    vx_vec<TT> old;
-                    if (!TINY) {
-                        old.raw = vx_load16<TT>(dst + part.at);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < W; ++j) old.e[j] = part.at + j < D ? dst[part.at + j] : (E)0.0f;
-                    }
-#pragma unroll
-                    for (int j = 0; j < W; ++j) f[j] = (float)old.e[j] + f[j];
-                }
-                part.template store<NT>(dst, f, D);
-            }
-        }
-    };
-    for (int item = w; item < VX_EG_ROWS * slices; item += 4) {
-        const int i = item / slices, c = (item - i * slices) * VX_EG_SLICE + lane * VEC;
+    for (int item = w; item < VX_EG_ROWS * a.slices; item += 4) {
+        const int i = item / a.slices, c = (item - i * a.slices) * VX_EG_SLICE + lane * VEC;
         const long long v = blockIdx.x + (long long)i * gridDim.x;
         const int s = __builtin_amdgcn_readfirstlane(s_at[2 * i]), e = __builtin_amdgcn_readfirstlane(s_at[2 * i + 1]);
-        if (v >= n_rows || (accumulate && s == e)) continue;
-        float sum[U * VEC] = {};
-        const int a1 = (s + VX_EG_CHUNK - 1) / VX_EG_CHUNK, b1 = e / VX_EG_CHUNK;
-        if (levels == 0 || a1 >= b1) {
-            vx_eg_add_tokens<GT, U, TINY>((const G *)grad, pos, s, e, D, c, sum);
-        } else {
-            vx_eg_add_tokens<GT, U, TINY>((const G *)grad, pos, s, a1 * VX_EG_CHUNK, D, c, sum);
-            const int a2 = (a1 + VX_EG_CHUNK - 1) / VX_EG_CHUNK, b2 = b1 / VX_EG_CHUNK;
-            if (levels == 1 || a2 >= b2) {
-                vx_eg_add_partials<GT, U>(part1, a1, b1, pitch, c, sum);
-            } else {
-                vx_eg_add_partials<GT, U>(part1, a1, (long long)a2 * VX_EG_CHUNK, pitch, c, sum);
-                vx_eg_add_partials<GT, U>(part2, a2, b2, pitch, c, sum);
-                vx_eg_add_partials<GT, U>(part1, (long long)b2 * VX_EG_CHUNK, b1, pitch, c, sum);
-            }
-            vx_eg_add_tokens<GT, U, TINY>((const G *)grad, pos, b1 * VX_EG_CHUNK, e, D, c, sum);
-        }
-        if (c < D) finish(v, c, sum);
+        if (v >= a.n_rows || (a.accumulate && s == e)) continue;
+        vx_eg_row<GT, TT, U, TINY, NT>(a, v, s, e, c);
     }
+}
+
+// The rows that have tokens: one wave (or, with few tokens, one for each slice) where a sorted token's id differs from the one
+// before it.
+template <int GT, int TT, int U, bool TINY>
+__global__ __launch_bounds__(256) void vx_k_eg_runs(vx_eg_sums a, int split) {
+    constexpr int VEC = 16 / sizeof(typename vx_elem<GT>::type);
+    const int lane = vx_lane();
+    const long long item = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), s_ = item / split;
+    if (s_ >= a.T) return;
+    const int s = (int)s_, part = (int)(item - s_ * split);
+    const unsigned k = a.key[s];
+    if (k >= a.n_rows || (s > 0 && a.key[s - 1] == k)) return;
+    int e = s + 1;
+    while (true) {                                                // 64 tokens at a time as far as the id is the same
+        const u64 other = __ballot(e + lane >= a.T || a.key[min(e + lane, a.T - 1)] != k);
+        if (other) { e += __builtin_ctzll(other); break; }
+        e += 64;
+    }
+    for (int i = part; i < a.slices; i += split) vx_eg_row<GT, TT, U, TINY, false>(a, k, s, e, i * VX_EG_SLICE + lane * VEC);
 }
 
 extern "C" size_t vx_embed_tokens_grad_workspace_bytes(int64_t n_tokens, int64_t n_rows, int D) {
@@ -467,7 +531,7 @@ extern "C" size_t vx_embed_tokens_grad_workspace_bytes(int64_t n_tokens, int64_t
 // steps 2 and 3, once the tokens are sorted (key, pos)
 template <int GT, int TT, bool TINY>
 static void vx_eg_sum(const vx_eg_plan &p, const unsigned *key, const int *pos, int T, const void *grad, long long n_rows, int D,
-                      float scale, void *out, int accumulate, float *part1, float *part2, hipStream_t st) {
+                      float scale, void *out, int accumulate, bool runs, float *part1, float *part2, hipStream_t st) {
     constexpr int U = vx_eg_u<GT>();
     const int slices = (int)(p.pitch / VX_EG_SLICE), slices2 = (int)(p.pitch / 256);
     if (p.chunks)
@@ -476,14 +540,17 @@ static void vx_eg_sum(const vx_eg_plan &p, const unsigned *key, const int *pos, 
     if (p.chunks2)
         hipLaunchKernelGGL(vx_k_eg_chunks2, dim3((unsigned)(((int64_t)p.chunks2 * slices2 + 3) / 4)), dim3(256), 0, st, key, p.chunks2,
                            (unsigned)n_rows, slices2, p.pitch, part1, part2);
+    const vx_eg_sums a = {key, pos, grad, p.pitch, n_rows, part1, part2, T, D, slices, p.chunks2 ? 2 : (p.chunks ? 1 : 0), scale, out, accumulate};
+    if (runs) {
+        const int split = (int64_t)T * slices <= VX_EG_SPLIT ? slices : 1;
+        hipLaunchKernelGGL((vx_k_eg_runs<GT, TT, U, TINY>), dim3((unsigned)(((int64_t)T * split + 3) / 4)), dim3(256), 0, st, a, split);
+        return;
+    }
     const dim3 grid((unsigned)((n_rows + VX_EG_ROWS - 1) / VX_EG_ROWS));
-    const int levels = p.chunks2 ? 2 : (p.chunks ? 1 : 0);
     if (!TINY && !accumulate && vx_past_caches(out, n_rows, D, TT))
-        hipLaunchKernelGGL((vx_k_eg_rows<GT, TT, U, TINY, !TINY>), grid, dim3(256), 0, st, key, pos, T, grad, n_rows, D, slices, scale, out,
-                           accumulate, levels, p.pitch, part1, part2);
+        hipLaunchKernelGGL((vx_k_eg_rows<GT, TT, U, TINY, !TINY>), grid, dim3(256), 0, st, a);
     else
-        hipLaunchKernelGGL((vx_k_eg_rows<GT, TT, U, TINY, false>), grid, dim3(256), 0, st, key, pos, T, grad, n_rows, D, slices, scale, out,
-                           accumulate, levels, p.pitch, part1, part2);
+        hipLaunchKernelGGL((vx_k_eg_rows<GT, TT, U, TINY, false>), grid, dim3(256), 0, st, a);
 }
 
 extern "C" int vx_embed_tokens_grad(const void *d_ids, int id_bytes, int64_t n_tokens, const void *d_grad_out,
@@ -508,10 +575,23 @@ extern "C" int vx_embed_tokens_grad(const void *d_ids, int id_bytes, int64_t n_t
     float *part1 = (float *)(ws + p.part1), *part2 = (float *)(ws + p.part2);
     hipStream_t st = (hipStream_t)stream;
     vx_prof_begin(VX_PROF_EMBED_GRAD, st);
+    const int es = vx_elem_size(table_dtype);
+    const int64_t bytes = n_rows * D * es;
+    const bool runs = T <= VX_EG_COUNT_MAX && 2 * n_tokens <= n_rows && (accumulate || bytes <= VX_EG_CLEAR_MAX || 64 * n_tokens <= n_rows);
     int at = 0;                                                   // the buffers that hold the sorted tokens
     if (T <= VX_EG_COUNT_MAX) {
-        hipLaunchKernelGGL(vx_k_eg_count_sort, dim3((T + 63) / 64), dim3(1024), 0, st, d_ids, id_bytes, T, (long long)n_rows, key[0],
-                           pos[0], d_status);
+        vx_eg_zero z = {};
+        int own = (T + 63) / 64, clear = 0;
+        if (runs && !accumulate) {
+            char *const first = (char *)d_grad_table, *const last = first + bytes;
+            char *const base = (char *)(((uintptr_t)first + 15) & ~(uintptr_t)15), *const mid = base < last ? base : last;
+            const int64_t pieces = (last - mid) / 16;
+            z = vx_eg_zero{mid, pieces, (unsigned short *)first, (unsigned short *)(mid + pieces * 16), (int)((mid - first) / 2),
+                           (int)((last - mid - pieces * 16) / 2)};
+            clear = (int)min((int64_t)VX_EG_CLEAR_BLOCKS, pieces / 1024 + 1);
+        }
+        hipLaunchKernelGGL(vx_k_eg_count_sort, dim3(own + clear), dim3(1024), 0, st, d_ids, id_bytes, T, (long long)n_rows, key[0],
+                           pos[0], d_status, own, z);
     } else {
         for (int i = 0; i < p.passes; ++i) {
             at = i & 1;
@@ -523,12 +603,12 @@ extern "C" int vx_embed_tokens_grad(const void *d_ids, int id_bytes, int64_t n_t
     }
     VX_DISPATCH_DTYPE(grad_dtype, {
         if (D < 16 / vx_elem_size(DT)) {
-            if (table_dtype == DT) vx_eg_sum<DT, DT, true>(p, key[at], pos[at], T, d_grad_out, n_rows, D, scale, d_grad_table, accumulate, part1, part2, st);
-            else vx_eg_sum<DT, VX_DTYPE_F32, true>(p, key[at], pos[at], T, d_grad_out, n_rows, D, scale, d_grad_table, accumulate, part1,
+            if (table_dtype == DT) vx_eg_sum<DT, DT, true>(p, key[at], pos[at], T, d_grad_out, n_rows, D, scale, d_grad_table, accumulate, runs, part1, part2, st);
+            else vx_eg_sum<DT, VX_DTYPE_F32, true>(p, key[at], pos[at], T, d_grad_out, n_rows, D, scale, d_grad_table, accumulate, runs, part1,
                                                     part2, st);
         } else {
-            if (table_dtype == DT) vx_eg_sum<DT, DT, false>(p, key[at], pos[at], T, d_grad_out, n_rows, D, scale, d_grad_table, accumulate, part1, part2, st);
-            else vx_eg_sum<DT, VX_DTYPE_F32, false>(p, key[at], pos[at], T, d_grad_out, n_rows, D, scale, d_grad_table, accumulate, part1,
+            if (table_dtype == DT) vx_eg_sum<DT, DT, false>(p, key[at], pos[at], T, d_grad_out, n_rows, D, scale, d_grad_table, accumulate, runs, part1, part2, st);
+            else vx_eg_sum<DT, VX_DTYPE_F32, false>(p, key[at], pos[at], T, d_grad_out, n_rows, D, scale, d_grad_table, accumulate, runs, part1,
                                                      part2, st);
         }
     });
