@@ -186,6 +186,16 @@ def test_embed_grad_of_few_tokens_clears_the_other_rows(T, Vr, D, dt):
     assert torch.equal(ops.embed_tokens_grad(I, G, Vr, 0.5), out[lead:lead + Vr * D].view(Vr, D))
 
 
+@pytest.mark.parametrize("T,Vr", [(10, 40), (30, 40), (20000, 70000)])
+def test_embed_grad_rows_without_tokens_are_zero_at_any_scale(T, Vr):
+    ids = torch.arange(T, device=DEV) % (Vr // 2)
+    for scale in (float("inf"), float("nan"), -1.0):
+        got = ops.embed_tokens_grad(ids, torch.ones(T, 24, device=DEV), Vr, scale)
+        n = min(T, Vr // 2)
+        assert not got[n:].any() and not got[n:].isnan().any()
+        assert not got[:n].isfinite().any() if scale != -1.0 else bool((got[:n] < 0).all())
+
+
 def test_embed_grad_keeps_nan_and_inf_in_their_rows():
     ids = torch.tensor([1, 2, 2, 3], device=DEV)
     grad = torch.ones(4, 9, device=DEV)

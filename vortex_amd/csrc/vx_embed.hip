@@ -447,8 +447,9 @@ __device__ __forceinline__ void vx_eg_row(const vx_eg_sums &a, long long v, int 
     }
     if (c >= D) return;
     E *dst = (E *)a.out + v * D;
+    const float scale = s == e ? 0.f : a.scale;                   // zeros without a token, whatever the scale
 #pragma unroll
-    for (int k = 0; k < U * VEC; ++k) sum[k] *= a.scale;
+    for (int k = 0; k < U * VEC; ++k) sum[k] *= scale;
     // columns at .. at + VEC of the sums, from c on to be stored; the table's pieces are VEC wide, or half of it where a
     // 16-bit gradient is summed into fp32
     constexpr int W = 16 / sizeof(E);
