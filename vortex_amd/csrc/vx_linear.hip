@@ -980,16 +980,18 @@ __global__ __launch_bounds__(256) void vx_k_pad_rows(const int8_t *__restrict__ 
     *(vx_i4 *)(dst + r * pitch + k) = k + 16 <= K ? (vx_i4)*(const vx_i4_at1 *)(row + k) : vx_i8_tail(row, k, K);
 }
 
-// Which kernel takes M tokens (us of the product alone; N x K, weights from memory):
-//   M <= 8: streaming (32000 x 4096: 30 against 33 by 64 x 64 tiles; at M = 16 36 against 33)
-//   M <= 64: streaming with few channels or an odd K, which the tiles would have to copy (8192 x 8192, M = 32: 27 against 30;
-//            50021 x 1000, M = 37: 23), 64 x 64 tiles from 16384 channels on (32000 x 4096, M = 32: 33 against 43)
+// Which kernel takes M tokens (us of the product alone; N x K, weights from memory), streaming / 64 x 64 tiles:
+//   M <= 8: streaming (32000 x 4096: 30/33)
+//   M <= 16: streaming up to 16384 channels (4096 x 4096 7/12, 12000 x 2048 8.4/8.7, 16000 x 4096 18/20)
+//   M <= 32: streaming up to 10240 channels (M = 32: 4096 x 4096 11/13, 8192 x 4096 13/17, but 12000 x 2048 11/9, 16000 x 4096 23/20;
+//            M = 64: 4096 x 4096 16/13, 8192 x 1024 9/7, 8192 x 4096 17/17, 8192 x 8192 30/32)
+//   M <= 64: streaming with an odd K, which the tiles would have to copy
 //   more: the largest tile that is at least half full of tokens and gives at least 192 workgroups, three for four compute
 //   units (32000 x 4096, M = 64: 34 by 64 against 37 by 128; M = 96: 44 against 38.  8192 x 4096: M = 1536, 192 tiles
 //   of 256: 54 against 60 by 128; M = 1024, 128 tiles: 48 against 41.  8192 x 8192, M = 128, 64 tiles of 128: 43 against 33 by
 //   64; M = 512, 256 tiles: 47 against 58)
 static bool vx_linear_streams(int64_t M, int64_t N, int K) {
-    return vx_i8_by_few(M, N, K) || M <= 8 || (M <= VX_STREAM_MAX && (N < 16384 || K % 16 != 0));
+    return vx_i8_by_few(M, N, K) || M <= 8 || (M <= 16 && N <= 16384) || (M <= 32 && N <= 10240) || (M <= VX_STREAM_MAX && K % 16);
 }
 
 static size_t vx_up256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -1041,10 +1043,10 @@ static int vx_linear_launch(const int8_t *q, long long qs, bool q_padded, const 
             else vx_linear_tiles<DT, 64, 2, 2>(q, qs, s, M, w, ws, sw, N, K, bias, out, os, st);
         });
     } else {
-        // two tiles of channels share the tokens' loads where there is more than one tile of tokens (37 x 50021 x 1000: 30 ->
-        // 23 us with two waves); few channels: more waves side by side along K
+        // two tiles of channels share the tokens' loads where there is more than one tile of tokens, and eight waves their K
+        // (16000 x 2048, M = 32: 13 us, two / four waves 16 / 14); one tile: four waves, or 16 with few channels
         const int mt = (int)min(4LL, (M + 15) / 16), nt = mt == 1 ? 1 : 2;
-        const int waves = N <= 4096 ? 16 / nt : (K <= 2048 && mt > 1 ? 2 : 4);
+        const int waves = mt > 1 ? 8 : (N <= 4096 ? 16 : 4);
         const dim3 grid((unsigned)((N + 16 * nt - 1) / (16 * nt)), (unsigned)((M + 16 * mt - 1) / (16 * mt)));
         const size_t lds = (size_t)waves * mt * nt * 1024;
         VX_DISPATCH_DTYPE(out_dtype, {
