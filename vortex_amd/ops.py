@@ -459,7 +459,7 @@ def embed_tokens(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
         _bad("table is empty: %s", tuple(table.shape))
     st = None if status is None else _status_word(status, dev)
     ids, table = ids.contiguous(), _rows(table)
-    out = torch.empty(ids.shape + (D,), dtype=table.dtype, device=dev)
+    out = torch.empty(*ids.shape, D, dtype=table.dtype, device=dev)      # sizes one by one: a torch.Size takes 2 us to unpack
     T = ids.numel()
     if T:
         rc = L.lib().vx_embed_tokens(ids.data_ptr(), ids.element_size(), T, table.data_ptr(), V, D, _row_stride(table),
@@ -492,7 +492,7 @@ def embed_tokens_grad(ids: torch.Tensor, grad_out: torch.Tensor, n_rows: int, sc
     if T == 0:
         return out if accumulate else torch.zeros((n_rows, D), dtype=grad_out.dtype, device=dev)
     if not accumulate:
-        out = torch.empty((n_rows, D), dtype=grad_out.dtype, device=dev)
+        out = torch.empty(n_rows, D, dtype=grad_out.dtype, device=dev)
     ids, grad_out = ids.contiguous(), grad_out.contiguous()
     lib = L.lib()
     nb = lib.vx_embed_tokens_grad_workspace_bytes(T, n_rows, D)
@@ -517,7 +517,7 @@ def quantize_rows_i8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     _tensor(x, "input", None, _DTYPES)
     K, lead, dev = _last_dim(x, "input"), x.shape[:-1], x.device
     M = x.numel() // K
-    q = torch.empty(x.shape, dtype=torch.int8, device=dev)
+    q = torch.empty(*x.shape, dtype=torch.int8, device=dev)
     s = torch.empty(lead, dtype=torch.float32, device=dev)
     if M:
         x = _rows(x if x.dim() == 2 else x.reshape(M, K))
@@ -563,7 +563,7 @@ def linear_i8(q: torch.Tensor, scale: torch.Tensor, qw: torch.Tensor, w_scale: t
         _bad("out_dtype %s: expected one of %s", out_dtype, [str(d) for d in _DTYPES])
     qw, w_scale, bias, N = _linear_weights(qw, w_scale, bias, K, dev)
     M = q.numel() // K
-    out = torch.empty(lead + (N,), dtype=out_dtype, device=dev)
+    out = torch.empty(*lead, N, dtype=out_dtype, device=dev)
     if M:
         lib = L.lib()
         q, scale = _rows(q if q.dim() == 2 else q.reshape(M, K)), scale.contiguous()
@@ -590,7 +590,7 @@ def linear_w8a8(x: torch.Tensor, qw: torch.Tensor, w_scale: torch.Tensor, bias: 
     K, lead = _last_dim(x, "input"), x.shape[:-1]
     qw, w_scale, bias, N = _linear_weights(qw, w_scale, bias, K, dev)
     M = x.numel() // K
-    out = torch.empty(lead + (N,), dtype=out_dtype, device=dev)
+    out = torch.empty(*lead, N, dtype=out_dtype, device=dev)
     if M:
         lib = L.lib()
         x = _rows(x if x.dim() == 2 else x.reshape(M, K))
@@ -649,10 +649,10 @@ def verify_drafts(target_logits: torch.Tensor, draft_tokens: torch.Tensor, unifo
         if not t_all >= 0.0:
             _bad("temperature must not be negative, got %s", t_all)
     draft_tokens, uniforms = draft_tokens.contiguous(), uniforms.contiguous()
-    tokens = torch.empty((B, K1), dtype=torch.int64, device=dev)
-    accept = torch.empty((B, K), dtype=torch.float32, device=dev)
-    counts = torch.empty((B,), dtype=torch.int32, device=dev)
-    status = torch.empty((B,), dtype=torch.int32, device=dev)
+    tokens = torch.empty(B, K1, dtype=torch.int64, device=dev)
+    accept = torch.empty(B, K, dtype=torch.float32, device=dev)
+    counts = torch.empty(B, dtype=torch.int32, device=dev)
+    status = torch.empty(B, dtype=torch.int32, device=dev)
     if B:
         lib = L.lib()
         nb = lib.vx_verify_drafts_workspace_bytes(B, K, V)
