@@ -352,8 +352,10 @@ struct vx_pick_smem {
     int first, last;
 };
 
-// Thread t holds the weight `sum` of the t-th of up to 256 parts: the first part at which the running weight, from `base`
-// on, passes `goal`, and the weight in front of it; -1 where none does.  `last`: the last part with a weight (-1: none).
+// Thread t holds the weight `sum` of the t-th of up to 256 parts: the first part with a weight at which the running weight, from
+// `base` on, passes `goal`, and the weight in front of it; -1 where none does.  `last`: the last part with a weight (-1: none).
+// Each running weight has its own order of additions, so one may pass that only adds nothing to the one before it, which did not:
+// parts without a weight are never taken.
 __device__ __forceinline__ int vx_pick_part(double sum, double base, double goal, vx_pick_smem &S, double &before, int &last) {
     const int lane = vx_lane(), w = threadIdx.x >> 6;
     double run = sum;
@@ -370,7 +372,7 @@ __device__ __forceinline__ int vx_pick_part(double sum, double base, double goal
     for (int i = 0; i < w; ++i) front += S.run[i];
     run += front;
     const double prev = __shfl_up(run, 1, VX_WAVE);
-    const u64 passed = __ballot(run > goal), any = __ballot(sum > 0.0);
+    const u64 passed = __ballot(run > goal && sum > 0.0), any = __ballot(sum > 0.0);
     if (lane == 0) {
         if (passed) atomicMin(&S.first, w * 64 + __builtin_ctzll(passed));
         if (any) atomicMax(&S.last, w * 64 + 63 - __builtin_clzll(any));
@@ -403,7 +405,8 @@ __device__ __forceinline__ int vx_verify_pick(int runs, int V, float u, S sums, 
         int c = -1;
         for (int k = part * per; k < min(runs, (part + 1) * per); ++k) {
             const double v = sums(k);
-            if (v > 0.0) c = k;
+            if (!(v > 0.0)) continue;
+            c = k;
             if (before + v > goal) break;
             before += v;
         }
