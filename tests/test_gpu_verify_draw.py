@@ -50,3 +50,25 @@ def test_running_sums_that_pass_the_border_at_a_masked_run(dt):
     target[0, 0, at] = torch.tensor([-37.0, -37.0, 0.0, 0.0])
     tok = ops.verify_drafts(target.to(dt).to(DEV), torch.zeros(1, 0, dtype=torch.int64, device=DEV), torch.full((1, 1), 0.5, device=DEV))[0]
     assert tok.item() in at[2:]
+
+
+@pytest.mark.parametrize("rejected", [False, True])
+@pytest.mark.parametrize("u_last", [1.0, float("inf"), float("nan")])
+@pytest.mark.parametrize("dt,Vn", [(torch.float32, 5000), (torch.float32, 50021), (torch.bfloat16, 32000), (torch.float16, 131072)])
+def test_uniforms_of_one_and_above_draw_the_last_token_with_weight(dt, Vn, u_last, rejected):
+    target, draft, tokens, w = random_rows(dt, Vn, 0.7, rejected, Vn + 1)
+    u = torch.ones(target.size(0), 1 + rejected)
+    u[:, -1] = u_last
+    tok = ops.verify_drafts(target.to(DEV), tokens.to(DEV), u.to(DEV), draft.to(DEV) if rejected else None)[0]
+    assert tok[:, 0].tolist() == [int(np.nonzero(r)[0][-1]) for r in w]
+
+
+@pytest.mark.parametrize("u", [1.0, 2.0, float("nan")])
+@pytest.mark.parametrize("dt", TYPES)
+def test_a_uniform_of_one_is_behind_every_running_sum(dt, u):
+    """Weights 0.77 h, 0.77 h, 1, 7e-4 h, 7e-4 h: the sum of all is 1 in its own order, the running sum is 1 + 2 h at the fourth."""
+    run = RUN[dt]
+    target = torch.full((1, 1, 5 * run + 100), -float("inf"))
+    target[0, 0, [3, run + 5, 2 * run + 77, 3 * run + 9, 4 * run + 1]] = torch.tensor([-37.0, -37.0, 0.0, -44.0, -44.0])
+    tok = ops.verify_drafts(target.to(dt).to(DEV), torch.zeros(1, 0, dtype=torch.int64, device=DEV), torch.full((1, 1), u, device=DEV))[0]
+    assert tok.item() == 4 * run + 1

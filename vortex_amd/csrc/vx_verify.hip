@@ -396,10 +396,11 @@ __device__ __forceinline__ int vx_verify_pick(int runs, int V, float u, S sums, 
     double mine = 0.0, before;
     int last;
     for (int k = tid * per; k < min(runs, (tid + 1) * per); ++k) mine += sums(k);
-    double goal = (double)u * vx_verify_sum(mine, s_sum);
+    // a uniform of 1 and above (or NaN) is behind all running sums, whatever they are rounded to
+    double goal = u < 1.f ? (double)u * vx_verify_sum(mine, s_sum) : INFINITY;
     int part = vx_pick_part(mine, 0.0, goal, sm, before, last);
     if (last < 0) return -1;
-    if (part < 0) { part = last; goal = INFINITY; before = 0.0; } // a uniform of 1, or rounding
+    if (part < 0) { part = last; goal = INFINITY; before = 0.0; }
     int run = part * per;
     if (per > 1) {                                                // more than 256 runs: on through this thread's
         int c = -1;
