@@ -72,3 +72,19 @@ def test_a_uniform_of_one_is_behind_every_running_sum(dt, u):
     target[0, 0, [3, run + 5, 2 * run + 77, 3 * run + 9, 4 * run + 1]] = torch.tensor([-37.0, -37.0, 0.0, -44.0, -44.0])
     tok = ops.verify_drafts(target.to(dt).to(DEV), torch.zeros(1, 0, dtype=torch.int64, device=DEV), torch.full((1, 1), u, device=DEV))[0]
     assert tok.item() == 4 * run + 1
+
+
+@pytest.mark.parametrize("dt,Vn", [(torch.float32, 400000), (torch.float16, 800000)])
+def test_two_runs_a_thread_and_no_running_sum_that_passes(dt, Vn):
+    """From 257 runs on a thread has two.  Weights 1 | v, (a, b) | 1 at three threads with v = 0.496 h, a = 1.018 h, b = 1.787 h, the
+    uniform one half: the sum of all is rounded to 2 + 4 h, so the border is 1 + 2 h, which the second thread passes as a whole
+    (1 + 3.3 h: 1 + 4 h) and run by run does not (1 + v: 1, and 2.8 h more: 1 + 2 h).  The token is then the thread's last, b; it
+    is in exact arithmetic too (v + a < (v + a + b) / 2)."""
+    run = RUN[dt]
+    target = torch.full((1, 1, Vn), -float("inf"))
+    at = [5, 2 * run + 40, 3 * run + 300, 3 * run + 700, 4 * run + 9]
+    target[0, 0, at] = torch.tensor([0.0, -37.4375, -36.71875, -36.15625, 0.0])
+    w = np.exp(np.array([-37.4375, -36.71875, -36.15625])) * 2.0 ** 53
+    assert 256 * run < Vn < 512 * run and w[1] > 1 and w[0] < 1 and w[1] + w[2] < 3 < w.sum() < 5 and 2 * (w[0] + w[1]) < w.sum()
+    tok = ops.verify_drafts(target.to(dt).to(DEV), torch.zeros(1, 0, dtype=torch.int64, device=DEV), torch.full((1, 1), 0.5, device=DEV))[0]
+    assert tok.item() == at[3]

@@ -403,15 +403,15 @@ __device__ __forceinline__ int vx_verify_pick(int runs, int V, float u, S sums, 
     if (part < 0) { part = last; goal = INFINITY; before = 0.0; }
     int run = part * per;
     if (per > 1) {                                                // more than 256 runs: on through this thread's
-        int c = -1;
-        for (int k = part * per; k < min(runs, (part + 1) * per); ++k) {
+        bool passed = false;
+        for (int k = part * per; k < min(runs, (part + 1) * per) && !passed; ++k) {
             const double v = sums(k);
             if (!(v > 0.0)) continue;
-            c = k;
-            if (before + v > goal) break;
-            before += v;
+            run = k;
+            passed = before + v > goal;
+            if (!passed) before += v;
         }
-        run = c < 0 ? run : c;
+        if (!passed) goal = INFINITY;                             // rounding: `before` holds the last run already
     }
     mine = part_weight(run * RUN + tid * PART);
     part = vx_pick_part(mine, before, goal, sm, before, last);
