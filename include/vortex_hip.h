@@ -393,7 +393,8 @@ int vx_linear_w8a8(const void *d_x, int x_dtype, int64_t x_stride, int64_t M, co
  * draws the last token with r > 0.
  * -inf masks a token (in either distribution); other logits of a row differ by less than FLT_MAX.  K = 0 draws one token from
  * each row 0.
- * The drawn token and every accepted / rejected are decided in fp64 from the logits on; d_accept is within 2^-15 relative.
+ * The drawn token and every accepted / rejected are decided in fp64 from the logits on; d_accept is within 2^-15 relative, and
+ * rounded from the fp64 quotient for a draft that is decided next to the border (so it is never on the other side of u_{b,j}).
  * d_status[b] (written, not ORed): VX_STATUS_NAN a NaN or +inf in a row that is used,
  * VX_STATUS_EMPTY_ROW all of such a row is -inf, VX_STATUS_BAD_TOKEN a drafted token outside [0, V) (it is rejected).  A
  * draft is rejected at an invalid row; where the row that is drawn from is invalid, the token behind is -1.

@@ -275,7 +275,8 @@ __global__ __launch_bounds__(256) void vx_k_verify_choose(vx_verify_args a) {
     }
     __syncthreads();
     auto invalid = [](float m) { return m != m ? VX_STATUS_NAN : (m == -INFINITY ? VX_STATUS_EMPTY_ROW : 0); };
-    double ratio = 0.0, p = 0.0, uq = 0.0;
+    double ratio = 0.0, p = 0.0, q = 1.0;
+    auto accept = [&] { return p >= q ? (p > 0.0 ? 1.0 : 0.0) : p / q; };
     int st = 0;
     if (w == 0) {
         bool ok = false, unsure = false;
@@ -288,11 +289,11 @@ __global__ __launch_bounds__(256) void vx_k_verify_choose(vx_verify_args a) {
                     ratio = ok ? 1.0 : 0.0;
                 } else {
                     p = vx_weight(tx, s_m[lane], c) / s_z[lane];
-                    const double q = has_q ? vx_weight(dx, s_m[VX_MAX_DRAFTS + 1 + lane], c) / s_z[VX_MAX_DRAFTS + 1 + lane] : 1.0;
-                    uq = (double)un * q;
+                    if (has_q) q = vx_weight(dx, s_m[VX_MAX_DRAFTS + 1 + lane], c) / s_z[VX_MAX_DRAFTS + 1 + lane];
+                    const double uq = (double)un * q;
                     ok = uq < p;
                     unsure = p > 0.0 && fabs(uq - p) <= p * ((42.0 + 4.2 * (32 - __clz(a.V))) * 0x1p-24);
-                    ratio = p >= q ? (p > 0.0 ? 1.0 : 0.0) : p / q;
+                    ratio = accept();
                 }
             }
         }
@@ -311,10 +312,11 @@ __global__ __launch_bounds__(256) void vx_k_verify_choose(vx_verify_args a) {
             for (int k = 0; k < a.chunks; ++k) zq += vx_verify_chunk_sum<DT>(vx_verify_draft<DT>(a, b, j), k, a.V, s_m[VX_MAX_DRAFTS + 1 + j], c);
         zp = vx_verify_sum(zp, s_sum);
         zq = vx_verify_sum(zq, s_sum);
-        if (threadIdx.x == j) {                                   // p and u q from the exact sums
+        if (threadIdx.x == j) {                                   // p and q from the exact sums
             p = p * s_z[j] / zp;
-            if (has_q) uq = uq * s_z[VX_MAX_DRAFTS + 1 + j] / zq;
-            s_ok = uq < p ? s_ok | (1ull << j) : s_ok & ~(1ull << j);
+            if (has_q) q = q * s_z[VX_MAX_DRAFTS + 1 + j] / zq;
+            s_ok = (double)un * q < p ? s_ok | (1ull << j) : s_ok & ~(1ull << j);
+            ratio = accept();
         }
         __syncthreads();
     }
