@@ -1,0 +1,27 @@
+"""Token-model operators at sizes whose launches have more than 2^24 workgroups: HIP takes fewer than 2^32 threads along an axis."""
+import pytest
+import torch
+
+from test_gpu_tokens import DEV, gen
+from vortex_amd import _lib as L
+from vortex_amd import ops
+
+pytestmark = pytest.mark.gpu
+MANY = 2 ** 26 + 5                              # tokens: one wave each, four to a workgroup
+
+
+@pytest.mark.parametrize("dt,D", [(torch.float32, 1), (torch.bfloat16, 8)])
+def test_embed_more_tokens_than_one_axis_of_a_launch(dt, D):
+    Vr = 100003
+    table = torch.randn(Vr, D, generator=gen(D)).to(dt).to(DEV)
+    ids = (torch.arange(MANY, device=DEV, dtype=torch.int32) * 7919) % Vr        # wraps around below 0 now and then: padding
+    ids[-1] = Vr - 1
+    st = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got = ops.embed_tokens(ids, table, 2.0, status=st)
+    for a in range(0, MANY, 1 << 24):
+        i = ids[a:a + (1 << 24)].long()
+        ref = torch.where((i >= 0)[:, None], table[i.clamp_min(0)] * 2.0, torch.zeros((), dtype=dt, device=DEV))
+        assert torch.equal(got[a:a + (1 << 24)], ref), a
+    assert int(st) == 0
+    ids[-1] = Vr
+    assert not ops.embed_tokens(ids, table, 2.0, status=st)[-1].any() and int(st) == L.VX_STATUS_BAD_TOKEN

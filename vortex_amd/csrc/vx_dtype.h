@@ -19,6 +19,15 @@ static inline bool vx_dtype_ok(int dtype) { return dtype == VX_DTYPE_F32 || dtyp
         else { constexpr int DT = VX_DTYPE_BF16; __VA_ARGS__; }                \
     } while (0)
 
+// A launch of `blocks` workgroups and the number of one.  HIP takes fewer than 2^32 threads along an axis, and drops the others
+// without an error: beyond 2^21 workgroups (of up to 1024 threads) they are laid out along two axes, in the same order.  The last
+// of the second axis may be numbers from `blocks` on: the kernels have nothing to do there.
+static inline dim3 vx_grid(int64_t blocks) {
+    const int64_t y = (blocks + (1 << 21) - 1) >> 21;
+    return dim3((unsigned)((blocks + y - 1) / y), (unsigned)y);
+}
+__device__ __forceinline__ unsigned vx_block() { return blockIdx.y * gridDim.x + blockIdx.x; }
+
 // fp32 -> the stored type, to nearest even.  The empty asm keeps the fp32 value as computed: hipcc otherwise folds a product
 // and its conversion to fp16 into one instruction that skips the fp32 rounding, and the same operator would then round
 // differently in its three types.

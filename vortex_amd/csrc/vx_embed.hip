@@ -17,7 +17,7 @@ __global__ __launch_bounds__(256) void vx_k_embed(const void *__restrict__ ids, 
                                                   int *__restrict__ status) {
     typedef typename vx_elem<DT>::type E;
     constexpr int VEC = 16 / sizeof(E);
-    const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const long long item = (long long)vx_block() * 4 + (threadIdx.x >> 6);
     if (item >= T * slices) return;
     const long long t = item / slices;
     const int slice = (int)(item - t * slices), lane = vx_lane();
@@ -57,7 +57,7 @@ extern "C" int vx_embed_tokens(const void *d_ids, int id_bytes, int64_t n_tokens
     if (blocks > 2147483647LL) return VX_ERR_UNSUPPORTED;
     vx_prof_begin(VX_PROF_EMBED, st);
 #define VX_EMBED_GO(...)                                                                                                       \
-    hipLaunchKernelGGL((vx_k_embed<__VA_ARGS__>), dim3((unsigned)blocks), dim3(256), 0, st, d_ids, id_bytes, (long long)n_tokens, d_table, \
+    hipLaunchKernelGGL((vx_k_embed<__VA_ARGS__>), vx_grid(blocks), dim3(256), 0, st, d_ids, id_bytes, (long long)n_tokens, d_table, \
                        (long long)n_rows, D, slices, (long long)table_stride, scale, d_out, d_status)
     VX_DISPATCH_DTYPE(dtype, {
         if (D < vec) VX_EMBED_GO(DT, 1, true, false);
