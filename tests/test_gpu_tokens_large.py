@@ -25,3 +25,16 @@ def test_embed_more_tokens_than_one_axis_of_a_launch(dt, D):
     assert int(st) == 0
     ids[-1] = Vr
     assert not ops.embed_tokens(ids, table, 2.0, status=st)[-1].any() and int(st) == L.VX_STATUS_BAD_TOKEN
+
+
+@pytest.mark.parametrize("D", [1, 4])
+def test_embed_grad_of_more_rows_than_one_axis_of_a_launch(D):
+    """2^27 table rows and more, eight to a workgroup.  Whole numbers below 2^24: fp32 sums are exact."""
+    T, Vr = 20000, 2 ** 27 + 9
+    ids = torch.randint(0, Vr, (T,), generator=gen(D)).to(DEV)
+    ids[:3000], ids[3000:4000], ids[4000] = Vr - 1, 2 ** 26 + 1, 0
+    grad = torch.randint(-8, 9, (T, D), generator=gen(D + 1)).float().to(DEV)
+    ref = torch.zeros(Vr, D, device=DEV).index_put_((ids,), grad, accumulate=True)
+    assert torch.equal(ops.embed_tokens_grad(ids, grad, Vr), ref)
+    out = torch.ones(Vr, D, device=DEV)
+    assert torch.equal(ops.embed_tokens_grad(ids, grad, Vr, out=out), ref + 1)

@@ -361,7 +361,7 @@ __global__ __launch_bounds__(256) void vx_k_eg_chunks(const unsigned *__restrict
                                                       long long pitch, float *__restrict__ part1) {
     typedef typename vx_elem<GT>::type G;
     constexpr int VEC = 16 / sizeof(G);
-    const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const long long item = (long long)vx_block() * 4 + (threadIdx.x >> 6);
     const long long c1 = item / slices;
     if (c1 >= chunks) return;
     const int a = (int)c1 * VX_EG_CHUNK, c = (int)(item - c1 * slices) * VX_EG_SLICE + vx_lane() * VEC;
@@ -479,7 +479,7 @@ __device__ __forceinline__ void vx_eg_row(const vx_eg_sums &a, long long v, int 
     }
 }
 
-// Every table row: blockIdx + i * gridDim (i < 8), as frequent ids lie next to each other and go to different workgroups.
+// Every table row: block + i * blocks (i < 8), as frequent ids lie next to each other and go to different workgroups.
 // A wave sums one slice of one row.  Bound by the write of the table: few registers, so that many waves have their loads and
 // stores on the way (a version that split long rows over the waves of a workgroup held 94 instead of 62 registers: 292
 // instead of 265 us for the rows of 65536 tokens x 4096 columns bf16 over 131072).
@@ -488,16 +488,18 @@ __global__ __launch_bounds__(256) void vx_k_eg_rows(vx_eg_sums a) {
     constexpr int VEC = 16 / sizeof(typename vx_elem<GT>::type);
     __shared__ int s_at[2 * VX_EG_ROWS];
     const int lane = vx_lane(), w = threadIdx.x >> 6;
+    const long long block = vx_block(), blocks = (a.n_rows + VX_EG_ROWS - 1) / VX_EG_ROWS;
+    if (block >= blocks) return;
     {
         const int q = threadIdx.x >> 4;                           // 16 searches: the beginning and the end of 8 rows
-        const long long v = blockIdx.x + (long long)(q >> 1) * gridDim.x + (q & 1);
+        const long long v = block + (q >> 1) * blocks + (q & 1);
         const int at = vx_eg_lower_bound(a.key, a.T, (unsigned)min(v, a.n_rows));
         if ((lane & 15) == 0) s_at[q] = at;
     }
     __syncthreads();
     for (int item = w; item < VX_EG_ROWS * a.slices; item += 4) {
         const int i = item / a.slices, c = (item - i * a.slices) * VX_EG_SLICE + lane * VEC;
-        const long long v = blockIdx.x + (long long)i * gridDim.x;
+        const long long v = block + i * blocks;
         const int s = __builtin_amdgcn_readfirstlane(s_at[2 * i]), e = __builtin_amdgcn_readfirstlane(s_at[2 * i + 1]);
         if (v >= a.n_rows || (a.accumulate && s == e)) continue;
         vx_eg_row<GT, TT, U, TINY, NT>(a, v, s, e, c);
@@ -536,7 +538,7 @@ static void vx_eg_sum(const vx_eg_plan &p, const unsigned *key, const int *pos, 
     constexpr int U = vx_eg_u<GT>();
     const int slices = (int)(p.pitch / VX_EG_SLICE), slices2 = (int)(p.pitch / 256);
     if (p.chunks)
-        hipLaunchKernelGGL((vx_k_eg_chunks<GT, U, TINY>), dim3((unsigned)(((int64_t)p.chunks * slices + 3) / 4)), dim3(256), 0, st, key,
+        hipLaunchKernelGGL((vx_k_eg_chunks<GT, U, TINY>), vx_grid(((int64_t)p.chunks * slices + 3) / 4), dim3(256), 0, st, key,
                            pos, p.chunks, (unsigned)n_rows, grad, D, slices, p.pitch, part1);
     if (p.chunks2)
         hipLaunchKernelGGL(vx_k_eg_chunks2, dim3((unsigned)(((int64_t)p.chunks2 * slices2 + 3) / 4)), dim3(256), 0, st, key, p.chunks2,
@@ -547,7 +549,7 @@ static void vx_eg_sum(const vx_eg_plan &p, const unsigned *key, const int *pos, 
         hipLaunchKernelGGL((vx_k_eg_runs<GT, TT, U, TINY>), dim3((unsigned)(((int64_t)T * split + 3) / 4)), dim3(256), 0, st, a, split);
         return;
     }
-    const dim3 grid((unsigned)((n_rows + VX_EG_ROWS - 1) / VX_EG_ROWS));
+    const dim3 grid = vx_grid((n_rows + VX_EG_ROWS - 1) / VX_EG_ROWS);
     if (!TINY && !accumulate && vx_past_caches(out, n_rows, D, TT))
         hipLaunchKernelGGL((vx_k_eg_rows<GT, TT, U, TINY, !TINY>), grid, dim3(256), 0, st, a);
     else
