@@ -38,3 +38,9 @@ def test_embed_grad_of_more_rows_than_one_axis_of_a_launch(D):
     assert torch.equal(ops.embed_tokens_grad(ids, grad, Vr), ref)
     out = torch.ones(Vr, D, device=DEV)
     assert torch.equal(ops.embed_tokens_grad(ids, grad, Vr, out=out), ref + 1)
+
+
+def test_quantize_more_rows_than_one_axis_of_a_launch():
+    x = torch.arange(MANY, device=DEV, dtype=torch.float32)[:, None] - 2 ** 25
+    q, s = ops.quantize_rows_i8(x)
+    assert torch.equal(q, torch.sign(x).to(torch.int8) * 127) and torch.equal(s.cpu(), x[:, 0].cpu().abs() / 127.0)

@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256) void vx_k_quant_rows(const void *__restrict__ 
     constexpr int VEC = 16 / sizeof(E), THREADS = WAVES * 64;
     __shared__ unsigned s_max[4];
     const int w = threadIdx.x >> 6, tid = WAVES == 1 ? vx_lane() : (int)threadIdx.x;
-    const long long m = WAVES == 1 ? (long long)blockIdx.x * 4 + w : (long long)blockIdx.x;
+    const long long m = WAVES == 1 ? (long long)vx_block() * 4 + w : (long long)vx_block();
     if (m >= M) return;                                           // WAVES == 1 has no barrier behind this
     const E *row = (const E *)x + m * xs;
     unsigned top = 0;
@@ -148,11 +148,11 @@ static int vx_quant_launch(const void *x, int dtype, long long M, int K, long lo
     VX_DISPATCH_DTYPE(dtype, {
         constexpr int PIECE = 64 * 16 / (int)sizeof(typename vx_elem<DT>::type);
         if (K <= 4 * PIECE && M >= 256)
-            hipLaunchKernelGGL((vx_k_quant_rows<DT, 1, 4>), dim3((unsigned)((M + 3) / 4)), dim3(256), 0, st, x, M, K, xs, q, qs, s);
+            hipLaunchKernelGGL((vx_k_quant_rows<DT, 1, 4>), vx_grid((M + 3) / 4), dim3(256), 0, st, x, M, K, xs, q, qs, s);
         else if (K <= 8 * PIECE && M >= 256)
-            hipLaunchKernelGGL((vx_k_quant_rows<DT, 1, 8>), dim3((unsigned)((M + 3) / 4)), dim3(256), 0, st, x, M, K, xs, q, qs, s);
+            hipLaunchKernelGGL((vx_k_quant_rows<DT, 1, 8>), vx_grid((M + 3) / 4), dim3(256), 0, st, x, M, K, xs, q, qs, s);
         else
-            hipLaunchKernelGGL((vx_k_quant_rows<DT, 4, 4>), dim3((unsigned)M), dim3(256), 0, st, x, M, K, xs, q, qs, s);
+            hipLaunchKernelGGL((vx_k_quant_rows<DT, 4, 4>), vx_grid(M), dim3(256), 0, st, x, M, K, xs, q, qs, s);
     });
     vx_prof_end(VX_PROF_QUANT, st);
     return hipGetLastError() == hipSuccess ? VX_OK : VX_ERR_LAUNCH;
@@ -972,7 +972,7 @@ static int vx_linear_rows_launch(const void *x, int dtype, long long xs, long lo
 __global__ __launch_bounds__(256) void vx_k_pad_rows(const int8_t *__restrict__ src, long long stride, long long rows, int K,
                                                      int8_t *__restrict__ dst, int pitch) {
     const int pieces = pitch / 16;
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long i = (long long)vx_block() * 256 + threadIdx.x;
     if (i >= rows * pieces) return;
     const long long r = i / pieces;
     const int k = (int)(i - r * pieces) * 16;
@@ -1021,14 +1021,14 @@ static int vx_linear_launch(const int8_t *q, long long qs, bool q_padded, const 
     if (tiles) {
         if (K % 128 && !q_padded) {
             const long long n = M * (pitch / 16);
-            hipLaunchKernelGGL(vx_k_pad_rows, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, q, qs, M, K, pad, (int)pitch);
+            hipLaunchKernelGGL(vx_k_pad_rows, vx_grid((n + 255) / 256), dim3(256), 0, st, q, qs, M, K, pad, (int)pitch);
             q = pad;
             qs = pitch;
             pad += vx_up256((size_t)(M * pitch));
         }
         if (K % 16) {
             const long long n = N * (pitch / 16);
-            hipLaunchKernelGGL(vx_k_pad_rows, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, w, ws, N, K, pad, (int)pitch);
+            hipLaunchKernelGGL(vx_k_pad_rows, vx_grid((n + 255) / 256), dim3(256), 0, st, w, ws, N, K, pad, (int)pitch);
             w = pad;
             ws = pitch;
         }
