@@ -44,3 +44,23 @@ def test_quantize_more_rows_than_one_axis_of_a_launch():
     x = torch.arange(MANY, device=DEV, dtype=torch.float32)[:, None] - 2 ** 25
     q, s = ops.quantize_rows_i8(x)
     assert torch.equal(q, torch.sign(x).to(torch.int8) * 127) and torch.equal(s.cpu(), x[:, 0].cpu().abs() / 127.0)
+
+
+@pytest.mark.parametrize("with_draft", [False, True])
+def test_verify_more_chunks_than_one_axis_of_a_launch(with_draft):
+    """65535 sequences with room for 64 drafts and four chunks of logits, all on the same logits: more than 2^24 chunks of
+    rows, of which only the first sequences' and the last ones' have drafts."""
+    B, K, Vn, n = 65535, 64, 3 * 4096 + 1, 5
+    g = gen(3)
+    target, draft = torch.randn(1, K + 1, Vn, generator=g).to(DEV), torch.randn(1, K, Vn, generator=g).to(DEV)
+    tokens, u = torch.randint(0, Vn, (B, K), generator=g).to(DEV), torch.rand(B, K + 1, generator=g).to(DEV)
+    tokens[:, 0] = target[0, 0].argmax()
+    u[::2, 0] = 0.0                                               # accepted
+    lens = torch.zeros(B, dtype=torch.int32, device=DEV)
+    lens[:n], lens[-n:] = 3, 64
+    got = ops.verify_drafts(target.expand(B, K + 1, Vn), tokens, u, draft.expand(B, K, Vn) if with_draft else None, lens)
+    for part in (slice(0, n), slice(B // 2, B // 2 + n), slice(B - n, B)):
+        ref = ops.verify_drafts(target.expand(n, K + 1, Vn), tokens[part], u[part], draft.expand(n, K, Vn) if with_draft else None, lens[part])
+        assert all(torch.equal(a[part], b) for a, b in zip(got, ref)), part
+    assert int(got[1].min()) >= 1 and int(got[1].max()) >= 2 and not got[3].any()
+    assert bool((got[0][:, 0] >= 0).all()) and bool((got[0] < Vn).all())

@@ -135,8 +135,10 @@ template <int DT>
 __global__ __launch_bounds__(256) void vx_k_verify_stats(vx_verify_args a) {
     constexpr int VEC = 16 / sizeof(typename vx_elem<DT>::type), PER = VX_VERIFY_U * VEC;
     const int rows = a.draft ? 2 * a.K + 1 : a.K + 1;
-    const int item = blockIdx.x / a.chunks, chunk = blockIdx.x - item * a.chunks;
-    const int b = item / rows, j = item - b * rows, n = vx_verify_len(a, b);
+    const int item = vx_block() / a.chunks, chunk = vx_block() - item * a.chunks;
+    const int b = item / rows, j = item - b * rows;
+    if (b >= a.B) return;
+    const int n = vx_verify_len(a, b);
     const bool is_draft = j > a.K;
     const float T = vx_verify_t(a, b);
     const bool greedy = !(T > 0.f);
@@ -212,7 +214,9 @@ __global__ __launch_bounds__(256) void vx_k_verify_choose(vx_verify_args a) {
     __shared__ float s_m[2 * VX_MAX_DRAFTS + 1];
     __shared__ int s_best[VX_MAX_DRAFTS + 1];
     __shared__ u64 s_ok, s_unsure;
-    const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks, K = a.K, n = vx_verify_len(a, b);
+    const int b = vx_block() / a.chunks, chunk = vx_block() - b * a.chunks, K = a.K;
+    if (b >= a.B) return;
+    const int n = vx_verify_len(a, b);
     const int lane = vx_lane(), w = threadIdx.x >> 6;
     const float T = vx_verify_t(a, b);
     const bool greedy = !(T > 0.f), has_q = a.draft && !greedy;
@@ -445,7 +449,8 @@ template <int DT>
 __global__ __launch_bounds__(256) void vx_k_verify_rest(vx_verify_args a) {
     constexpr int CHUNK = vx_verify_chunk<DT>(), PER = VX_VERIFY_U * 16 / sizeof(typename vx_elem<DT>::type);
     __shared__ double s_sum[4];
-    const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks;
+    const int b = vx_block() / a.chunks, chunk = vx_block() - b * a.chunks;
+    if (b >= a.B) return;
     const vx_choice ch = a.choice[b];
     if (ch.mode != 3) return;
     float x[PER], y[PER];
@@ -559,9 +564,9 @@ extern "C" int vx_verify_drafts(const void *d_target, int64_t target_seq_stride,
     hipStream_t st = (hipStream_t)stream;
     vx_prof_begin(VX_PROF_VERIFY, st);
     VX_DISPATCH_DTYPE(dtype, {
-        hipLaunchKernelGGL((vx_k_verify_stats<DT>), dim3((unsigned)blocks), dim3(256), 0, st, a);
-        hipLaunchKernelGGL((vx_k_verify_choose<DT>), dim3((unsigned)(B * p.chunks)), dim3(256), 0, st, a);
-        if (d_draft) hipLaunchKernelGGL((vx_k_verify_rest<DT>), dim3((unsigned)(B * p.chunks)), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((vx_k_verify_stats<DT>), vx_grid(blocks), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((vx_k_verify_choose<DT>), vx_grid((int64_t)B * p.chunks), dim3(256), 0, st, a);
+        if (d_draft) hipLaunchKernelGGL((vx_k_verify_rest<DT>), vx_grid((int64_t)B * p.chunks), dim3(256), 0, st, a);
         hipLaunchKernelGGL((vx_k_verify_draw<DT>), dim3((unsigned)B), dim3(256), 0, st, a);
     });
     vx_prof_end(VX_PROF_VERIFY, st);
