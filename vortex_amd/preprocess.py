@@ -3,6 +3,8 @@ FlipNormalize :79-95, get_preprocess :102-121) and preprocess/__init__.py:47-55 
 `normalizer`, `normalize`, `flip_normalizer`, `flip_normalize`).  The arithmetic runs in the
 HIP kernel vx_preprocess_u8hwc_f32nchw; same constructor arguments, buffers, annotations and
 assertions as the reference."""
+from typing import Optional
+
 import torch
 import torch.nn as nn
 
@@ -63,22 +65,29 @@ class FlipNormalize(Normalize):
 
 class _EmbedTokens(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, ids, weight, scale):
+    def forward(ctx, ids, weight, scale, status):
         ctx.save_for_backward(ids)
         ctx.n_rows, ctx.scale = weight.size(0), scale
-        return ops.embed_tokens(ids, weight, scale)
+        return ops.embed_tokens(ids, weight, scale, status)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         ids, = ctx.saved_tensors
-        return None, ops.embed_tokens_grad(ids, grad, ctx.n_rows, ctx.scale), None
+        return None, ops.embed_tokens_grad(ids, grad, ctx.n_rows, ctx.scale), None, None
 
 
 class TokenEmbedding(nn.Module):
     """The pre-process of a token model: integer ids -> the network's input vectors, scale * weight[ids] (what Normalize
     is for images).  An id below 0 is padding: a row of zeros that gets no gradient.  The gradient of `weight` is summed in
     fp32 over the tokens in a fixed order (vx_embed_tokens_grad), dense, in the type of `weight`.
+
+    An id at or beyond n_rows gives zeros and no gradient as well, since a call does not wait for the GPU to say so.  Where such ids
+    can occur, hand over a word for them and look at it when the host waits anyway:
+
+        status = torch.zeros(1, dtype=torch.int32, device=ids.device)
+        h = embed(ids, status=status)
+        ops.raise_on_status(int(status))               # VortexHipError; VX_STATUS_BAD_TOKEN is ORed in, nothing clears it
 
     In a captured HIP graph, take the gradient with torch.autograd.grad: a captured backward() accumulates into `weight.grad`
     on the stream of whatever eager graph of `weight` is still alive, which torch answers by ending the process."""
@@ -89,10 +98,10 @@ class TokenEmbedding(nn.Module):
         self.weight = nn.Parameter(torch.empty(n_rows, dim, dtype=dtype, device=device))
         nn.init.normal_(self.weight, std=dim ** -0.5)
 
-    def forward(self, input: torch.Tensor) -> torch.Tensor:
+    def forward(self, input: torch.Tensor, status: Optional[torch.Tensor] = None) -> torch.Tensor:
         if torch.is_grad_enabled() and self.weight.requires_grad:
-            return _EmbedTokens.apply(input, self.weight, self.scale)
-        return ops.embed_tokens(input, self.weight, self.scale)
+            return _EmbedTokens.apply(input, self.weight, self.scale, status)
+        return ops.embed_tokens(input, self.weight, self.scale, status)
 
 
 preproc_map = dict(
