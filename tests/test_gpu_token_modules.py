@@ -33,3 +33,12 @@ def test_token_embedding_refuses_a_status_that_is_no_word_on_its_device():
     for status in (torch.zeros(1, dtype=torch.int64, device=DEV), torch.zeros(1, dtype=torch.int32), torch.zeros(0, dtype=torch.int32, device=DEV), 0):
         with pytest.raises(L.VortexHipError, match="status"):
             m(ids, status=status)
+
+
+@pytest.mark.parametrize("padding", ["same", "valid"])
+def test_int8_head_of_a_1x1_convolution_whose_padding_is_none_by_name(padding):
+    conv = torch.nn.Conv2d(64, 20, 1, padding=padding).to(DEV)
+    plain = torch.nn.Conv2d(64, 20, 1).to(DEV)
+    plain.load_state_dict(conv.state_dict())
+    x = torch.randn(2, 64, 5, 7, device=DEV)
+    assert torch.equal(V.Int8Head.from_module(conv)(x), V.Int8Head.from_module(plain)(x))

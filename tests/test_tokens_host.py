@@ -133,3 +133,12 @@ def test_status_bits_become_errors():
     with pytest.raises(L.VortexHipError):
         ops.raise_on_status(L.VX_STATUS_BAD_TOKEN)
     assert not ops.status_ok(L.VX_STATUS_BAD_TOKEN) and not ops.status_ok(L.VX_STATUS_EMPTY_ROW)
+
+
+def test_int8_head_takes_1x1_convolutions_whose_padding_is_none_by_name():
+    """"same" and "valid" add nothing to a 1x1 kernel: such layers get as far as the GPU they need."""
+    for padding in ("same", "valid"):
+        with pytest.raises(L.VortexHipError, match="must live on"):
+            V.Int8Head.from_module(torch.nn.Conv2d(4, 4, 1, padding=padding))
+    with pytest.raises(RuntimeError, match="Int8Head takes"):
+        V.Int8Head.from_module(torch.nn.Conv2d(4, 4, 3, padding="same"))

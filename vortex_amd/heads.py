@@ -110,7 +110,7 @@ class Int8Head(nn.Module):
         conv = isinstance(module, nn.Conv2d)
         if conv:
             one = all(tuple(getattr(module, n)) == (1, 1) for n in ("kernel_size", "stride", "dilation"))
-            if not one or module.groups != 1 or tuple(module.padding) != (0, 0):
+            if not one or module.groups != 1 or module.padding not in ((0, 0), "same", "valid"):
                 raise RuntimeError("Int8Head takes a 1x1 convolution without stride, padding or groups, got %s" % module)
         elif not isinstance(module, nn.Linear):
             raise RuntimeError("Int8Head takes nn.Linear or a 1x1 nn.Conv2d, got %s" % type(module).__name__)
