@@ -23,13 +23,22 @@ def yolo_rows(img_size: int) -> int:
     return 3 * sum((img_size // d) ** 2 for d in (32, 16, 8))
 
 
+def _first_tensor(values):
+    for v in values:
+        if isinstance(v, (list, tuple)) and v:
+            v = v[0]
+        if torch.is_tensor(v):
+            return v
+    return None
+
+
 def _on_device(fn):
     """The library keys per-device state (LDS attributes, events, the static scratch) off HIP's CURRENT device and
     launches on the stream it is given: when the tensors live on another device than the current one, make theirs
     current for the duration of the call (a torch op would do the same).  One comparison when nothing has to change."""
     @functools.wraps(fn)
     def call(*args, **kwargs):
-        t = args[0]
+        t = args[0] if args else _first_tensor(kwargs.values())
         if isinstance(t, (list, tuple)):
             t = t[0]
         if torch.is_tensor(t) and t.is_cuda and t.device.index not in (None, torch.cuda.current_device()):
