@@ -179,7 +179,8 @@ __device__ __forceinline__ float vx_linear_out(int acc, float s, float sw, bool 
 // ---- few tokens: the weights stream once from memory into registers, no LDS between.
 // One workgroup per 16 NT channels, its waves share K; mfma 16x16x64 with the weights as rows: lane l holds 16 bytes of
 // channel l % 16 at k = 64 b + 16 (l / 16), and MT tiles of 16 tokens stand against them.  Bound by the read of the weights:
-// 131 MB in 21 us (6.2 TB/s) for one token against 32000 x 4096.
+// 131 MB in 25 us (5.3 TB/s) for one token against 32000 x 4096.  (Times in this file, where nothing else is said: a call in a
+// graph of calls, each with weights of its own, 600 MB of them in turn; the median of 9 replays.)
 __device__ __forceinline__ vx_i4 vx_i8_tail(const int8_t *row, int k, int K) {      // bytes k .. k+15, 0 from K on
     union { vx_i4 v; int8_t b[16]; } o;
     o.v = vx_i4{0, 0, 0, 0};
@@ -277,7 +278,7 @@ __global__ __launch_bounds__(1024) void vx_k_linear_stream(const int8_t *__restr
 
 // The same for one token that is quantised on the way: every workgroup does it for itself, in LDS, while its first weights are
 // coming, and then takes several tiles of 16 channels.  The loads of a tile's first weights are on their way while the waves
-// join the sums of the tile before.  32000 x 4096: 131 MB, 25 us for the whole call, against 28 in two
+// join the sums of the tile before.  32000 x 4096: 131 MB, 26 us for the whole call, against 29 in two
 // launches.
 template <int DT>
 __global__ __launch_bounds__(1024) void vx_k_linear_one(const void *__restrict__ x, const int8_t *__restrict__ w, long long ws,
@@ -366,9 +367,9 @@ __global__ __launch_bounds__(1024) void vx_k_linear_one(const void *__restrict__
     }
 }
 
-// Which single tokens go this way (us in a graph, this / quantise and stream; bf16): 1000 x 512 4/7, 4096 x 4096 7/10,
-// 8192 x 8192 16/19, 32000 x 1024 9/13, 32000 x 4096 25/28; beyond two tiles a workgroup the next kernel is faster
-// (50021 x 1000 17/13, 4000 49/40; 65536 x 512 10.6/9.6).
+// Which single tokens go this way (us, this / quantise and stream; bf16): 1000 x 512 3.7/6.7, 4096 x 4096 7.7/10.1,
+// 8192 x 8192 17/20, 32000 x 1024 10/13, 32000 x 4096 26/29; beyond two tiles a workgroup the next kernel is faster (this / the
+// next: 50021 x 1000 17/14, 50021 x 4000 49/40, 65536 x 512 13/11; 32000 x 4096 26/27).
 #define VX_ONE_MAX_N 32768
 #define VX_ONE_MAX_K 32768
 static bool vx_linear_by_one(int64_t M, int64_t N, int K) { return M == 1 && N <= VX_ONE_MAX_N && K <= VX_ONE_MAX_K; }
@@ -410,7 +411,7 @@ __device__ __forceinline__ void vx_store4(void *out, long long at, const float y
 // its waves take tiles of 16 channels, the first weights of each on their way since the tile before.  With fewer than 16 tiles
 // a compute unit 2 to 16 waves share a tile's K and join their sums in LDS.  Rows in LDS are an odd number of 16-byte pieces
 // long: 16 of them lie in all banks.  Bound by the read of the weights and, with more tokens, of LDS:
-// 37 x 50021 x 1000 fp16 to fp32 in 18 us of the whole call (57 MB), where quantising to memory and streaming took 26.
+// 37 x 50021 x 1000 bf16 in 21 us of the whole call (54 MB), where quantising to memory first takes 24.
 #define VX_SRC_I8 3                                               // the tokens come quantised, with their scales
 template <int SRC, int MT, int UN>
 __global__ __launch_bounds__(1024) void vx_k_linear_few(const void *__restrict__ x, long long xs, const float *__restrict__ s, int M,
@@ -600,15 +601,19 @@ static size_t vx_few_lds(int64_t M, int64_t N, int K) {
 }
 #define VX_FEW_MAX 64
 static bool vx_few_fits(int64_t M, int64_t N, int K) { return M <= VX_FEW_MAX && vx_few_lds(M, N, K) <= 160 * 1024 - 512; }
-// Which products with quantisation go this way (us in a graph, this / quantise and multiply; bf16): every workgroup quantises all
-// M x K values, which costs it what the saved launch cost at about 32768 of them (65536 where the tiles would copy an odd K):
-//   32000 x 4096, M = 4: 27/29, 8: 29/33    4096 x 4096, M = 4: 9/10, 8: 10/10, 16: 12/11    8192 x 8192, M = 4: 18/19, 8: 21/20
-//   131072 x 2048, M = 16: 56/59, 32: 63/62    1000 x 512, M = 64: 9/12    16384 x 1024, M = 32: 11/12, 64: 16/12
-//   50021 x 1000, M = 32: 18/29, 64: 25/38
+// Which products with quantisation go this way (us, this / quantise and multiply; bf16): every workgroup quantises all M x K values,
+// which costs it what the saved launch cost at about 32768 of them:
+//   32000 x 4096, M = 4: 28/29, 8: 29/30    4096 x 4096, M = 4: 10/11, 8: 11/11, 16: 13/11    8192 x 8192, M = 4: 19/20, 8: 22/21
+//   131072 x 2048, M = 16: 55/56, 32: 60/58    16384 x 1024, M = 32: 11/12, 64: 16/13
+// With K not a multiple of 16 the quantised tokens would not go by tiles but by this kernel (more than 16384 channels) or the
+// streaming one, both slower at odd addresses, and it is about 65536 (with few channels less, where neither is far behind):
+//   50021 x 1000, M = 32: 19/22, 37: 21/24, 64: 25/27    16000 x 1000, M = 64: 17/18    16000 x 1500, M = 40: 18/19
+//   4096 x 1001, M = 33: 10/11    4096 x 1000, M = 64: 13/12    8192 x 600, M = 64: 14/12    12000 x 1023, M = 64: 24/22
+//   8192 x 8201, M = 5: 31/33    32000 x 5000, M = 8: 37/37    32000 x 4001, M = 16: 51/50    32000 x 2001, M = 32: 32/32
 static bool vx_linear_by_few(int64_t M, int64_t N, int K) { return vx_few_fits(M, N, K) && M * K <= (K % 16 ? 65536 : 32768); }
-// Which products of quantised tokens: many channels, and few tokens or an odd K (this / streaming or tiles):
-//   32000 x 4096, M = 1: 26/26, 4: 25/26, 8: 26/29, 16: 26/31    131072 x 2048, M = 1: 49/45, 8: 50/56, 16: 54/55, 32: 58/57
-//   50021 x 1000, M = 4: 14/16, 16: 15/21, 37: 19/29, 64: 22/36    4096 x 4096, M = 8: 7/6.5    16384 x 1024, M = 16: 7/7
+// Which products of quantised tokens: many channels, and few tokens or K not a multiple of 16 (us, this / streaming or tiles):
+//   32000 x 4096, M = 4: 26/26, 8: 26/30, 16: 27/32    131072 x 2048, M = 1: 47/46, 8: 50/56, 16: 52/53, 32: 55/54
+//   50021 x 1000, M = 4: 15/18, 16: 15/22, 37: 20/34, 64: 23/43    4096 x 4096, M = 8: 7.7/6.7    16384 x 1024, M = 16: 7/7
 static bool vx_i8_by_few(int64_t M, int64_t N, int K) { return M > 1 && N > 16384 && (M <= 16 || K % 16) && vx_few_fits(M, N, K); }
 
 template <int SRC>
@@ -632,8 +637,8 @@ static void vx_few_launch(const void *x, long long xs, const float *s, int M, co
 // reads stage d any more.
 // The 16-byte pieces of an LDS row are stored at piece ^ ((row >> 1) & 7), so the 16 rows that a quarter of a wave's 16-byte
 // LDS read covers lie in all 64 banks.
-// 8192 x 16384 x 4096: 500 us, 2.2 PFLOP/s of int8; the matrix instructions are busy 57 % of the cycles, at a clock that the
-// card has brought down to 1.7 GHz.
+// 8192 x 16384 x 4096: 508 us (the kernel's median), 2.16 Pop/s; the matrix instructions are busy 58 % of the cycles (counted), at a
+// clock that the card has brought down to 1.8 GHz.
 // Needs 16-byte aligned rows; q padded with zeros to a multiple of 128, w's pieces beyond K read as piece 0 (K % 16 == 0).
 template <int N>
 __device__ __forceinline__ void vx_wait_stage() {                 // at most N loads and no LDS read outstanding, then the barrier
@@ -946,9 +951,9 @@ __global__ __launch_bounds__(1024) void vx_k_linear_rows(const void *__restrict_
     }
 }
 
-// Which products with quantisation go this way (us of the whole call, this / quantise and multiply; N = 255, x fp32):
-// M = 43264: K = 256 26/39, 512 31/44, 1024 54/67; M = 8192: 16/18, 15/17, 20/19; M = 65: 15/17.  At M = 1 it is
-// 11 us of kernel time against 7 (the weights take longer to arrive than to be used).  N = 64 behaves alike.
+// Which products with quantisation go this way (us, this / quantise and multiply; N = 255, x fp32):
+// M = 43264: K = 256 23/39, 512 31/48, 1024 54/69; M = 8192: 8/13, 11/16, 20/19; M = 65: 5/8, 7/8, 12/10 (the weights take longer to
+// arrive than to be used; called one by one, 15/17, the saved launch is worth more).  N = 64 behaves alike.
 #define VX_STREAM_MAX 64
 #define VX_ROWS_MAX_K 1024
 static bool vx_linear_by_rows(int64_t M, int64_t N, int K) {
@@ -980,16 +985,15 @@ __global__ __launch_bounds__(256) void vx_k_pad_rows(const int8_t *__restrict__ 
     *(vx_i4 *)(dst + r * pitch + k) = k + 16 <= K ? (vx_i4)*(const vx_i4_at1 *)(row + k) : vx_i8_tail(row, k, K);
 }
 
-// Which kernel takes M tokens (us of the product alone; N x K, weights from memory), streaming / 64 x 64 tiles:
-//   M <= 8: streaming (32000 x 4096: 30/33)
-//   M <= 16: streaming up to 16384 channels (4096 x 4096 7/12, 12000 x 2048 8.4/8.7, 16000 x 4096 18/20)
-//   M <= 32: streaming up to 10240 channels (M = 32: 4096 x 4096 11/13, 8192 x 4096 13/17, but 12000 x 2048 11/9, 16000 x 4096 23/20;
-//            M = 64: 4096 x 4096 16/13, 8192 x 1024 9/7, 8192 x 4096 17/17, 8192 x 8192 30/32)
-//   M <= 64: streaming with an odd K, which the tiles would have to copy
+// Which kernel takes M quantised tokens (us of the product, N x K), streaming / 64 x 64 tiles:
+//   M <= 8: streaming (16000 x 4096: 18/22, 4096 x 4096 7/17)
+//   M <= 16: streaming up to 16384 channels (4096 x 4096 8/17, 12000 x 2048 9/11, 16000 x 4096 19/20)
+//   M <= 32: streaming up to 10240 channels (M = 32: 4096 x 4096 13/17, 8192 x 4096 15/18, but 12000 x 2048 13/11, 16000 x 4096 23/21;
+//            M = 64: 4096 x 4096 17/17, 8192 x 1024 9/7, 8192 x 4096 19/18, 8192 x 8192 31/32)
+//   M <= 64: streaming with K not a multiple of 16, which the tiles would have to copy (5000 x 1000, M = 64: 9/16)
 //   more: the largest tile that is at least half full of tokens and gives at least 192 workgroups, three for four compute
-//   units (32000 x 4096, M = 64: 34 by 64 against 37 by 128; M = 96: 44 against 38.  8192 x 4096: M = 1536, 192 tiles
-//   of 256: 54 against 60 by 128; M = 1024, 128 tiles: 48 against 41.  8192 x 8192, M = 128, 64 tiles of 128: 43 against 33 by
-//   64; M = 512, 256 tiles: 47 against 58)
+//   units (by 64 / 128 / 256.  32000 x 4096: M = 64 32/35/55, 96 40/39/55, 384 99/70/67.  8192 x 4096: M = 1024, 128 tiles of
+//   256, 63/42/57; M = 1536, 192 of them, 87/66/61.  8192 x 8192: M = 128, 64 tiles of 128, 45/56/94; M = 512, 256 of them, 65/58/97)
 static bool vx_linear_streams(int64_t M, int64_t N, int K) {
     return vx_i8_by_few(M, N, K) || M <= 8 || (M <= 16 && N <= 16384) || (M <= 32 && N <= 10240) || (M <= VX_STREAM_MAX && K % 16);
 }

@@ -130,7 +130,7 @@ __device__ __forceinline__ void vx_verify_load(const typename vx_elem<DT>::type 
 }
 
 // One workgroup per (sequence, row, chunk): target rows 0..K, then draft rows 0..K-1.  Each wave leaves its own statistics: no
-// barrier between a workgroup's loads and its end (185 MB in 29 us at 64 x 11 rows of 131072 bf16).
+// barrier between a workgroup's loads and its end (185 MB in 32 us at 64 x 11 rows of 131072 bf16).
 template <int DT>
 __global__ __launch_bounds__(256) void vx_k_verify_stats(vx_verify_args a) {
     constexpr int VEC = 16 / sizeof(typename vx_elem<DT>::type), PER = VX_VERIFY_U * VEC;
