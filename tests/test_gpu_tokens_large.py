@@ -1,4 +1,5 @@
-"""Token-model operators at sizes whose launches have more than 2^24 workgroups: HIP takes fewer than 2^32 threads along an axis."""
+"""Token-model operators at the largest sizes: launches of more than 2^24 workgroups (HIP takes fewer than 2^32 threads along an axis),
+the most tokens and channels of the 8-bit product."""
 import pytest
 import torch
 
@@ -64,3 +65,36 @@ def test_verify_more_chunks_than_one_axis_of_a_launch(with_draft):
         assert all(torch.equal(a[part], b) for a, b in zip(got, ref)), part
     assert int(got[1].min()) >= 1 and int(got[1].max()) >= 2 and not got[3].any()
     assert bool((got[0][:, 0] >= 0).all()) and bool((got[0] < Vn).all())
+
+
+MOST = 4194240                                  # tokens or channels of the 8-bit product
+
+
+def check_product(q, s, qw, sw, got, two):
+    """Few enough terms that fp32 sums them exactly; the scales and the product as the operator rounds them.  In pieces: the library's
+    product leaves a result from its 2 GiB on at 0."""
+    for a in range(0, got.size(0), 1 << 18):
+        for b in range(0, got.size(1), 1 << 20):
+            r, c = slice(a, a + (1 << 18)), slice(b, b + (1 << 20))
+            ref = (q[r].float() @ qw[c].float().t().contiguous()) * (s[r, None] * sw[None, c])
+            assert torch.equal(got[r, c], ref) and torch.equal(two[r, c], ref), (a, b)
+
+
+@pytest.mark.parametrize("M", [1, 3, 40, 200])
+def test_linear_most_channels(M):
+    K, g = 16, gen(M)
+    x, sw = torch.randn(M, K, generator=g).to(DEV), torch.rand(MOST, generator=g).to(DEV)
+    qw = torch.randint(-128, 128, (MOST, K), generator=g, dtype=torch.int8).to(DEV)
+    q, s = ops.quantize_rows_i8(x)
+    check_product(q, s, qw, sw, ops.linear_w8a8(x, qw, sw), ops.linear_i8(q, s, qw, sw))
+
+
+@pytest.mark.parametrize("N,odd", [(20, 0), (20, 1), (300, 0)])
+def test_linear_most_tokens(N, odd):
+    """Few channels (the weights stay on the chip), tiles, and with weights at an odd address the streaming kernel, 64 tokens a workgroup."""
+    K, g = 16, gen(N)
+    x, sw = torch.randn(MOST, K, generator=g).to(DEV), torch.rand(N, generator=g).to(DEV)
+    flat = torch.randint(-128, 128, (N * K + odd,), generator=g, dtype=torch.int8).to(DEV)
+    qw = flat[odd:].view(N, K)
+    q, s = ops.quantize_rows_i8(x)
+    check_product(q, s, qw, sw, ops.linear_w8a8(x, qw, sw), ops.linear_i8(q, s, qw, sw))
