@@ -388,9 +388,10 @@ int vx_linear_w8a8(const void *d_x, int x_dtype, int64_t x_stride, int64_t M, co
  *   the token behind them is the first i with sum_{i' <= i} r_i' > u_{b,K} sum r, r = max(0, p_n - q_n) when x_n was
  *   rejected, r = p_n when n = n_b
  *   d_tokens[b,0..n) = x_0 .. x_{n-1}, d_tokens[b,n] = that token, -1 behind it; d_counts[b] = n + 1
- * T_b = d_temperature[b], or `temperature` for every sequence where d_temperature is NULL.  Not above 0: greedy -- x_j is accepted iff it is the first arg-max of target row j (d_accept 1 or 0), the
- * token behind is the arg-max of row n; the draft logits and d_uniforms are not used.  d_uniforms [B, K+1] in [0, 1); a d_uniforms[b,K] that is not below 1
- * draws the last token with r > 0.
+ * T_b = d_temperature[b], or `temperature` for every sequence where d_temperature is NULL.  Not above 0: greedy -- x_j is
+ * accepted iff it is the first arg-max of target row j (d_accept 1 or 0), the token behind is the arg-max of row n; the draft
+ * logits and d_uniforms are not used.  d_uniforms [B, K+1] in [0, 1); a d_uniforms[b,K] that is not below 1 draws the last token
+ * with r > 0.
  * -inf masks a token (in either distribution); other logits of a row differ by less than FLT_MAX.  K = 0 draws one token from
  * each row 0.
  * The drawn token and every accepted / rejected are decided in fp64 from the logits on; d_accept is within 2^-15 relative, and
